@@ -1,5 +1,6 @@
 """ctypes binding of libdejavu_b200.so (declared in include/dejavu_b200.h), libdejavu_b200_hybrid.so
-(include/dejavu_b200_hybrid.h) and libdejavu_b200_routed.so (include/dejavu_b200_routed.h).
+(include/dejavu_b200_hybrid.h), libdejavu_b200_routed.so (include/dejavu_b200_routed.h) and libdejavu_b200_serving.so
+(include/dejavu_b200_serving.h).
 
 The libraries are the only compute path of this package: if one is missing the import of any operator
 raises, there is no PyTorch or CPU fallback.
@@ -13,6 +14,7 @@ PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libdejavu_b200.so"
 HYBRID_LIB_PATH = PKG / "libdejavu_b200_hybrid.so"
 ROUTED_LIB_PATH = PKG / "libdejavu_b200_routed.so"
+SERVING_LIB_PATH = PKG / "libdejavu_b200_serving.so"
 
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_CUDA, ERR_SCRATCH, ERR_TIMEOUT = 0, -1, -2, -3, -4, -5
 ACT = {"id": 0, "relu": 1, "gelu": 2, "gelu_approx": 3, "squared_relu": 4, "softcap": 5, "clamped_glu": 6, "silu_glu": 7}
@@ -136,6 +138,19 @@ ROUTED_SIGNATURES = {
     "djv_moe_timeouts": (C.c_uint, []),
 }
 
+# mirrors include/dejavu_b200_serving.h one to one
+SERVING_SIGNATURES = {
+    "djv_paged_append": (_i, [_i, _vp, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _ll, _i, _i, _vp, _ll,
+                              _i, _vp, _vp, _vp, _f, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    "djv_paged_attention_scratch_bytes": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "djv_paged_attention": (_i, [_i, _vp, _vp, _ll, _ll, _vp, _vp, _ll, _ll, _ll, _i, _i, _vp, _ll, _i, _vp, _i, _i, _i, _i, _f, _vp,
+                                 _sz, _vp]),
+    "djv_paged_faults": (C.c_uint, []),
+    "djv_packed_attention": (_i, [_i, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _i, _i, _i, _i, _f, _i, _vp]),
+    "djv_sample": (_i, [_i, _vp, _vp, _ll, _vp, _vp, _ll, _vp, _i, _vp, _ll, _vp, _ll, _i, _i, _vp]),
+}
+_TABLES = (SIGNATURES, HYBRID_SIGNATURES, ROUTED_SIGNATURES, SERVING_SIGNATURES)
+
 # functions of the hybrid header that the routed library has as well
 SHARED = ("djv_hyper_step", "djv_residual_step", "djv_dense_gemv", "djv_glu", "djv_softcap", "djv_rotary",
           "djv_window_timeouts")
@@ -146,19 +161,20 @@ _LETTERS = {_i: "i", _vp: "p", _ll: "l", _sz: "z", _f: "f"}
 
 
 def _signature(fn_name: str) -> str:
-    for table in (SIGNATURES, HYBRID_SIGNATURES, ROUTED_SIGNATURES):
+    for table in _TABLES:
         if fn_name in table:
             res, args = table[fn_name]
             return "".join(_LETTERS.get(t, "?") for t in (res, *args))
     raise AttributeError(fn_name)
 
 
-KINDS = {k: n for n, k in enumerate(sorted({_signature(f) for t in (SIGNATURES, HYBRID_SIGNATURES, ROUTED_SIGNATURES) for f in t
+KINDS = {k: n for n, k in enumerate(sorted({_signature(f) for t in _TABLES for f in t
                                             if _signature(f)[0] in "iz" and "?" not in _signature(f)}))}
 
 _lib = None
 _hybrid = None
 _routed = None
+_serving = None
 _bound: dict = {}  # function name -> what `call` and `query` call, for the libraries loaded so far
 _calls = None  # the compiled bindings, once they are there
 
@@ -203,7 +219,17 @@ def load_routed() -> C.CDLL:
     return _routed
 
 
+def load_serving() -> C.CDLL:
+    """Loads the shared library of the paged cache, its attention and sampling (once). Raises if it has not been built."""
+    global _serving
+    if _serving is None:
+        _serving = _open(SERVING_LIB_PATH, {**SERVING_SIGNATURES, **{n: SIGNATURES[n] for n in _PLUMBING}})
+    return _serving
+
+
 def _library_of(fn_name: str) -> C.CDLL:
+    if fn_name in SERVING_SIGNATURES:
+        return load_serving()
     if fn_name in ROUTED_SIGNATURES:
         return load_routed()
     if fn_name in SHARED and _hybrid is None and (_routed is not None or not HYBRID_LIB_PATH.exists()):
@@ -251,4 +277,4 @@ def query(fn_name: str, *args) -> int:
 
 def launch_count() -> int:
     """Kernels launched by the loaded libraries since load."""
-    return sum(int(lib.djv_launch_count()) for lib in (_lib, _hybrid, _routed) if lib is not None)
+    return sum(int(lib.djv_launch_count()) for lib in (_lib, _hybrid, _routed, _serving) if lib is not None)

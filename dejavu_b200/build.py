@@ -1,10 +1,11 @@
 """Builds the C-ABI libraries of sm_100a kernels in-tree with nvcc.
 
-    python -m dejavu_b200.build [--force] [--verbose] [--lib sparse|hybrid|routed]
+    python -m dejavu_b200.build [--force] [--verbose] [--lib sparse|hybrid|routed|serving]
 
   sparse  libdejavu_b200.so         the contextual-sparse OPT decode path
   hybrid  libdejavu_b200_hybrid.so  gated linear attention, sliding-window attention, hyper-connected streams
   routed  libdejavu_b200_routed.so  matrix memories, latent attention, routed feed-forwards
+  serving libdejavu_b200_serving.so paged caches, attention over pages and packed prompts, sampling
 
 Each .cu file is compiled to an object in parallel, then linked into the shared libraries that sit next to this file. Beside them
 stands _calls, a small extension module with a binding for each signature of the libraries' functions (_lib.py): a call with 17
@@ -30,13 +31,15 @@ OBJ = PKG / "build"
 LIB = PKG / "libdejavu_b200.so"
 HYBRID_LIB = PKG / "libdejavu_b200_hybrid.so"
 ROUTED_LIB = PKG / "libdejavu_b200_routed.so"
-LIBS = {"sparse": LIB, "hybrid": HYBRID_LIB, "routed": ROUTED_LIB}
+SERVING_LIB = PKG / "libdejavu_b200_serving.so"
+LIBS = {"sparse": LIB, "hybrid": HYBRID_LIB, "routed": ROUTED_LIB, "serving": SERVING_LIB}
 
 # translation units of the hybrid decoders' libraries; those both use are compiled once and linked into both
 _BOTH = ("api", "hybrid_gemv", "hybrid_residual", "hybrid_rotary", "hybrid_window_simple", "hybrid_window_prefill")
 _UNITS = {"hybrid": _BOTH + ("hybrid_attention", "hybrid_gla", "hybrid_gla_mma"),
           "routed": _BOTH + ("hybrid_mlstm", "hybrid_mlstm_prefill", "hybrid_latent", "hybrid_latent_decode", "hybrid_moe",
-                             "hybrid_moe_gemm")}
+                             "hybrid_moe_gemm"),
+          "serving": ("api", "serving_append", "serving_decode", "serving_packed", "serving_sample")}
 
 NVCC_FLAGS = [
     "-O3",
@@ -63,7 +66,7 @@ def sources(lib: str | None = None) -> list[Path]:
         return out
     if lib in _UNITS:
         return [p for p in out if p.stem in _UNITS[lib]]
-    return [p for p in out if not p.stem.startswith("hybrid_")]
+    return [p for p in out if not p.stem.startswith(("hybrid_", "serving_"))]
 
 
 CALLS = PKG / ("_calls" + sysconfig.get_config_var("EXT_SUFFIX"))

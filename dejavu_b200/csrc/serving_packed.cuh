@@ -1,0 +1,62 @@
+// Packed prompts: which rows a block takes.
+#pragma once
+#include "serving.cuh"
+
+namespace djv {
+
+struct PackedArgs {
+  void *out;
+  const void *q, *k, *v;
+  long long ldq, hq, ldk, hk, ldv, hv;
+  const int *cu;
+  int B, T, H, G, D;
+  float scale;
+  int keep_rest;
+};
+
+struct PackedTile {
+  int first, q0, rows;  // the sequence's first row, the tile's first query in it, its queries (<= 0: no tile)
+  int rest;             // 1: rows of no sequence
+};
+
+// Tiles of Q rows that B sequences of T rows in all can make, those of no sequence among them.
+template <int Q>
+inline int packed_tiles(int T, int B) { return T / Q + B + 2 < T + 2 ? T / Q + B + 2 : T + 2; }
+
+// Tile number `index`: tiles of the sequences in order, then of the rows in front of the first and behind the last. Whole warp. Whatever
+// cu holds, rows are within 0 .. T - 1.
+template <int Q>
+__device__ __forceinline__ PackedTile packed_tile(const PackedArgs &a, int index) {
+  const int lane = threadIdx.x % WARP;
+  int seen = 0;
+  for (int b0 = 0; b0 < a.B; b0 += WARP) {
+    const int b = b0 + lane;
+    int lo = 0, n = 0;
+    if (b < a.B) {
+      lo = max(0, min(a.cu[b], a.T));
+      n = max(0, min(a.cu[b + 1], a.T) - lo);
+    }
+    const int t = (n + Q - 1) / Q;
+    int s = t;
+#pragma unroll
+    for (int o = 1; o < WARP; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, s, o);
+      if (lane >= o) s += up;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, index < seen + s);
+    if (here) {
+      const int who = __ffs(here) - 1;
+      const int first = __shfl_sync(0xffffffffu, lo, who), rows = __shfl_sync(0xffffffffu, n, who);
+      const int before = seen + __shfl_sync(0xffffffffu, s - t, who), q0 = (index - before) * Q;
+      return {first, q0, min(Q, rows - q0), 0};
+    }
+    seen += __shfl_sync(0xffffffffu, s, WARP - 1);
+  }
+  const int head = max(0, min(a.cu[0], a.T)), tail = max(0, min(a.cu[a.B], a.T));
+  const int at = (index - seen) * Q;
+  const int in_head = (head + Q - 1) / Q * Q;
+  if (at < in_head) return {0, at, min(Q, head - at), 1};
+  return {tail, at - in_head, min(Q, a.T - tail - (at - in_head)), 1};
+}
+
+}  // namespace djv

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import os
+import struct
 
 from typing import Optional
 
@@ -844,3 +845,182 @@ def moe_decode(x, z, w_gu, w_down, top: int, shared_gu=None, shared_down=None, i
          w_gu.data_ptr(), w_down.data_ptr(), _ptr(shared_gu), _ptr(shared_down), _ptr(init), B, E, top, D, F, Fs, ld, stages,
          _stream())
     return y
+
+
+# ---- requests of different lengths: paged caches, packed prompts, sampling (fp16, bf16 or fp32) ------------------------------
+
+_CODES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+
+
+def _device_of(*tensors):
+    """A block in which the device of the tensors, one for all, is the current one."""
+    _require_cuda(*tensors)
+    devices = {t.device.index for t in tensors if t is not None}
+    assert len(devices) == 1, f"tensors on several devices: {sorted(devices)}"
+    device = devices.pop()
+    return contextlib.nullcontext() if device == torch._C._cuda_getDevice() else torch.cuda.device(device)
+
+
+def _one_type(*tensors) -> int:
+    dtype = tensors[0].dtype
+    assert dtype in _CODES, f"fp16, bf16 or fp32 expected, got {dtype}"
+    assert all(t is None or t.dtype == dtype for t in tensors), f"one type expected, got {[t.dtype for t in tensors if t is not None]}"
+    return _CODES[dtype]
+
+
+def _last_adjacent(t):
+    """t, or a copy of it, whose last dimension is contiguous."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _pages(k_pages, v_pages, table, pos, G: int, D: int):
+    """Checks a paged cache against what is stored in it; its arguments of the C ABI."""
+    P, heads, page, dim = k_pages.shape
+    assert (heads, dim) == (G, D) and v_pages.shape == k_pages.shape, f"pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} for {G} heads of {D}"
+    assert v_pages.stride() == k_pages.stride() and k_pages.stride(3) == 1, "K and V pages have one layout, dimensions adjacent"
+    unit = 16 // k_pages.element_size()
+    assert D % unit == 0 and all(s % unit == 0 for s in k_pages.stride()[:3]), f"rows of a page start on multiples of {unit} elements"
+    assert k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, "pages start on multiples of 16 bytes"
+    B, width = table.shape
+    assert table.dtype == torch.int32 and width >= 1 and (table.stride(1) == 1 or width == 1), "table: (B, width) int32, rows of adjacent entries"
+    assert width * page < 2 ** 31, "more than 2^31 tokens per sequence"
+    assert pos.shape == (B,) and pos.dtype == torch.int64 and pos.is_contiguous(), "pos: (B,) int64"
+    return (k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], P, page, table.data_ptr(), table.stride(0), width,
+            pos.data_ptr())
+
+
+def _cumulative(cu_seqlens) -> int:
+    assert cu_seqlens.dim() == 1 and cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.numel() >= 2, \
+        "cu_seqlens: (B + 1,) int32"
+    return cu_seqlens.numel() - 1
+
+
+def paged_append(q, k, v, k_pages, v_pages, table, pos, cu_seqlens=None, freqs=None, amp: float = 1.0, interleaved: bool = False,
+                 keys: bool = False):
+    """New tokens of B sequences enter their paged caches, rotated on the way (djv_paged_append).
+
+    k, v (T, G, D), q (T, H, D) or None: any row and head strides. k_pages, v_pages (P, G, page, D), of one layout; table (B, width)
+    int32: the page of tokens i * page ... of each sequence. cu_seqlens (B + 1,) int32: the rows cu[b] ... cu[b + 1] - 1 are tokens of
+    sequence b, from position pos[b] (int64) on; None: one row per sequence. freqs (half,) fp32: the first 2 * half dimensions of q
+    and k are rotated, pairs (i, i + half) or, interleaved, (2i, 2i + 1), cos and sin times amp; None: no rotation.
+    Returns q rotated (T, H, D), or None without q, and with `keys` the rotated k (T, G, D), for packed_attention, else None. Rows of
+    no sequence and rows at negative positions (padding of a batch) are not stored and come back as zeros. Table entries that are no
+    page are not stored to but counted (paged_faults)."""
+    T, G, D = k.shape
+    assert v.shape == k.shape and (q is None or (q.dim() == 3 and q.shape[0] == T and q.shape[2] == D)), "q (T, H, D), k and v (T, G, D)"
+    code = _one_type(k, v, q, k_pages, v_pages)
+    with _device_of(k, v, q, k_pages, v_pages, table, pos, cu_seqlens, freqs):
+        q, k, v = _last_adjacent(q), _last_adjacent(k), _last_adjacent(v)
+        pages = _pages(k_pages, v_pages, table, pos, G, D)
+        B = table.shape[0]
+        if cu_seqlens is None:
+            assert T == B, f"{T} rows of {B} sequences"
+        else:
+            assert _cumulative(cu_seqlens) == B, "cu_seqlens and table are of one batch"
+        half = 0
+        if freqs is not None:
+            _f32(freqs)
+            half = freqs.numel()
+            assert freqs.dim() == 1 and 2 * half <= D, f"{2 * half} rotary dimensions in heads of {D}"
+        H = 0 if q is None else q.shape[1]
+        q_out = None if q is None else torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(T, G, D, dtype=k.dtype, device=k.device) if keys else None
+        if T:
+            call("djv_paged_append", code, _ptr(q_out), _ptr(k_out), _ptr(q), 0 if q is None else q.stride(0),
+                 0 if q is None else q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *pages,
+                 _ptr(cu_seqlens), _ptr(freqs), float(amp), half, int(interleaved), B, T, H, G, D, _stream())
+    return q_out, k_out
+
+
+def paged_attention(q, k_pages, v_pages, table, pos, scale: float):
+    """One new token per sequence over its pages (djv_paged_attention): q (B, H, D) rotated, the sequence's tokens at positions
+    0 .. pos[b] (int64), its own among them, in k_pages, v_pages (P, G, page, D) by table (B, width) int32; H a multiple of G, D at
+    most 256. Returns (B, H, D). A sequence at position -1 gets zeros; table entries that are no page are not seen and counted
+    (paged_faults)."""
+    B, H, D = q.shape
+    G = k_pages.shape[1]
+    assert H >= 1 and H % G == 0, f"{H} query heads over {G} key/value heads"
+    assert D <= 256, f"heads of {D}"
+    assert table.shape[0] == B, "q and table are of one batch"
+    code = _one_type(q, k_pages, v_pages)
+    with _device_of(q, k_pages, v_pages, table, pos):
+        unit = 16 // q.element_size()
+        if q.stride(2) != 1 or q.stride(0) % unit or q.stride(1) % unit or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+        pages = _pages(k_pages, v_pages, table, pos, G, D)
+        out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
+        if B:
+            need = query("djv_paged_attention_scratch_bytes", code, B, H, G, D, k_pages.shape[2], table.shape[1])
+            scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # (one for each call: captured ones keep theirs)
+            call("djv_paged_attention", code, out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), *pages, B, H, G, D, float(scale),
+                 _ptr(scratch), need, _stream())
+    return out
+
+
+def paged_faults() -> int:
+    """Table entries and positions that paged_append and paged_attention refused since load, on the current device (synchronises)."""
+    return int(_lib.load_serving().djv_paged_faults())
+
+
+def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
+    """Causal attention over whole prompts, packed row after row (djv_packed_attention): rows cu[b] .. cu[b + 1] - 1 of q (T, H, D), k
+    and v (T, G, D) are sequence b, cu_seqlens (B + 1,) int32. H a multiple of G, D at most 256; any row and head strides. Returns
+    (T, H, D). Rows of no sequence are zeros or, with `out` given (T, H, D, contiguous), left as they are."""
+    T, H, D = q.shape
+    G = k.shape[1]
+    assert k.shape == v.shape == (T, G, D) and G >= 1, "q (T, H, D), k and v (T, G, D)"
+    assert H >= 1 and H % G == 0, f"{H} query heads over {G} key/value heads"
+    assert 1 <= D <= 256, f"heads of {D}"
+    B = _cumulative(cu_seqlens)
+    code = _one_type(q, k, v, out)
+    with _device_of(q, k, v, cu_seqlens, out):
+        q, k, v = _last_adjacent(q), _last_adjacent(k), _last_adjacent(v)
+        keep = out is not None
+        if keep:
+            assert out.shape == (T, H, D) and out.is_contiguous(), "out (T, H, D), contiguous"
+        else:
+            out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
+        if T:
+            call("djv_packed_attention", code, out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+                 v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens.data_ptr(), B, T, H, G, D, float(scale), int(keep), _stream())
+    return out
+
+
+def _bits(x: float) -> int:
+    """The bits of a 64-bit number, as the C ABI takes it."""
+    return struct.unpack("q", struct.pack("d", x))[0]
+
+
+def _setting(name: str, value, dtype, B: int, device):
+    """A setting of sample_tokens: (array or None, number)."""
+    if not torch.is_tensor(value):
+        return None, value
+    assert value.shape == (B,) and value.dtype == dtype and value.is_contiguous(), f"{name}: a number or ({B},) {dtype}"
+    assert value.device == device, f"{name} on {value.device}, logits on {device}"
+    return value.data_ptr(), 0
+
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token per row of logits (B, V), fp16, bf16 or fp32, from given numbers uniform (B,) fp32 in [0, 1) (djv_sample). Of the
+    entries that are neither -inf nor NaN, largest first and equal ones by index, the first top_k are kept (0: all), of those the
+    ones in front of which less than top_p of their weight lies (1: all), of those the ones with at least min_p of the largest
+    weight; weights are exp(logit / temperature). The token is the lowest index at which the running weight of what is kept exceeds
+    uniform times its total. temperature 0: the largest entry. Each setting is a number or a tensor (B,) on the device (top_k int32,
+    the others fp32). Returns (B,) int64, -1 for a row without entries."""
+    assert logits.dim() == 2 and logits.shape[1] >= 1, f"logits (B, V), got {tuple(logits.shape)}"
+    B, V = logits.shape
+    code = _one_type(logits)
+    assert uniform.shape == (B,) and uniform.dtype == torch.float32 and uniform.is_contiguous(), f"uniform ({B},) fp32"
+    with _device_of(logits, uniform):
+        if logits.stride(1) != 1 or logits.stride(0) < V:
+            logits = logits.contiguous()
+        dev = logits.device
+        t, t_all = _setting("temperature", temperature, torch.float32, B, dev)
+        k, k_all = _setting("top_k", top_k, torch.int32, B, dev)
+        p, p_all = _setting("top_p", top_p, torch.float32, B, dev)
+        m, m_all = _setting("min_p", min_p, torch.float32, B, dev)
+        token = torch.empty(B, dtype=torch.int64, device=dev)
+        if B:
+            call("djv_sample", code, token.data_ptr(), logits.data_ptr(), max(logits.stride(0), V), uniform.data_ptr(), t, _bits(t_all), k,
+                 min(int(k_all), 2 ** 31 - 1), p, _bits(p_all), m, _bits(m_all), B, V, _stream())
+    return token
