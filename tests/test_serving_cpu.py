@@ -99,7 +99,7 @@ def test_operators_refuse_tensors_of_the_cpu():
 
 
 def compiled(tmp_path, body):
-    (tmp_path / "t.cpp").write_text(f'#include "{ROOT}/dejavu_b200/csrc/serving_plan.cuh"\n#include <stdio.h>\n#include <limits.h>\n'
+    (tmp_path / "t.cpp").write_text(f'#include "{ROOT}/dejavu_b200/csrc/serving_plan.cuh"\n#include <stdio.h>\n#include <limits.h>\n#include <initializer_list>\n'
                                     "#define CHECK(c) if (!(c)) { printf(\"%s line %d\\n\", #c, __LINE__); return 1; }\nusing namespace djv;\n"
                                     "int main() {\n" + body + "\nreturn 0;\n}\n")
     subprocess.run([shutil.which("g++"), "-std=c++17", "-O1", "-fsanitize=address,undefined", str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")],
