@@ -39,7 +39,8 @@ _BOTH = ("api", "hybrid_gemv", "hybrid_residual", "hybrid_rotary", "hybrid_windo
 _UNITS = {"hybrid": _BOTH + ("hybrid_attention", "hybrid_gla", "hybrid_gla_mma"),
           "routed": _BOTH + ("hybrid_mlstm", "hybrid_mlstm_prefill", "hybrid_latent", "hybrid_latent_decode", "hybrid_moe",
                              "hybrid_moe_gemm"),
-          "serving": ("api", "serving_append", "serving_decode", "serving_packed", "serving_sample")}
+          "serving": ("api", "serving_append", "serving_decode", "serving_packed", "serving_packed_tc",
+                      "serving_sample")}
 
 NVCC_FLAGS = [
     "-O3",

@@ -5,11 +5,10 @@
 // rows of the next one that a tile's load brings along are not stored). Roles: one thread issues TMA loads into a ring of
 // stages, one thread issues the products into one of two accumulators in TMEM, four warps store the other one. Tiles of one
 // expert that share weight columns are neighbours, so they meet in L2.
-#include <cuda.h>
-
 #include "../../include/dejavu_b200_routed.h"
 #include "hybrid_moe.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.cuh"
 
 namespace djv {
 
@@ -19,9 +18,6 @@ constexpr int MG_MAX_EXPERTS = 1024;
 
 __device__ unsigned g_moe_timeouts;  // bounded waits that ran out (never, in a healthy run)
 
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 // a box of the tensor map at (element x, row y) into this block's shared memory
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
   asm volatile(
@@ -206,24 +202,6 @@ moe_grouped_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_co
     tmem_fence_after();
     tmem_dealloc(tm, 2 * BN);
   }
-}
-
-using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiled encode_tiled() {
-  static const EncodeTiled fn = [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess) {
-      cudaGetLastError();
-      p = nullptr;
-    }
-    return reinterpret_cast<EncodeTiled>(p);
-  }();
-  return fn;
 }
 
 // rows x cols of bf16, boxes of 64 columns with the 128-byte swizzle, zeros outside

@@ -12,6 +12,7 @@
 // behind its scores, K of the next one behind the values' products.
 #include "../../include/dejavu_b200_hybrid.h"
 #include "hybrid_attention.cuh"
+#include "pairs.cuh"
 #include "tcgen05.cuh"
 
 #include <type_traits>
@@ -22,37 +23,6 @@ constexpr int WP_THREADS = 256;
 constexpr int WP_TILE = 128;  // queries per block, keys per tile
 
 __device__ unsigned g_window_timeouts;  // bounded waits that ran out (never, in a healthy run)
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// pairs of floats: one instruction for two
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 
 template <int KB, int VB>  // 64-element blocks of a query/key row and of a value row
 __global__ void __launch_bounds__(WP_THREADS, VB > 2 ? 1 : 2) window_prefill_kernel(WindowArgs a) {

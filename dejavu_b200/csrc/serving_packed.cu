@@ -150,6 +150,7 @@ extern "C" int djv_packed_attention(int dtype, void *out, const void *q, long lo
   if (T == 0) return DJV_OK;
   const PackedArgs a{out, q, k, v, ldq, hq, ldk, hk, ldv, hv, cu, B, T, H, G, D, scale, keep_rest};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (packed_tc_supported(dtype, a)) return packed_tc(dtype, a, st);
   const cudaError_t e = dtype == DJV_DTYPE_F16    ? launch_packed_simple<__half>(a, st)
                         : dtype == DJV_DTYPE_BF16 ? launch_packed_simple<bf16>(a, st)
                                                   : launch_packed_simple<float>(a, st);

@@ -14,6 +14,10 @@ struct PackedArgs {
   int keep_rest;
 };
 
+// the tensor-core form: fp16 and bf16, rows that TMA can read
+bool packed_tc_supported(int dtype, const PackedArgs &a);
+int packed_tc(int dtype, const PackedArgs &a, cudaStream_t st);
+
 struct PackedTile {
   int first, q0, rows;  // the sequence's first row, the tile's first query in it, its queries (<= 0: no tile)
   int rest;             // 1: rows of no sequence

@@ -1,7 +1,7 @@
 // The 5th-generation tensor cores: shared-memory operand tiles, TMEM, and the instructions a block needs to run
 // matrix products with accumulators (and, where wanted, the A operand) in TMEM. One-block form (cta_group::1) only.
 //
-// Operand tiles are bf16 with 128-byte rows of 64 elements and the 128-byte swizzle: element (row, e) of a tile sits in
+// Operand tiles are bf16 or fp16 with 128-byte rows of 64 elements and the 128-byte swizzle: element (row, e) of a tile sits in
 // block e / 64 (blocks are rows * 128 bytes apart), row `row`, 16-byte chunk (e % 64 / 8) ^ (row % 8). The same bytes
 // serve as
 //   a K-major operand:  rows = M or N, elements along K     (scores: q and k rows)
@@ -31,9 +31,9 @@ __device__ __forceinline__ uint64_t desc_k_major(uint32_t tile, int rows, int k1
 __device__ __forceinline__ uint64_t desc_mn_major(uint32_t tile, int rows, int k16) {
   return sw128_desc(tile + (uint32_t)k16 * 2048, (uint32_t)rows * 128, 1024);
 }
-// Instruction descriptor: fp32 accumulators, bf16 operands, M x N
-__host__ __device__ constexpr uint32_t mma_idesc(int M, int N, bool a_mn_major, bool b_mn_major) {
-  return 1u << 4 | 1u << 7 | 1u << 10 | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) |
+// Instruction descriptor: fp32 accumulators, bf16 (or fp16) operands, M x N
+__host__ __device__ constexpr uint32_t mma_idesc(int M, int N, bool a_mn_major, bool b_mn_major, bool fp16 = false) {
+  return 1u << 4 | (fp16 ? 0u : 1u << 7 | 1u << 10) | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) |
          (uint32_t)(N >> 3) << 17 | (uint32_t)(M >> 4) << 24;
 }
 

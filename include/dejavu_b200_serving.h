@@ -60,6 +60,8 @@ unsigned djv_paged_faults(void);
 int djv_packed_attention(int dtype, void *out, const void *q, long long ldq, long long hq, const void *k, long long ldk, long long hk,
                          const void *v, long long ldv, long long hv, const int32_t *cu, int B, int T, int H, int G, int D, float scale,
                          int keep_rest, void *stream);
+/* Waits of the tensor-core kernel on its own copies and products that ran out since load (0 in a healthy process; synchronises). */
+unsigned djv_packed_timeouts(void);
 
 /* One token per row of logits (B, V), rows ld elements apart, from a given number u[b] in [0, 1) (fp32). Of the entries that are neither
  * -inf nor NaN, ordered by (logit descending, index ascending), with w_i = exp((x_i - max) / temperature), are kept
