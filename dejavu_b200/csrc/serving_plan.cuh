@@ -32,4 +32,23 @@ DJV_HOST_DEVICE int sequence_of(const int *cu, int B, int t) {
   return lo;
 }
 
+// How the cached tokens of a batch are dealt out to blocks: sequence b of n tokens is `share` items (key/value heads times groups of
+// query heads), each of units_of(n) units of DECODE_UNIT tokens, an empty one of a unit too. All units stand in a row, sequence by
+// sequence and item by item, and every block takes `per` of them, so that an item may begin in one block and end in another.
+constexpr int DECODE_UNIT = 64;
+DJV_HOST_DEVICE long long units_of(long long tokens) { return tokens <= 0 ? 1 : (tokens + DECODE_UNIT - 1) / DECODE_UNIT; }
+DJV_HOST_DEVICE long long units_per_block(long long units, int blocks, int least) {
+  const long long per = (units + blocks - 1) / blocks;
+  return per < least ? least : per;
+}
+// Part of an item that a block has: units from .. to - 1 of the item (to > from).
+struct DecodePart {
+  long long item, from, to;  // item: within its sequence
+};
+// The part that begins at unit x, for a block whose units end before `end`; base: the sequence's first unit, units: of one of its items.
+DJV_HOST_DEVICE DecodePart decode_part(long long x, long long end, long long base, long long units) {
+  const long long item = (x - base) / units, from = x - base - item * units, left = end - x;
+  return {item, from, from + left < units ? from + left : units};
+}
+
 }  // namespace djv

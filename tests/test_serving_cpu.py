@@ -68,7 +68,7 @@ def sample(lib, dtype=2, logits=P, ld=100, t=1.0, k=0, p=1.0, m=0.0, B=2, V=100)
              {"half": 33}, {"half": -1}, {"B": 0}, {"T": 3}, {"T": -1}, {"H": 0}, {"G": 0}, {"D": 60}, {"D": 0}, {"D": 4096},
              {"page": 1 << 20, "width": 1 << 12}],
     attend: [{"dtype": -1}, {"q": None}, {"q": P + 4}, {"ldq": 257}, {"pages_at": P + 2}, {"H": 5}, {"H": 0}, {"D": 264}, {"D": 12}, {"B": -1},
-             {"B": 70000}, {"scale": float("nan")}, {"scale": float("inf")}, {"page": 1 << 20, "width": 1 << 12}],
+             {"scale": float("nan")}, {"scale": float("inf")}, {"page": 1 << 20, "width": 1 << 12}],
     packed: [{"dtype": 7}, {"out": None}, {"cu": None}, {"B": 0}, {"T": -1}, {"H": 3}, {"G": 0}, {"D": 0}, {"D": 257}, {"scale": float("inf")},
              {"scale": float("nan")}],
     sample: [{"dtype": 9}, {"logits": None}, {"ld": 99}, {"t": -0.5}, {"t": float("nan")}, {"t": float("inf")}, {"k": -1}, {"p": -0.1},
@@ -161,3 +161,42 @@ def test_definitions_agree_with_torch():
     turn = torch.polar(torch.full((2,), 2.0, dtype=torch.float64), 7 * f.double())
     want = torch.view_as_real(torch.view_as_complex(x[:, :4].reshape(2, 2, 2)) * turn).flatten(1)
     assert torch.allclose(y[:, :4], want) and torch.equal(y[:, 4:], x[:, 4:])
+
+
+def test_units_of_a_batch_are_dealt_out_once(tmp_path):
+    """Every unit of every item belongs to one block, in order; parts stay inside their item; an item that is split has one beginning and
+    one end, and the block after a part's block goes on where it stopped."""
+    compiled(tmp_path, """
+  const long long lengths[5][4] = {{1, 1, 1, 1}, {0, 64, 65, 5000}, {100000, 1, 0, 7}, {640, 640, 640, 640}, {0, 0, 0, 0}};
+  for (auto &tokens : lengths)
+    for (int share : {1, 3, 8})
+      for (int blocks : {1, 2, 7, 296})
+        for (int least : {1, 4}) {
+          long long total = 0, base[4];
+          for (int b = 0; b < 4; ++b) {
+            base[b] = total;
+            CHECK(units_of(tokens[b]) >= 1 && units_of(tokens[b]) * DECODE_UNIT >= tokens[b])
+            total += units_of(tokens[b]) * share;
+          }
+          const long long per = units_per_block(total, blocks, least);
+          CHECK(per >= least && per * blocks >= total)
+          long long at = 0;
+          for (int c = 0; c < blocks; ++c) {
+            long long x = c * per;
+            const long long end = x + per < total ? x + per : total;
+            if (x >= end) continue;
+            int b = 3;
+            while (base[b] > x) --b;
+            while (x < end) {
+              const long long units = units_of(tokens[b]);
+              const DecodePart p = decode_part(x, end, base[b], units);
+              CHECK(x == at && p.item >= 0 && p.item < share && p.from >= 0 && p.from < p.to && p.to <= units)
+              CHECK(base[b] + p.item * units + p.from == x)
+              x += p.to - p.from;
+              at = x;
+              CHECK(p.to == units || x == end)
+              if (x < end && x == base[b] + units * share) ++b;
+            }
+          }
+          CHECK(at == total)
+        }""")
