@@ -147,7 +147,7 @@ SERVING_SIGNATURES = {
                                  _sz, _vp]),
     "djv_paged_faults": (C.c_uint, []),
     "djv_packed_attention": (_i, [_i, _vp, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _ll, _ll, _vp, _i, _i, _i, _i, _i, _f, _i, _vp]),
-    "djv_packed_timeouts": (C.c_uint, []),
+    "djv_serving_timeouts": (C.c_uint, []),
     "djv_sample": (_i, [_i, _vp, _vp, _ll, _vp, _vp, _ll, _vp, _i, _vp, _ll, _vp, _ll, _i, _i, _vp]),
 }
 _TABLES = (SIGNATURES, HYBRID_SIGNATURES, ROUTED_SIGNATURES, SERVING_SIGNATURES)

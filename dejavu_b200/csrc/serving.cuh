@@ -8,6 +8,8 @@ namespace djv {
 
 // table entries and positions that each kernel refused (djv_paged_faults)
 unsigned append_faults(), decode_faults();
+// waits that ran out (djv_serving_timeouts)
+unsigned decode_timeouts(), packed_timeouts();
 
 struct Pool {  // strides in elements
   long long ld_page, ld_head, ld_slot;

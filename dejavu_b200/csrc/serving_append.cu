@@ -116,6 +116,8 @@ using namespace djv;
 
 extern "C" unsigned djv_paged_faults(void) { return append_faults() + decode_faults(); }
 
+extern "C" unsigned djv_serving_timeouts(void) { return decode_timeouts() + packed_timeouts(); }
+
 extern "C" int djv_paged_append(int dtype, void *q_out, void *k_out, const void *q, long long ldq, long long hq, const void *k,
                                 long long ldk, long long hk, const void *v, long long ldv, long long hv, void *k_pages,
                                 void *v_pages, long long ld_page, long long ld_head, long long ld_slot, int pages, int page,

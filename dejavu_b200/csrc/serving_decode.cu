@@ -8,7 +8,8 @@
 // than a few units a block takes an item and there is no second kernel.
 //
 // A block's four warps take 16 tokens at a time, each with a softmax of its own, joined in shared memory at the item's end. Rows of K and V
-// arrive in a ring per warp by 16-byte asynchronous copies (any page size, any strides), swizzled for ldmatrix; the page of a tile is
+// arrive in a ring per warp by 16-byte asynchronous copies (any page size, any strides), swizzled for ldmatrix; the ring runs on from
+// item to item, so that the next one's rows are on their way while one ends, and the page of a tile is
 // looked up a tile ahead. fp16 and bf16 go through mma.sync, 16 query heads x 16 tokens: tcgen05 would have to pad the heads to
 // 64 or 128 rows, and the tensor work is a small part of the time either way. The weights enter the second product as two terms
 // of the cache's type, hi + lo, so that they keep 16 (bf16) or 22 bits. fp32 goes through the CUDA cores, 4 heads at a time.
@@ -17,11 +18,14 @@
 
 #include "mma.cuh"
 #include "pairs.cuh"
+#include "ring.cuh"
 #include "serving.cuh"
+#include "tensor_map.cuh"
 
 namespace djv {
 
 __device__ unsigned g_decode_faults;
+__device__ unsigned g_decode_timeouts;  // bounded waits that ran out (never, in a healthy run)
 
 constexpr int DE_WARPS = 4, DE_THREADS = DE_WARPS * WARP;
 
@@ -108,9 +112,18 @@ struct DecodeRows {  // query heads of an item
 template <typename T, int DP>
 struct DecodeSums;
 
-template <typename T, int DP>
-__device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {  // of a 16-byte chunk in a tile
-  return (uint32_t)(row * DP * (int)sizeof(T) + ((chunk ^ (row & 7)) << 4));
+// Of a 16-byte chunk in a tile: blocks of 128 bytes of every row, swizzled as TMA does and as ldmatrix reads without bank conflicts.
+template <int ROWS>
+__device__ __forceinline__ uint32_t tile_offset(int row, int chunk) {
+  return (uint32_t)((chunk >> 3) * (ROWS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+}
+
+// a box of one tile's rows and 128 bytes of each: slots of a page of one head
+__device__ __forceinline__ void tma_load_slots(uint32_t dst, const CUtensorMap *map, int d, int slot, int head, int page, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map),
+      "r"(d), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
 }
 
 template <typename T>
@@ -160,7 +173,7 @@ struct MmaSums {
     for (int k = 0; k < DP / 16; ++k) {
       if (k * 16 >= D) break;
       uint32_t b[4];
-      ldmatrix_x4(b, k_sm + tile_offset<T, DP>((lane >> 4) * 8 + lane % 8, k * 2 + ((lane >> 3) & 1)));
+      ldmatrix_x4(b, k_sm + tile_offset<TOKENS>((lane >> 4) * 8 + lane % 8, k * 2 + ((lane >> 3) & 1)));
       mma_m16n8k16_t<T>(s[0], q[k][0], q[k][1], q[k][2], q[k][3], b[0], b[1]);
       mma_m16n8k16_t<T>(s[1], q[k][0], q[k][1], q[k][2], q[k][3], b[2], b[3]);
     }
@@ -205,27 +218,69 @@ struct MmaSums {
     for (int i = 0; i < DP / 16; ++i) {
       if (i * 16 >= D) break;
       uint32_t b[4];
-      ldmatrix_x4_trans(b, v_sm + tile_offset<T, DP>(((lane >> 3) & 1) * 8 + lane % 8, i * 2 + (lane >> 4)));
+      ldmatrix_x4_trans(b, v_sm + tile_offset<TOKENS>(((lane >> 3) & 1) * 8 + lane % 8, i * 2 + (lane >> 4)));
       mma_m16n8k16_t<T>(o[2 * i], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
       mma_m16n8k16_t<T>(o[2 * i + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
       mma_m16n8k16_t<T>(o[2 * i], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
       mma_m16n8k16_t<T>(o[2 * i + 1], lo[0], lo[1], lo[2], lo[3], b[2], b[3]);
     }
   }
-  // sums (rows, DP), and the maxima and sums of the rows
-  __device__ __forceinline__ void store(float *sums, float *sm, float *sl) {
-    const int lane = threadIdx.x % WARP, g = lane / 4, t = lane % 4;
+  __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    }
+  }
+  // another warp's sums join this one's
+  __device__ __forceinline__ void absorb(const float *sums, const float *sm, const float *sl) {
+    const int lane = threadIdx.x % WARP, g = lane / 4, t = lane % 4;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float other = sm[g + r * 8], top = fmaxf(m[r], other), base = top == -INFINITY ? 0.f : top;
+      const float mine = exp2_approx(m[r] - base), its = exp2_approx(other - base);
+      m[r] = top;
+      l[r] = l[r] * mine + sl[g + r * 8] * its;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        const float2 y = *reinterpret_cast<const float2 *>(sums + (g + r * 8) * DP + ((i ^ g) * 8 + t * 2));
+        o[i][2 * r] = o[i][2 * r] * mine + y.x * its;
+        o[i][2 * r + 1] = o[i][2 * r + 1] * mine + y.y * its;
+      }
+    }
+  }
+  // the result, where the item is whole (slot NULL), or what the second kernel joins
+  __device__ __forceinline__ void emit(T *out, float *slot, int rows, int D) const {
+    const int lane = threadIdx.x % WARP, g = lane / 4, t = lane % 4;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int row = g + r * 8;
+      if (row >= rows) continue;
+      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i) {
+        if (i * 8 >= D) continue;
+        if (slot == nullptr) *reinterpret_cast<uint32_t *>(out + row * D + i * 8 + t * 2) = pair_of<T>(o[i][2 * r] * inv, o[i][2 * r + 1] * inv);
+        else *reinterpret_cast<float2 *>(slot + row * DP + i * 8 + t * 2) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+      }
+      if (slot != nullptr && t == 0) {
+        slot[16 * DP + row] = m[r];
+        slot[16 * DP + 16 + row] = l[r];
+      }
+    }
+  }
+  // sums (rows, DP), 8-column pieces of a row in an order of its own (no bank conflicts), and the rows' maxima and sums
+  __device__ __forceinline__ void store(float *sums, float *sm, float *sl) const {
+    const int lane = threadIdx.x % WARP, g = lane / 4, t = lane % 4;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
       if (t == 0) {
         sm[g + r * 8] = m[r];
         sl[g + r * 8] = l[r];
       }
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i)
-        *reinterpret_cast<float2 *>(sums + (g + r * 8) * DP + i * 8 + t * 2) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
+        *reinterpret_cast<float2 *>(sums + (g + r * 8) * DP + ((i ^ g) * 8 + t * 2)) = make_float2(o[i][2 * r], o[i][2 * r + 1]);
     }
   }
 };
@@ -264,7 +319,7 @@ struct DecodeSums<float, DP> {
     const int lane = threadIdx.x % WARP, token = lane % TOKENS, part = lane / TOKENS;
     float s[4] = {};
     for (int ch = part; ch * 4 < D; ch += PARTS) {
-      const float4 k = at(k_sm + tile_offset<float, DP>(token, ch));
+      const float4 k = at(k_sm + tile_offset<TOKENS>(token, ch));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (r >= rows) break;
@@ -298,17 +353,49 @@ struct DecodeSums<float, DP> {
       for (int i = 0; i < W; ++i) {
         float v;
         const int d = i * WARP + lane;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(v_sm + tile_offset<float, DP>(t, d / 4) + (d % 4) * 4) : "memory");
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(v_sm + tile_offset<TOKENS>(t, d / 4) + (d % 4) * 4) : "memory");
 #pragma unroll
         for (int r = 0; r < 4; ++r) o[r][i] = fmaf(p[r], v, o[r][i]);
       }
     }
   }
-  __device__ __forceinline__ void store(float *sums, float *sm, float *sl) {
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) l[r] = warp_sum(l[r]);
+  }
+  __device__ __forceinline__ void absorb(const float *sums, const float *sm, const float *sl) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float top = fmaxf(m[r], sm[r]), base = top == -INFINITY ? 0.f : top, mine = exp2f(m[r] - base), its = exp2f(sm[r] - base);
+      m[r] = top;
+      l[r] = l[r] * mine + sl[r] * its;
+#pragma unroll
+      for (int i = 0; i < W; ++i) o[r][i] = o[r][i] * mine + sums[r * DP + i * WARP + threadIdx.x % WARP] * its;
+    }
+  }
+  __device__ __forceinline__ void emit(float *out, float *slot, int n, int D) const {
     const int lane = threadIdx.x % WARP;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      l[r] = warp_sum(l[r]);
+      if (r >= n) continue;
+      const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const int d = i * WARP + lane;
+        if (d >= D) continue;
+        if (slot == nullptr) out[r * D + d] = o[r][i] * inv;
+        else slot[r * DP + d] = o[r][i];
+      }
+      if (slot != nullptr && lane == 0) {
+        slot[4 * DP + r] = m[r];
+        slot[4 * DP + 4 + r] = l[r];
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float *sums, float *sm, float *sl) const {
+    const int lane = threadIdx.x % WARP;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
       if (lane == 0) {
         sm[r] = m[r];
         sl[r] = l[r];
@@ -324,207 +411,318 @@ struct DecodeRing {
   static constexpr int TILE = DecodeSums<T, DP>::TOKENS * DP * (int)sizeof(T);  // bytes of a tile of keys, or of values
   // as many blocks and stages as shared memory has room for: 16 to 24 KB in flight per warp, 96 to 192 KB per multiprocessor
   static constexpr int BLOCKS = TILE <= 2048 ? 3 : (TILE <= 4096 ? 2 : 1), STAGES = TILE <= 2048 ? 4 : 3;
-  static constexpr int SMEM = DE_WARPS * STAGES * 2 * TILE;
+  static constexpr int BYTES = DE_WARPS * STAGES * 2 * TILE, SUMS = DecodeRows<T>::N * DP;  // sums: floats of one warp's
+  struct Rest {
+    uint64_t full[DE_WARPS][STAGES];
+    long long slots[DE_WARPS + 2];
+    float sm[2][DecodeRows<T>::N], sl[2][DecodeRows<T>::N];
+    unsigned seen[DE_WARPS][STAGES];
+  };
+  static constexpr int SMEM = BYTES + 2 * SUMS * 4 + (int)sizeof(Rest);
 };
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(DE_THREADS, DecodeRing<T, DP>::BLOCKS) decode_kernel(DecodeArgs a, int least) {
+// Where a block is in its units.
+struct DecodeCursor {
+  long long x, end, base;  // next unit, the last one's end, the sequence's first unit
+  int b, tokens, units;    // of an item of the sequence
+  int item, from, to;      // the part: units from .. to - 1 of the item
+  int t0, t1;
+  int tiles, i;  // rounds of four tiles of this part, and the next of them
+};
+
+// BOXES: pages are whole tiles, which TMA brings, one thread asking; else every lane copies 16-byte chunks.
+template <typename T, int DP, bool BOXES>
+__global__ void __launch_bounds__(DE_THREADS, DecodeRing<T, DP>::BLOCKS)
+decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, DecodeArgs a, int least) {
   using Sums = DecodeSums<T, DP>;
   using Ring = DecodeRing<T, DP>;
   constexpr int ROWS = DecodeRows<T>::N, TOKENS = Sums::TOKENS, STAGES = Ring::STAGES, TILE = Ring::TILE;
   constexpr int N = Chunk<T>::N, CHUNKS = DP / N;                              // of a row
   constexpr int AT_ONCE = CHUNKS >= WARP ? 1 : WARP / CHUNKS, WIDE = CHUNKS > WARP ? CHUNKS / WARP : 1;
-  extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ float sm[DE_WARPS][ROWS], sl[DE_WARPS][ROWS];
-  __shared__ long long slots[DE_WARPS + 2];
+  extern __shared__ __align__(1024) unsigned char ring[];
+  float *const joined = reinterpret_cast<float *>(ring + Ring::BYTES);
+  // (not of their own beside the ring: what stands in front of it would be padded to its alignment)
+  auto &rest = *reinterpret_cast<typename Ring::Rest *>(joined + 2 * Ring::SUMS);
+  auto &full = rest.full;
+  auto &sm = rest.sm, &sl = rest.sl;
+  auto &seen = rest.seen;
+  long long *const slots = rest.slots;
   const int tid = threadIdx.x, lane = tid % WARP, warp = tid / WARP;
-  pdl_prologue();
+  if (BOXES) {
+    if (lane == 0) {
+      for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
+      mbar_fence_init();
+    }
+    __syncwarp();
+  }
+  // (in this order: what the second kernel reads ahead of its wait, the positions, is complete when it starts)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int share = a.G * a.groups, R = a.H / a.G;
-  long long x, end, base, units, tokens;
-  int b;
-  long long mine = 0;  // first unit of this block
+  auto sequence = [&](DecodeCursor &c) {
+    c.tokens = (int)decode_tokens(a, c.b);
+    c.units = (int)units_of(c.tokens);
+  };
+  auto open = [&](DecodeCursor &c) {  // the part that begins at c.x
+    const DecodePart p = decode_part(c.x, c.end, c.base, c.units);
+    c.item = (int)p.item;
+    c.from = (int)p.from;
+    c.to = (int)p.to;
+    c.t0 = (int)tokens_before(p.from, c.tokens);
+    c.t1 = (int)tokens_before(p.to, c.tokens);
+    c.tiles = c.t1 > c.t0 ? (c.t1 - c.t0 + DE_WARPS * TOKENS - 1) / (DE_WARPS * TOKENS) : 1;
+    c.i = 0;
+  };
+  auto close = [&](DecodeCursor &c) {  // on to the next part; false: there is none
+    c.x += c.to - c.from;
+    if (c.x >= c.end) return false;
+    if (c.x == c.base + (long long)c.units * share) {
+      c.base = c.x;
+      ++c.b;
+      sequence(c);
+    }
+    open(c);
+    return true;
+  };
+  DecodeCursor at;  // of the products
   if (a.parts == nullptr) {  // an item each
-    b = blockIdx.x / share;
-    tokens = decode_tokens(a, b);
-    units = units_of(tokens);
-    base = 0;
-    x = (blockIdx.x - (long long)b * share) * units;
-    end = x + units;
+    at.b = blockIdx.x / share;
+    at.base = 0;
+    sequence(at);
+    at.x = (long long)(blockIdx.x - at.b * share) * at.units;
+    at.end = at.x + at.units;
   } else {
     long long per;
     const DecodePlace w = decode_locate(a, [&](long long total) {
       per = units_per_block(total, gridDim.x, least);
       return blockIdx.x * per;
     }, slots);
-    x = mine = blockIdx.x * per;
-    end = x + per < w.total ? x + per : w.total;
-    if (x >= end || w.b < 0) return;
-    b = w.b;
-    base = w.base;
-    tokens = decode_tokens(a, b);
-    units = units_of(tokens);
+    at.x = blockIdx.x * per;
+    at.end = at.x + per < w.total ? at.x + per : w.total;
+    if (at.x >= at.end || w.b < 0) return;
+    at.b = w.b;
+    at.base = w.base;
+    sequence(at);
   }
-  if (tid == 0 && a.pos[b] >= (long long)a.width * a.page && x == base) atomicAdd(&g_decode_faults, 1u);
+  open(at);
+  DecodeCursor ahead = at;  // of the loads
+  bool more = true;
   const uint32_t warp_ring = smem_addr(ring) + warp * STAGES * 2 * TILE;
-  float *warp_sums = reinterpret_cast<float *>(ring + warp * STAGES * 2 * TILE);
   const float c = a.scale * 1.4426950408889634f;
 
-  while (x < end) {
-    const DecodePart part = decode_part(x, end, base, units);
-    const int g = (int)(part.item / a.groups), h0 = (int)(part.item % a.groups) * ROWS, rows = min(ROWS, R - h0), h = g * R + h0;
-    const long long t0 = part.from * DECODE_UNIT, t1 = min(tokens, part.to * DECODE_UNIT);
-    const PageMap map{a.table + b * a.ld_table, a.width, a.page, a.pages};
-    const T *k = static_cast<const T *>(a.k) + g * a.pool.ld_head, *v = static_cast<const T *>(a.v) + g * a.pool.ld_head;
-    const int tiles = t1 > t0 ? (int)((t1 - t0 + DE_WARPS * TOKENS - 1) / (DE_WARPS * TOKENS)) : 0;
-    auto first_of = [&](int i) { return t0 + (long long)(i * DE_WARPS + warp) * TOKENS; };
-    // where the row of the lane's token of tile i is (lanes beyond the tokens repeat them), or -1
-    auto row_of = [&](int i) -> long long {
-      const long long t = first_of(i) + lane % TOKENS;
-      if (i >= tiles || t >= t1) return -1;
-      int slot;
-      const long long page = page_of(map, t, slot);
-      if (page != NO_PAGE) return page * a.pool.ld_page + slot * a.pool.ld_slot;
-      if (part.item == 0 && lane < TOKENS && (slot == 0 || lane == 0)) atomicAdd(&g_decode_faults, 1u);
-      return -1;
-    };
-    unsigned seen[STAGES];
-    auto load = [&](int i, long long row, unsigned &bits) {
-      bits = __ballot_sync(0xffffffffu, row >= 0) & (TOKENS == 32 ? 0xffffffffu : (1u << TOKENS) - 1);
-      if (i < tiles) {
-        const uint32_t dst = warp_ring + i % STAGES * 2 * TILE;
+  const PageMap no_map{nullptr, a.width, a.page, a.pages};
+  // The first token of the warp's next tile; where its row is in the pools (BOXES: the page and, in the upper half, the slot), or -1.
+  // Without BOXES the lane's own token's, lanes beyond the tile's tokens repeat them.
+  auto row_ahead = [&]() -> long long {
+    const int t = ahead.t0 + (ahead.i * DE_WARPS + warp) * TOKENS + (BOXES ? 0 : lane % TOKENS);
+    if (!more || t >= ahead.t1) return -1;
+    int slot;
+    PageMap map = no_map;
+    map.table = a.table + ahead.b * a.ld_table;
+    const long long page = page_of(map, t, slot);
+    if (page != NO_PAGE) return BOXES ? (long long)slot << 32 | page : page * a.pool.ld_page + slot * a.pool.ld_slot;
+    if (ahead.item == 0 && lane < (BOXES ? 1 : TOKENS) && (slot == 0 || lane == 0)) atomicAdd(&g_decode_faults, 1u);
+    return -1;
+  };
+  long long row = row_ahead();
+  unsigned asked = 0, taken = 0;  // phases of the stages' barriers, a bit each
+  bool dead = false;              // a wait ran out: wait no more, finish and report
+  auto load = [&](int stage) {
+    if (more) {
+      const uint32_t dst = warp_ring + stage * 2 * TILE;
+      const int g = ahead.item / a.groups;
+      if (BOXES) {
+        const int left = ahead.t1 - ahead.t0 - (ahead.i * DE_WARPS + warp) * TOKENS;
+        if (lane == 0) {
+          seen[warp][stage] = row < 0 ? 0u : (left >= TOKENS ? (1u << TOKENS) - 1 : (1u << left) - 1);
+          if (row >= 0) {
+            mbar_arrive_expect_tx(&full[warp][stage], 2 * TILE);
+#pragma unroll
+            for (int x = 0; x < DP * (int)sizeof(T) / 128; ++x) {
+              const int d = x * (128 / (int)sizeof(T));
+              tma_load_slots(dst + x * TOKENS * 128, &map_k, d, (int)(row >> 32), g, (int)row, &full[warp][stage]);
+              tma_load_slots(dst + TILE + x * TOKENS * 128, &map_v, d, (int)(row >> 32), g, (int)row, &full[warp][stage]);
+            }
+          }
+        }
+        if (row >= 0) asked ^= 1u << stage;
+      } else {
+        const unsigned bits = __ballot_sync(0xffffffffu, row >= 0) & ((1u << TOKENS) - 1);
+        if (lane == 0) seen[warp][stage] = bits;
+        const long long head = g * a.pool.ld_head;
+        const T *k = static_cast<const T *>(a.k), *v = static_cast<const T *>(a.v);
 #pragma unroll
         for (int p = 0; p < TOKENS / AT_ONCE; ++p) {
           const int r = p * AT_ONCE + (CHUNKS >= WARP ? 0 : lane / CHUNKS);
-          const long long at = __shfl_sync(0xffffffffu, row, r);
+          const long long off = __shfl_sync(0xffffffffu, row, r);
 #pragma unroll
           for (int y = 0; y < WIDE; ++y) {
             const int ch = CHUNKS >= WARP ? y * WARP + lane : lane % CHUNKS;
-            const bool ok = at >= 0 && ch * N < a.D;
-            const uint32_t to = dst + tile_offset<T, DP>(r, ch);
-            cp_async16_zfill(to, ok ? k + at + ch * N : k, ok ? 16 : 0);
-            cp_async16_zfill(to + TILE, ok ? v + at + ch * N : v, ok ? 16 : 0);
+            const bool ok = off >= 0 && ch * N < a.D;
+            const long long from = ok ? off + head + ch * N : 0;
+            const uint32_t to = dst + tile_offset<TOKENS>(r, ch);
+            cp_async16_zfill(to, k + from, ok ? 16 : 0);
+            cp_async16_zfill(to + TILE, v + from, ok ? 16 : 0);
           }
         }
       }
-      cp_async_commit();
-    };
-    Sums sums;
-    long long next = row_of(0);
-    sums.start(static_cast<const T *>(a.q) + b * a.ldq + h * a.hq, a.hq, rows, a.D);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      load(i, next, seen[i]);
-      next = row_of(i + 1);
+      if (++ahead.i == ahead.tiles) more = close(ahead);
+      row = row_ahead();
     }
-    for (int i0 = 0; i0 < tiles; i0 += STAGES) {
-#pragma unroll
-      for (int y = 0; y < STAGES; ++y) {
-        const int i = i0 + y;
-        if (i >= tiles) break;
-        cp_async_wait<STAGES - 2>();
-        __syncwarp();
-        load(i + STAGES - 1, next, seen[(y + STAGES - 1) % STAGES]);
-        next = row_of(i + STAGES);
-        if (seen[y]) sums.tile(warp_ring + y * 2 * TILE, warp_ring + y * 2 * TILE + TILE, seen[y], c, a.D);
-        __syncwarp();
-      }
-    }
-    cp_async_wait<0>();
+    if (!BOXES) cp_async_commit();
+  };
+  // Waits for a stage; its tokens that are there. Values that are not (behind the sequence's last token) become zeros.
+  auto arrived = [&](int stage) -> unsigned {
+    if (!BOXES) cp_async_wait<STAGES - 1>();
     __syncwarp();
-    sums.store(warp_sums, sm[warp], sl[warp]);
-    __syncthreads();
-    const bool whole = part.from == 0 && part.to == units;
-    // the slot of a part: 1 of an item that begins here, 0 of one that began in a block before
-    float *slot = whole ? nullptr : a.parts + (blockIdx.x * 2 + (part.from == 0 ? 1 : 0)) * (long long)(ROWS * (DP + 2));
-    for (int i = tid; i < rows * (DP / 4); i += DE_THREADS) {
-      const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-      if (d >= a.D) continue;
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < DE_WARPS; ++w) top = fmaxf(top, sm[w][r]);
-      const float down = top == -INFINITY ? 0.f : top;
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < DE_WARPS; ++w) {
-        const float f = exp2f(sm[w][r] - down);
-        const float4 y = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(ring + w * STAGES * 2 * TILE) + r * DP + d);
-        sum += sl[w][r] * f;
-        o.x += y.x * f;
-        o.y += y.y * f;
-        o.z += y.z * f;
-        o.w += y.w * f;
-      }
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T *out = static_cast<T *>(a.out) + ((long long)b * a.H + h + r) * a.D + d;
-        T r4[4] = {from_f<T>(o.x * inv), from_f<T>(o.y * inv), from_f<T>(o.z * inv), from_f<T>(o.w * inv)};
-        if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<uint4 *>(r4);
-        else *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<uint2 *>(r4);
-      } else {
-        *reinterpret_cast<float4 *>(slot + r * DP + d) = o;
-        if (d == 0) {
-          slot[ROWS * DP + r] = top;
-          slot[ROWS * DP + ROWS + r] = sum;
-        }
+    const unsigned bits = seen[warp][stage];
+    if (BOXES && bits) {
+      if (!dead) dead = !mbar_wait(&full[warp][stage], (taken >> stage) & 1);
+      taken ^= 1u << stage;
+      if (bits != (1u << TOKENS) - 1) {
+        const int first = __popc(bits);  // (they are the last ones)
+        for (int i = lane; i < (TOKENS - first) * CHUNKS; i += WARP)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(warp_ring + stage * 2 * TILE + TILE +
+                                                                         tile_offset<TOKENS>(first + i / CHUNKS, i % CHUNKS)),
+                       "r"(0)
+                       : "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
       }
     }
-    __syncthreads();
-    x += part.to - part.from;
-    if (x < end && x == base + units * share) {
-      base = x;
-      ++b;
-      tokens = decode_tokens(a, b);
-      units = units_of(tokens);
-      if (tid == 0 && a.pos[b] >= (long long)a.width * a.page) atomicAdd(&g_decode_faults, 1u);
+    return bits;
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; ++i) load(i);
+
+  Sums sums;
+  int stage = 0;
+  for (;;) {
+    const int g = (int)(at.item / a.groups), h0 = (int)(at.item % a.groups) * ROWS, rows = min(ROWS, R - h0), h = g * R + h0;
+    if (tid == 0 && at.item == 0 && at.from == 0 && a.pos[at.b] >= (long long)a.width * a.page) atomicAdd(&g_decode_faults, 1u);
+    sums.start(static_cast<const T *>(a.q) + at.b * a.ldq + h * a.hq, a.hq, rows, a.D);
+#pragma unroll 1
+    for (int i = 0; i < at.tiles; ++i) {
+      load(stage == 0 ? STAGES - 1 : stage - 1);
+      const unsigned bits = arrived(stage);
+      if (bits) sums.tile(warp_ring + stage * 2 * TILE, warp_ring + stage * 2 * TILE + TILE, bits, c, a.D);
+      __syncwarp();
+      stage = stage == STAGES - 1 ? 0 : stage + 1;
     }
+    // the four warps' sums: two and two, then the two that are left
+    sums.finish();
+    __syncthreads();  // (the last item's sums have been read)
+    if (warp >= 2) sums.store(joined + (warp - 2) * Ring::SUMS, sm[warp - 2], sl[warp - 2]);
+    __syncthreads();
+    if (warp < 2) sums.absorb(joined + warp * Ring::SUMS, sm[warp], sl[warp]);
+    __syncwarp();
+    if (warp == 1) sums.store(joined + Ring::SUMS, sm[1], sl[1]);
+    __syncthreads();
+    if (warp == 0) {
+      sums.absorb(joined + Ring::SUMS, sm[1], sl[1]);
+      const bool whole = at.from == 0 && at.to == at.units;
+      // the slot of a part: 1 of an item that begins here, 0 of one that began in a block before
+      float *slot = whole ? nullptr : a.parts + (blockIdx.x * 2 + (at.from == 0 ? 1 : 0)) * (long long)(ROWS * (DP + 2));
+      sums.emit(static_cast<T *>(a.out) + ((long long)at.b * a.H + h) * a.D, slot, rows, a.D);
+    }
+    if (!close(at)) break;
   }
-  (void)mine;
+  cp_async_wait<0>();
+  if (BOXES && dead) {  // copies that nobody waited for still land
+    for (int i = 0; i < STAGES; ++i)
+      if (asked != 0 || taken != 0) mbar_wait(&full[warp][i], ((asked >> i) & 1) ^ 1);
+    if (lane == 0) atomicAdd(&g_decode_timeouts, 1u);
+  }
 }
 
-// Joins the parts of the item that begins in block blockIdx.x of `blocks` and ends in a later one, if there is one.
+// Joins the parts of the item that begins in block blockIdx.x of `blocks` and ends in a later one, if there is one: row blockIdx.y, the
+// parts dealt out to the warps, four dimensions to a lane.
 template <typename T, int DP>
 __global__ void __launch_bounds__(DE_THREADS) decode_join_kernel(DecodeArgs a, int blocks, int least) {
-  constexpr int ROWS = DecodeRows<T>::N;
+  constexpr int ROWS = DecodeRows<T>::N, WIDE = DP > 128 ? 2 : 1;
   constexpr long long SLOT = ROWS * (DP + 2);
   __shared__ long long slots[DE_WARPS + 2];
-  pdl_prologue();
+  __shared__ float4 so[DE_WARPS][WIDE * WARP];
+  __shared__ float sm[DE_WARPS], sl[DE_WARPS];
+  const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   long long per;
   const int share = a.G * a.groups, R = a.H / a.G;
+  // (positions and their like are those the first kernel worked with: it let this one start when they were complete)
   const DecodePlace w = decode_locate(a, [&](long long total) {
     per = units_per_block(total, blocks, least);
     return (blockIdx.x + 1) * per - 1;
   }, slots);
   const long long last = (blockIdx.x + 1) * per - 1;  // this block's last unit
-  if (last + 1 >= w.total || w.b < 0) return;
-  const long long units = units_of(decode_tokens(a, w.b)), item = (last - w.base) / units, from = w.base + item * units, to = from + units;
-  if (to == last + 1 || from < blockIdx.x * per) return;  // it ends here, or began in a block before
-  const int end = (int)((to - 1) / per);
-  const int g = (int)(item / a.groups), h0 = (int)(item % a.groups) * ROWS, rows = min(ROWS, R - h0);
-  const float *begin = a.parts + (blockIdx.x * 2 + 1) * SLOT, *rest = a.parts + (blockIdx.x + 1) * 2 * SLOT;
-  const int more = end - blockIdx.x;  // slots after the first, 2 * SLOT apart
-  for (int i = threadIdx.x; i < rows * (DP / 4); i += DE_THREADS) {
-    const int r = i / (DP / 4), d = i % (DP / 4) * 4;
-    if (d >= a.D) continue;
-    float top = begin[ROWS * DP + r];
-    for (int s = 0; s < more; ++s) top = fmaxf(top, rest[s * 2 * SLOT + ROWS * DP + r]);
-    const float down = top == -INFINITY ? 0.f : top;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    for (int s = -1; s < more; ++s) {
-      const float *p = s < 0 ? begin : rest + s * 2 * SLOT;
-      const float f = exp2f(p[ROWS * DP + r] - down);
-      const float4 y = *reinterpret_cast<const float4 *>(p + r * DP + d);
-      sum += p[ROWS * DP + ROWS + r] * f;
-      o.x += y.x * f;
-      o.y += y.y * f;
-      o.z += y.z * f;
-      o.w += y.w * f;
+  bool mine = last + 1 < w.total && w.b >= 0;
+  long long item = 0;
+  int more = 0;  // parts after the first, 2 * SLOT apart
+  if (mine) {
+    const long long units = units_of(decode_tokens(a, w.b));
+    item = (last - w.base) / units;
+    const long long from = w.base + item * units, to = from + units;
+    mine = to > last + 1 && from >= blockIdx.x * per;  // else it ends here, or began in a block before
+    more = (int)((to - 1) / per) - (int)blockIdx.x;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int g = (int)(item / a.groups), h0 = (int)(item % a.groups) * ROWS, r = blockIdx.y;
+  if (!mine || r >= min(ROWS, R - h0)) return;
+  const float *begin = a.parts + (blockIdx.x * 2 + 1) * SLOT, *rest = a.parts + blockIdx.x * 2 * SLOT;  // part s > 0: rest + s * 2 * SLOT
+  float m = -INFINITY, l = 0.f;
+  float4 o[WIDE] = {};
+  for (int s0 = warp; s0 <= more; s0 += 4 * DE_WARPS) {  // four parts at a time
+    float pm[4], pl[4];
+    float4 y[4][WIDE];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int s = s0 + x * DE_WARPS;
+      const float *p = s == 0 ? begin : rest + s * 2 * SLOT;
+      pm[x] = s <= more ? p[ROWS * DP + r] : -INFINITY;
+      pl[x] = s <= more ? p[ROWS * DP + ROWS + r] : 0.f;
+#pragma unroll
+      for (int z = 0; z < WIDE; ++z) {
+        const int d = (z * WARP + lane) * 4;
+        y[x][z] = s <= more && d < a.D ? *reinterpret_cast<const float4 *>(p + r * DP + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T *out = static_cast<T *>(a.out) + ((long long)w.b * a.H + g * R + h0 + r) * a.D + d;
-    T r4[4] = {from_f<T>(o.x * inv), from_f<T>(o.y * inv), from_f<T>(o.z * inv), from_f<T>(o.w * inv)};
-    if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(out) = *reinterpret_cast<uint4 *>(r4);
-    else *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<uint2 *>(r4);
+    float top = m;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) top = fmaxf(top, pm[x]);
+    const float base = top == -INFINITY ? 0.f : top, corr = exp2f(m - base);
+    m = top;
+    l *= corr;
+#pragma unroll
+    for (int z = 0; z < WIDE; ++z) o[z] = make_float4(o[z].x * corr, o[z].y * corr, o[z].z * corr, o[z].w * corr);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = exp2f(pm[x] - base);
+      l = fmaf(pl[x], f, l);
+#pragma unroll
+      for (int z = 0; z < WIDE; ++z)
+        o[z] = make_float4(fmaf(y[x][z].x, f, o[z].x), fmaf(y[x][z].y, f, o[z].y), fmaf(y[x][z].z, f, o[z].z), fmaf(y[x][z].w, f, o[z].w));
+    }
+  }
+#pragma unroll
+  for (int z = 0; z < WIDE; ++z) so[warp][z * WARP + lane] = o[z];
+  if (lane == 0) {
+    sm[warp] = m;
+    sl[warp] = l;
+  }
+  __syncthreads();
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int x = 0; x < DE_WARPS; ++x) top = fmaxf(top, sm[x]);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int d = threadIdx.x; d < a.D; d += DE_THREADS) {
+    float y = 0.f;
+    sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < DE_WARPS; ++x) {
+      const float f = exp2f(sm[x] - base);
+      sum = fmaf(sl[x], f, sum);
+      y = fmaf(reinterpret_cast<const float *>(so[x])[d], f, y);
+    }
+    static_cast<T *>(a.out)[((long long)w.b * a.H + g * R + h0 + r) * a.D + d] = from_f<T>(sum == 0.f ? 0.f : y / sum);
   }
 }
 
@@ -549,21 +747,48 @@ static DecodePlan decode_plan(int B, int H, int G, int page, int width) {
   return p;
 }
 
+// A pool as TMA reads it: boxes of 128 bytes x `rows` slots of a page of a head. False: strides that TMA does not take.
+template <typename T>
+static bool slots_map(CUtensorMap *map, const void *p, const DecodeArgs &a, int rows) {
+  // (a stride that nothing depends on can be anything)
+  const auto bytes = [](long long stride, int n) { return n > 1 ? stride * (long long)sizeof(T) : 16ll; };
+  const long long slot = bytes(a.pool.ld_slot, a.page), head = bytes(a.pool.ld_head, a.G), page = bytes(a.pool.ld_page, a.pages);
+  for (long long s : {slot, head, page})
+    if (s <= 0 || s % 16 || s >= (1ll << 40)) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page, (cuuint64_t)a.G, (cuuint64_t)a.pages},
+                   strides[3] = {(cuuint64_t)slot, (cuuint64_t)head, (cuuint64_t)page};
+  const cuuint32_t box[4] = {128 / (cuuint32_t)sizeof(T), (cuuint32_t)rows, 1, 1}, unit[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<T, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return encode_tiled() && encode_tiled()(map, type, 4, const_cast<void *>(p), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP>
 static cudaError_t launch_decode(DecodeArgs a, void *scratch, cudaStream_t st) {
+  using Ring = DecodeRing<T, DP>;
   static DevicePrep prep;
   const int(*unused)[4];
   cudaError_t e = prep.get(
-      [&](int(&)[4]) { return cudaFuncSetAttribute(decode_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeRing<T, DP>::SMEM); },
+      [&](int(&)[4]) {
+        cudaError_t f = cudaFuncSetAttribute(decode_kernel<T, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::SMEM);
+        return f != cudaSuccess ? f : cudaFuncSetAttribute(decode_kernel<T, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Ring::SMEM);
+      },
       unused);
   if (e != cudaSuccess) return e;
+  constexpr int TOKENS = DecodeSums<T, DP>::TOKENS;
+  CUtensorMap k{}, v{};
+  const bool boxes = a.page % TOKENS == 0 && slots_map<T>(&k, a.k, a, TOKENS) && slots_map<T>(&v, a.v, a, TOKENS);
   const DecodePlan p = decode_plan<T, DP>(a.B, a.H, a.G, a.page, a.width);
   a.groups = p.groups;
   a.parts = p.split ? static_cast<float *>(scratch) : nullptr;
-  e = djv::launch_kernel(decode_kernel<T, DP>, dim3(p.blocks), dim3(DE_THREADS), DecodeRing<T, DP>::SMEM, st, a, p.least);
+  e = djv::launch_kernel(boxes ? decode_kernel<T, DP, true> : decode_kernel<T, DP, false>, dim3(p.blocks), dim3(DE_THREADS), Ring::SMEM, st,
+                         k, v, a, p.least);
   count_launch();
   if (e == cudaSuccess && p.split && p.blocks > 1) {
-    e = djv::launch_kernel(decode_join_kernel<T, DP>, dim3(p.blocks - 1), dim3(DE_THREADS), 0, st, a, p.blocks, p.least);
+    e = djv::launch_kernel(decode_join_kernel<T, DP>, dim3(p.blocks - 1, a.H / a.G < DecodeRows<T>::N ? a.H / a.G : DecodeRows<T>::N),
+                           dim3(DE_THREADS), 0, st, a, p.blocks, p.least);
     count_launch();
   }
   return e;
@@ -583,6 +808,14 @@ static auto decode_form(int dtype, int D, F f) {
 unsigned decode_faults() {
   unsigned v = 0;
   if (cudaMemcpyFromSymbol(&v, g_decode_faults, sizeof(v)) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return v;
+}
+unsigned decode_timeouts() {
+  unsigned v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_decode_timeouts, sizeof(v)) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }

@@ -452,13 +452,13 @@ int packed_tc(int dtype, const PackedArgs &a, cudaStream_t st) {
   return a.D <= 64 ? launch_packed_tc<bf16, 1>(a, st) : launch_packed_tc<bf16, 2>(a, st);
 }
 
-}  // namespace djv
-
-extern "C" unsigned djv_packed_timeouts(void) {
+unsigned packed_timeouts() {
   unsigned v = 0;
-  if (cudaMemcpyFromSymbol(&v, djv::g_packed_timeouts, sizeof(v)) != cudaSuccess) {
+  if (cudaMemcpyFromSymbol(&v, g_packed_timeouts, sizeof(v)) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
   return v;
 }
+
+}  // namespace djv

@@ -13,9 +13,10 @@ struct PageMap {
 constexpr long long NO_PAGE = -1;
 // Page of token t >= 0, or NO_PAGE where the table has none for it. slot receives its place in the page.
 DJV_HOST_DEVICE long long page_of(const PageMap &m, long long t, int &slot) {
-  const long long i = t / m.page;
-  slot = (int)(t - i * m.page);
-  if (t < 0 || i >= m.width) return NO_PAGE;
+  slot = 0;
+  if (t < 0 || t >= (long long)m.width * m.page) return NO_PAGE;
+  const unsigned i = (unsigned)t / (unsigned)m.page;  // (a table has room for less than 2^31 tokens)
+  slot = (int)((unsigned)t - i * (unsigned)m.page);
   const int entry = m.table[i];
   return entry >= 0 && entry < m.pages ? entry : NO_PAGE;
 }
@@ -33,10 +34,16 @@ DJV_HOST_DEVICE int sequence_of(const int *cu, int B, int t) {
 }
 
 // How the cached tokens of a batch are dealt out to blocks: sequence b of n tokens is `share` items (key/value heads times groups of
-// query heads), each of units_of(n) units of DECODE_UNIT tokens, an empty one of a unit too. All units stand in a row, sequence by
-// sequence and item by item, and every block takes `per` of them, so that an item may begin in one block and end in another.
+// query heads), each of units_of(n) units: one for its beginning and end, which take about as long as 64 tokens do, and one for every
+// DECODE_UNIT tokens. All units stand in a row, sequence by sequence and item by item, and every block takes `per` of them, so that
+// an item may begin in one block and end in another.
 constexpr int DECODE_UNIT = 64;
-DJV_HOST_DEVICE long long units_of(long long tokens) { return tokens <= 0 ? 1 : (tokens + DECODE_UNIT - 1) / DECODE_UNIT; }
+DJV_HOST_DEVICE long long units_of(long long tokens) { return tokens <= 0 ? 1 : (tokens + DECODE_UNIT - 1) / DECODE_UNIT + 1; }
+// Tokens of an item in front of its unit u.
+DJV_HOST_DEVICE long long tokens_before(long long u, long long tokens) {
+  const long long t = u <= 1 ? 0 : (u - 1) * DECODE_UNIT;
+  return t < tokens ? t : (tokens < 0 ? 0 : tokens);
+}
 DJV_HOST_DEVICE long long units_per_block(long long units, int blocks, int least) {
   const long long per = (units + blocks - 1) / blocks;
   return per < least ? least : per;

@@ -53,6 +53,9 @@ int djv_paged_attention(int dtype, void *out, const void *q, long long ldq, long
 /* Table entries and positions that were refused since load (synchronises). */
 unsigned djv_paged_faults(void);
 
+/* Waits of the library's kernels on their own copies and products that ran out since load (0 in a healthy process; synchronises). */
+unsigned djv_serving_timeouts(void);
+
 /* Causal attention over whole prompts, packed: rows cu[b] .. cu[b + 1] - 1 (cu: B + 1 int32, ascending, within 0 .. T) of q (T, H, D), k
  * and v (T, G, D) are sequence b; row i sees rows j <= i of its sequence, whatever the others hold. Rows ldq, ldk, ldv elements
  * apart, heads hq, hk, hv apart, dimensions adjacent. H % G == 0, D <= 256. out (T, H, D), contiguous. Rows of no sequence:
@@ -60,9 +63,6 @@ unsigned djv_paged_faults(void);
 int djv_packed_attention(int dtype, void *out, const void *q, long long ldq, long long hq, const void *k, long long ldk, long long hk,
                          const void *v, long long ldv, long long hv, const int32_t *cu, int B, int T, int H, int G, int D, float scale,
                          int keep_rest, void *stream);
-/* Waits of the tensor-core kernel on its own copies and products that ran out since load (0 in a healthy process; synchronises). */
-unsigned djv_packed_timeouts(void);
-
 /* One token per row of logits (B, V), rows ld elements apart, from a given number u[b] in [0, 1) (fp32). Of the entries that are neither
  * -inf nor NaN, ordered by (logit descending, index ascending), with w_i = exp((x_i - max) / temperature), are kept
  *   the first top_k (0: all); of those the ones in front of which less than top_p of their sum lies, the first always (1 or more:

@@ -14,8 +14,8 @@ F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 def ops(cuda):
     from dejavu_b200 import _lib, ops
 
-    _lib.load_serving()
-    return ops
+    yield ops
+    assert _lib.load_serving().djv_serving_timeouts() == 0
 
 
 def rnd(seed, *shape, dtype=F32):

@@ -175,7 +175,12 @@ def test_units_of_a_batch_are_dealt_out_once(tmp_path):
           long long total = 0, base[4];
           for (int b = 0; b < 4; ++b) {
             base[b] = total;
-            CHECK(units_of(tokens[b]) >= 1 && units_of(tokens[b]) * DECODE_UNIT >= tokens[b])
+            const long long u = units_of(tokens[b]);
+            CHECK(u >= 1 && tokens_before(0, tokens[b]) == 0 && tokens_before(1, tokens[b]) == 0 && tokens_before(u, tokens[b]) == tokens[b])
+            for (long long i = 0; i < u; ++i) {
+              const long long n = tokens_before(i + 1, tokens[b]) - tokens_before(i, tokens[b]);
+              CHECK(n >= (i > 0) && n <= (i > 0 ? DECODE_UNIT : 0))
+            }
             total += units_of(tokens[b]) * share;
           }
           const long long per = units_per_block(total, blocks, least);
