@@ -23,6 +23,7 @@ struct AppendArgs {
   long long ldq, hq, ldk, hk, ldv, hv;
   Pool pool;
   int pages, page;
+  Divider by_page;
   const int *table;
   long long ld_table;
   int width;
@@ -44,7 +45,7 @@ __device__ __forceinline__ AppendPlace append_place(const AppendArgs &a, int t) 
   w.p = a.pos[b] + (a.cu == nullptr ? 0 : t - a.cu[b]);
   if (w.p < 0) return w;
   int slot;
-  const PageMap m{a.table + b * a.ld_table, a.width, a.page, a.pages};
+  const PageMap m{a.table + b * a.ld_table, a.width, a.page, a.pages, a.by_page};
   const long long page = page_of(m, w.p, slot);
   if (page == NO_PAGE) atomicAdd(&g_append_faults, 1u);
   else w.at = page * a.pool.ld_page + slot * a.pool.ld_slot;
@@ -136,7 +137,7 @@ extern "C" int djv_paged_append(int dtype, void *q_out, void *k_out, const void 
               "paged_append: rows of the pages start on multiples of 16 bytes");
   if (T == 0) return DJV_OK;
   const AppendArgs a{q_out, k_out, k_pages, v_pages, q, k, v, ldq, hq, ldk, hk, ldv, hv, {ld_page, ld_head, ld_slot}, pages, page,
-                     table, ld_table, width, pos, cu, freqs, amp, half, B, H, G, D};
+                     divider_of(page), table, ld_table, width, pos, cu, freqs, amp, half, B, H, G, D};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == DJV_DTYPE_F16) djv::launch_kernel(append_simple_kernel<__half>, dim3(T), dim3(256), 0, st, a, interleaved);
   else if (dtype == DJV_DTYPE_BF16) djv::launch_kernel(append_simple_kernel<bf16>, dim3(T), dim3(256), 0, st, a, interleaved);

@@ -35,6 +35,7 @@ struct DecodeArgs {
   long long ldq, hq;
   Pool pool;
   int pages, page;
+  Divider by_page;
   const int *table;
   long long ld_table;
   int width;
@@ -148,6 +149,16 @@ struct MmaSums {
   static constexpr int TOKENS = 16;
   uint32_t q[DP / 16][4];
   float o[DP / 8][4], m[2], l[2];
+  uint32_t k_at[4], v_at[4];  // where the lane's rows and chunks of the operands are, in a 128-byte block of a tile
+
+  __device__ __forceinline__ MmaSums() {
+    const int lane = threadIdx.x % WARP;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      k_at[x] = tile_offset<TOKENS>((lane >> 4) * 8 + lane % 8, x * 2 + ((lane >> 3) & 1));
+      v_at[x] = tile_offset<TOKENS>(((lane >> 3) & 1) * 8 + lane % 8, x * 2 + (lane >> 4));
+    }
+  }
 
   __device__ __forceinline__ void start(const T *query, long long hq, int rows, int D) {
     const int g = threadIdx.x % WARP / 4, t = threadIdx.x % 4;
@@ -166,14 +177,13 @@ struct MmaSums {
     l[0] = l[1] = 0.f;
   }
   // c: scale in units of log 2; seen: a bit for each of the 16 tokens
-  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c, int D) {
-    const int lane = threadIdx.x % WARP, t = lane % 4;
+  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c, int) {
+    const int t = threadIdx.x % 4;
     float s[2][4] = {};
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
-      if (k * 16 >= D) break;
       uint32_t b[4];
-      ldmatrix_x4(b, k_sm + tile_offset<TOKENS>((lane >> 4) * 8 + lane % 8, k * 2 + ((lane >> 3) & 1)));
+      ldmatrix_x4(b, k_sm + k_at[k % 4] + k / 4 * (TOKENS * 128));
       mma_m16n8k16_t<T>(s[0], q[k][0], q[k][1], q[k][2], q[k][3], b[0], b[1]);
       mma_m16n8k16_t<T>(s[1], q[k][0], q[k][1], q[k][2], q[k][3], b[2], b[3]);
     }
@@ -216,9 +226,8 @@ struct MmaSums {
     }
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
-      if (i * 16 >= D) break;
       uint32_t b[4];
-      ldmatrix_x4_trans(b, v_sm + tile_offset<TOKENS>(((lane >> 3) & 1) * 8 + lane % 8, i * 2 + (lane >> 4)));
+      ldmatrix_x4_trans(b, v_sm + v_at[i % 4] + i / 4 * (TOKENS * 128));
       mma_m16n8k16_t<T>(o[2 * i], hi[0], hi[1], hi[2], hi[3], b[0], b[1]);
       mma_m16n8k16_t<T>(o[2 * i + 1], hi[0], hi[1], hi[2], hi[3], b[2], b[3]);
       mma_m16n8k16_t<T>(o[2 * i], lo[0], lo[1], lo[2], lo[3], b[0], b[1]);
@@ -425,7 +434,8 @@ struct DecodeRing {
 struct DecodeCursor {
   long long x, end, base;  // next unit, the last one's end, the sequence's first unit
   int b, tokens, units;    // of an item of the sequence
-  int item, from, to;      // the part: units from .. to - 1 of the item
+  int item, from, to;      // the part: units from .. to - 1 of the item, whose key/value head is
+  int head;
   int t0, t1;
   int tiles, i;  // rounds of four tiles of this part, and the next of them
 };
@@ -466,6 +476,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   auto open = [&](DecodeCursor &c) {  // the part that begins at c.x
     const DecodePart p = decode_part(c.x, c.end, c.base, c.units);
     c.item = (int)p.item;
+    c.head = c.item / a.groups;
     c.from = (int)p.from;
     c.to = (int)p.to;
     c.t0 = (int)tokens_before(p.from, c.tokens);
@@ -510,7 +521,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   const uint32_t warp_ring = smem_addr(ring) + warp * STAGES * 2 * TILE;
   const float c = a.scale * 1.4426950408889634f;
 
-  const PageMap no_map{nullptr, a.width, a.page, a.pages};
+  const PageMap no_map{nullptr, a.width, a.page, a.pages, a.by_page};
   // The first token of the warp's next tile; where its row is in the pools (BOXES: the page and, in the upper half, the slot), or -1.
   // Without BOXES the lane's own token's, lanes beyond the tile's tokens repeat them.
   auto row_ahead = [&]() -> long long {
@@ -526,16 +537,19 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   };
   long long row = row_ahead();
   unsigned asked = 0, taken = 0;  // phases of the stages' barriers, a bit each
+  unsigned there = 0;             // stages that have a tile
   bool dead = false;              // a wait ran out: wait no more, finish and report
   auto load = [&](int stage) {
     if (more) {
       const uint32_t dst = warp_ring + stage * 2 * TILE;
-      const int g = ahead.item / a.groups;
+      const int g = ahead.head;
       if (BOXES) {
-        const int left = ahead.t1 - ahead.t0 - (ahead.i * DE_WARPS + warp) * TOKENS;
-        if (lane == 0) {
-          seen[warp][stage] = row < 0 ? 0u : (left >= TOKENS ? (1u << TOKENS) - 1 : (1u << left) - 1);
-          if (row >= 0) {
+        const unsigned bit = 1u << stage;
+        there &= ~bit;
+        if (row >= 0) {
+          there |= bit;
+          asked ^= bit;
+          if (lane == 0) {
             mbar_arrive_expect_tx(&full[warp][stage], 2 * TILE);
 #pragma unroll
             for (int x = 0; x < DP * (int)sizeof(T) / 128; ++x) {
@@ -545,7 +559,6 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
             }
           }
         }
-        if (row >= 0) asked ^= 1u << stage;
       } else {
         const unsigned bits = __ballot_sync(0xffffffffu, row >= 0) & ((1u << TOKENS) - 1);
         if (lane == 0) seen[warp][stage] = bits;
@@ -572,11 +585,15 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     if (!BOXES) cp_async_commit();
   };
   // Waits for a stage; its tokens that are there. Values that are not (behind the sequence's last token) become zeros.
-  auto arrived = [&](int stage) -> unsigned {
-    if (!BOXES) cp_async_wait<STAGES - 1>();
-    __syncwarp();
-    const unsigned bits = seen[warp][stage];
-    if (BOXES && bits) {
+  auto arrived = [&](int stage, int i) -> unsigned {
+    if (!BOXES) {
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();
+      return seen[warp][stage];
+    }
+    const int left = at.t1 - at.t0 - (i * DE_WARPS + warp) * TOKENS;
+    const unsigned bits = !((there >> stage) & 1) ? 0u : (left >= TOKENS ? (1u << TOKENS) - 1 : (1u << left) - 1);
+    if (bits) {
       if (!dead) dead = !mbar_wait(&full[warp][stage], (taken >> stage) & 1);
       taken ^= 1u << stage;
       if (bits != (1u << TOKENS) - 1) {
@@ -598,13 +615,13 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   Sums sums;
   int stage = 0;
   for (;;) {
-    const int g = (int)(at.item / a.groups), h0 = (int)(at.item % a.groups) * ROWS, rows = min(ROWS, R - h0), h = g * R + h0;
+    const int g = at.head, h0 = (at.item - g * a.groups) * ROWS, rows = min(ROWS, R - h0), h = g * R + h0;
     if (tid == 0 && at.item == 0 && at.from == 0 && a.pos[at.b] >= (long long)a.width * a.page) atomicAdd(&g_decode_faults, 1u);
     sums.start(static_cast<const T *>(a.q) + at.b * a.ldq + h * a.hq, a.hq, rows, a.D);
 #pragma unroll 1
     for (int i = 0; i < at.tiles; ++i) {
       load(stage == 0 ? STAGES - 1 : stage - 1);
-      const unsigned bits = arrived(stage);
+      const unsigned bits = arrived(stage, i);
       if (bits) sums.tile(warp_ring + stage * 2 * TILE, warp_ring + stage * 2 * TILE + TILE, bits, c, a.D);
       __syncwarp();
       stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -851,7 +868,7 @@ extern "C" int djv_paged_attention(int dtype, void *out, const void *q, long lon
     set_error("paged_attention: scratch of %zu bytes, %zu needed, 16-byte aligned", scratch_bytes, need);
     return DJV_ERR_SCRATCH;
   }
-  const DecodeArgs a{out, q, k_pages, v_pages, ldq, hq, {ld_page, ld_head, ld_slot}, pages, page, table, ld_table, width, pos,
+  const DecodeArgs a{out, q, k_pages, v_pages, ldq, hq, {ld_page, ld_head, ld_slot}, pages, page, divider_of(page), table, ld_table, width, pos,
                      B, H, G, D, scale, nullptr, 1};
   const cudaError_t e = decode_form(
       dtype, D, [&](auto t, auto dp) { return launch_decode<decltype(t), decltype(dp)::value>(a, scratch, static_cast<cudaStream_t>(stream)); });

@@ -5,17 +5,36 @@
 
 namespace djv {
 
+// Division of numbers below 2^31 by a fixed one from 1 to 2^31 - 1: t / d = (t * times) >> (32 + shift), times = floor(2^(32 + shift) / d) + 1
+// with 2^shift < d <= 2^(shift + 1). (times * d exceeds 2^(32 + shift) by at most d <= 2^(shift + 1), which t < 2^31 keeps below one.)
+struct Divider {
+  unsigned times;
+  int shift;  // -1: by 1
+};
+inline Divider divider_of(unsigned d) {
+  Divider v{0, -1};
+  if (d == 1) return v;
+  while ((2ull << (v.shift + 1)) < d) ++v.shift;
+  ++v.shift;
+  v.times = (unsigned)((1ull << (32 + v.shift)) / d + 1);
+  return v;
+}
+DJV_HOST_DEVICE unsigned divided(unsigned t, const Divider &v) {
+  return v.shift < 0 ? t : (unsigned)(((unsigned long long)t * v.times) >> 32) >> v.shift;
+}
+
 // Where tokens of a paged cache are.
 struct PageMap {
   const int *table;  // this sequence's row
   int width, page, pages;
+  Divider by_page;
 };
 constexpr long long NO_PAGE = -1;
 // Page of token t >= 0, or NO_PAGE where the table has none for it. slot receives its place in the page.
 DJV_HOST_DEVICE long long page_of(const PageMap &m, long long t, int &slot) {
   slot = 0;
   if (t < 0 || t >= (long long)m.width * m.page) return NO_PAGE;
-  const unsigned i = (unsigned)t / (unsigned)m.page;  // (a table has room for less than 2^31 tokens)
+  const unsigned i = divided((unsigned)t, m.by_page);  // (a table has room for less than 2^31 tokens)
   slot = (int)((unsigned)t - i * (unsigned)m.page);
   const int entry = m.table[i];
   return entry >= 0 && entry < m.pages ? entry : NO_PAGE;

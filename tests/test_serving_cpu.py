@@ -113,7 +113,7 @@ def test_pages_of_tokens(tmp_path):
     compiled(tmp_path, """
   const int table[6] = {3, -1, 9, 10, INT_MAX, INT_MIN};
   for (int page : {1, 3, 16, 1000}) {
-    const PageMap m{table, 6, page, 10};
+    const PageMap m{table, 6, page, 10, divider_of(page)};
     const long long want[6] = {3, NO_PAGE, 9, NO_PAGE, NO_PAGE, NO_PAGE};
     for (long long t = 0; t < 6ll * page; ++t) {
       int slot;
@@ -123,6 +123,28 @@ def test_pages_of_tokens(tmp_path):
       int slot;
       CHECK(page_of(m, t, slot) == NO_PAGE)
     }
+  }""")
+
+
+def test_division_by_a_page(tmp_path):
+    compiled(tmp_path, """
+  unsigned r = 12345;
+  for (unsigned d = 1; d < 5000; ++d) {
+    const Divider v = divider_of(d);
+    for (unsigned t = 0; t < 300; ++t) CHECK(divided(t, v) == t / d)
+    for (unsigned k = 1; k < 40; ++k)
+      for (int e = -1; e <= 1; ++e) {
+        const unsigned t = (unsigned)(((unsigned long long)d * k * 997 + e) % 0x7fffffffu);
+        CHECK(divided(t, v) == t / d)
+      }
+    for (unsigned t : {0x7fffffffu, 0x7ffffffeu, 0x7fffffffu / d * d, 0x7fffffffu / d * d - 1}) CHECK(divided(t, v) == t / d)
+  }
+  for (int i = 0; i < 2000000; ++i) {
+    r = r * 1664525u + 1013904223u;
+    const unsigned d = (r >> (r % 31)) % 0x7fffffffu + 1;
+    r = r * 1664525u + 1013904223u;
+    const unsigned t = r >> 1;
+    CHECK(divided(t, divider_of(d)) == t / d)
   }""")
 
 
