@@ -1,8 +1,9 @@
 // New tokens enter a paged cache: rotation of q and k, store of k and v into their pages, in one pass over the rows.
 //
-// A block takes one row: its angles are shared by all heads. The row is in registers before the angles are known (16-byte loads that
-// depend on nothing), so what a block waits for is one round of loads, the position's own short chain beside it, and its stores.
-// Bound by HBM for prompts, by that one round for a few rows.
+// A block of 128 threads takes one row: its angles are shared by all heads. What it reads of q, k and v, 16 bytes at a time, depends on
+// nothing and is asked for first; beside it runs the chain offsets -> position -> angles, page, which every warp goes through for
+// itself, so that the block meets once, over the angles. Small blocks, many of them on a multiprocessor, hide that chain.
+// Bound by HBM for prompts, by the chain for a few rows. Layouts that 16-byte accesses cannot read go element by element.
 //
 // Angles: position * frequency is exact in 64 bits up to positions of 2^29; what is left of it after whole turns are taken off in 64
 // bits is rounded to 32 and goes through sincosf, so that far positions are as exact as near ones (in 32 bits the angle of position
@@ -34,12 +35,25 @@ struct AppendArgs {
   int half, B, H, G, D;
 };
 
-// Row t's position and page, by one thread. p < 0: no such token.
+// sequence_of, by a warp: 32 offsets at a time.
+__device__ __forceinline__ int warp_sequence_of(const int *cu, int B, int t) {
+  const int lane = threadIdx.x % WARP;
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + WARP - 1) / WARP, at = lo + (lane + 1) * step;
+    const unsigned not_after = __ballot_sync(0xffffffffu, at < hi && cu[at] <= t);
+    lo += (32 - __clz(not_after)) * step;  // (ascending offsets: the lanes up to the last one)
+    hi = min(hi, lo + step);
+  }
+  return cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+}
+
+// Row t's position and page, by all lanes of a warp. p < 0: no such token.
 struct AppendPlace {
   long long p, at;  // at: offset of (page, slot), head 0, or -1
 };
 __device__ __forceinline__ AppendPlace append_place(const AppendArgs &a, int t) {
-  const int b = a.cu == nullptr ? t : sequence_of(a.cu, a.B, t);
+  const int b = a.cu == nullptr ? t : warp_sequence_of(a.cu, a.B, t);
   AppendPlace w{-1, -1};
   if (b < 0) return w;
   w.p = a.pos[b] + (a.cu == nullptr ? 0 : t - a.cu[b]);
@@ -47,8 +61,8 @@ __device__ __forceinline__ AppendPlace append_place(const AppendArgs &a, int t) 
   int slot;
   const PageMap m{a.table + b * a.ld_table, a.width, a.page, a.pages, a.by_page};
   const long long page = page_of(m, w.p, slot);
-  if (page == NO_PAGE) atomicAdd(&g_append_faults, 1u);
-  else w.at = page * a.pool.ld_page + slot * a.pool.ld_slot;
+  if (page != NO_PAGE) w.at = page * a.pool.ld_page + slot * a.pool.ld_slot;
+  else if (threadIdx.x == 0) atomicAdd(&g_append_faults, 1u);
   return w;
 }
 
@@ -67,12 +81,9 @@ __device__ __forceinline__ void append_angles(const AppendArgs &a, long long p, 
 template <typename T>
 __global__ void append_simple_kernel(AppendArgs a, int interleaved) {
   __shared__ float cs[2 * AP_MAX_HALF];
-  __shared__ AppendPlace place;
   pdl_prologue();
   const int t = blockIdx.x;
-  if (threadIdx.x == 0) place = append_place(a, t);
-  __syncthreads();
-  const AppendPlace w = place;
+  const AppendPlace w = append_place(a, t);
   if (a.half && w.p >= 0) append_angles(a, w.p, cs);
   __syncthreads();
   const int heads = a.q_out ? a.H : 0, total = (heads + 2 * a.G) * a.D;
@@ -100,6 +111,118 @@ __global__ void append_simple_kernel(AppendArgs a, int interleaved) {
       static_cast<T *>(a.v_pages)[w.at + (h - heads - a.G) * a.pool.ld_head + d] = r;
     }
   }
+}
+
+constexpr int AP_THREADS = 128, AP_DEEP = 4;  // pieces of a thread that are asked for before the angles are known
+
+// 16 bytes at a time. A piece is two chunks that are rotated with each other, one of neighbouring pairs (NEXT), or one that is copied.
+template <typename T, bool NEXT>
+__global__ void __launch_bounds__(AP_THREADS) append_kernel(AppendArgs a) {
+  constexpr int N = Chunk<T>::N;
+  extern __shared__ float cs[];  // cos[half], sin[half]
+  pdl_prologue();
+  const int t = blockIdx.x, heads = a.q_out ? a.H : 0;
+  const int rot = (NEXT ? 2 * a.half : a.half) / N, rest = (a.D - 2 * a.half) / N, whole = a.D / N;  // pieces of a head
+  const int n_rot = (heads + a.G) * rot, n_rest = (heads + a.G) * rest, total = n_rot + n_rest + a.G * whole;
+  struct Piece {
+    int h, d;  // head: q's, then k's, then v's; first dimension
+    bool turned;
+  };
+  auto piece = [&](int i) {
+    Piece p;
+    if (i < n_rot) {
+      p.h = i / rot;
+      p.d = (i - p.h * rot) * N;
+      p.turned = true;
+    } else if (i < n_rot + n_rest) {
+      i -= n_rot;
+      p.h = i / rest;
+      p.d = 2 * a.half + (i - p.h * rest) * N;
+      p.turned = false;
+    } else {
+      i -= n_rot + n_rest;
+      p.h = i / whole;
+      p.d = (i - p.h * whole) * N;
+      p.h += heads + a.G;
+      p.turned = false;
+    }
+    return p;
+  };
+  auto source = [&](const Piece &p) {
+    return (p.h < heads ? static_cast<const T *>(a.q) + (long long)t * a.ldq + p.h * a.hq
+            : p.h < heads + a.G ? static_cast<const T *>(a.k) + (long long)t * a.ldk + (p.h - heads) * a.hk
+                                : static_cast<const T *>(a.v) + (long long)t * a.ldv + (p.h - heads - a.G) * a.hv) + p.d;
+  };
+  auto ask = [&](int i, uint4 &x, uint4 &y) {
+    if (i >= total) return;
+    const Piece p = piece(i);
+    const T *src = source(p);
+    x = ld_cached16(src);
+    if (!NEXT && p.turned) y = ld_cached16(src + a.half);
+  };
+  uint4 x[AP_DEEP] = {}, y[AP_DEEP] = {};
+#pragma unroll
+  for (int i = 0; i < AP_DEEP; ++i) ask(i * AP_THREADS + threadIdx.x, x[i], y[i]);
+  const AppendPlace w = append_place(a, t);
+  if (w.p >= 0) append_angles(a, w.p, cs);
+  __syncthreads();
+  auto put = [&](int i, uint4 x, uint4 y) {
+    if (i >= total) return;
+    const Piece p = piece(i);
+    const bool two = !NEXT && p.turned;
+    if (w.p < 0) {
+      x = y = make_uint4(0, 0, 0, 0);
+    } else if (p.turned) {
+      float u[N], v[N];
+      T ru[N], rv[N];
+      unpack_chunk<T>(x, u);
+      if (NEXT) {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+          const float c = cs[(p.d + e) / 2], s = cs[a.half + (p.d + e) / 2];
+          ru[e] = from_f<T>(u[e] * c - u[e + 1] * s);
+          ru[e + 1] = from_f<T>(u[e + 1] * c + u[e] * s);
+        }
+      } else {
+        unpack_chunk<T>(y, v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float c = cs[p.d + e], s = cs[a.half + p.d + e];
+          ru[e] = from_f<T>(u[e] * c - v[e] * s);
+          rv[e] = from_f<T>(v[e] * c + u[e] * s);
+        }
+        y = *reinterpret_cast<uint4 *>(rv);
+      }
+      x = *reinterpret_cast<uint4 *>(ru);
+    }
+    auto store = [&](T *dst) {
+      *reinterpret_cast<uint4 *>(dst) = x;
+      if (two) *reinterpret_cast<uint4 *>(dst + a.half) = y;
+    };
+    if (p.h < heads) {
+      store(static_cast<T *>(a.q_out) + ((long long)t * a.H + p.h) * a.D + p.d);
+    } else if (p.h < heads + a.G) {
+      const int g = p.h - heads;
+      if (a.k_out) store(static_cast<T *>(a.k_out) + ((long long)t * a.G + g) * a.D + p.d);
+      if (w.at >= 0) store(static_cast<T *>(a.k_pages) + w.at + g * a.pool.ld_head + p.d);
+    } else if (w.at >= 0) {
+      store(static_cast<T *>(a.v_pages) + w.at + (p.h - heads - a.G) * a.pool.ld_head + p.d);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < AP_DEEP; ++i) put(i * AP_THREADS + threadIdx.x, x[i], y[i]);
+  for (int i = AP_DEEP * AP_THREADS + threadIdx.x; i < total; i += AP_THREADS) {
+    uint4 p = {}, q = {};
+    ask(i, p, q);
+    put(i, p, q);
+  }
+}
+
+template <typename T>
+static cudaError_t launch_append(const AppendArgs &a, int rows, bool vec, int interleaved, cudaStream_t st) {
+  if (!vec) return djv::launch_kernel(append_simple_kernel<T>, dim3(rows), dim3(256), 0, st, a, interleaved);
+  return interleaved ? djv::launch_kernel(append_kernel<T, true>, dim3(rows), dim3(AP_THREADS), a.half * 8, st, a)
+                     : djv::launch_kernel(append_kernel<T, false>, dim3(rows), dim3(AP_THREADS), a.half * 8, st, a);
 }
 
 unsigned append_faults() {
@@ -139,9 +262,12 @@ extern "C" int djv_paged_append(int dtype, void *q_out, void *k_out, const void 
   const AppendArgs a{q_out, k_out, k_pages, v_pages, q, k, v, ldq, hq, ldk, hk, ldv, hv, {ld_page, ld_head, ld_slot}, pages, page,
                      divider_of(page), table, ld_table, width, pos, cu, freqs, amp, half, B, H, G, D};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == DJV_DTYPE_F16) djv::launch_kernel(append_simple_kernel<__half>, dim3(T), dim3(256), 0, st, a, interleaved);
-  else if (dtype == DJV_DTYPE_BF16) djv::launch_kernel(append_simple_kernel<bf16>, dim3(T), dim3(256), 0, st, a, interleaved);
-  else djv::launch_kernel(append_simple_kernel<float>, dim3(T), dim3(256), 0, st, a, interleaved);
+  const auto fits = [&](const void *p, long long ld, long long head) { return aligned16(p) && ld % chunk == 0 && head % chunk == 0; };
+  const bool vec = fits(k, ldk, hk) && fits(v, ldv, hv) && (!q_out || (fits(q, ldq, hq) && aligned16(q_out))) && aligned16(k_out) &&
+                   (interleaved ? 2 * half : half) % chunk == 0;
+  if (dtype == DJV_DTYPE_F16) launch_append<__half>(a, T, vec, interleaved, st);
+  else if (dtype == DJV_DTYPE_BF16) launch_append<bf16>(a, T, vec, interleaved, st);
+  else launch_append<float>(a, T, vec, interleaved, st);
   count_launch();
   return check_launch("paged_append");
 }

@@ -850,47 +850,50 @@ def moe_decode(x, z, w_gu, w_down, top: int, shared_gu=None, shared_down=None, i
 # ---- requests of different lengths: paged caches, packed prompts, sampling (fp16, bf16 or fp32) ------------------------------
 
 _CODES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+_UNIT = {torch.float16: 7, torch.bfloat16: 7, torch.float32: 3}  # elements of 16 bytes, less one
 
 
-def _device_of(*tensors):
-    """A block in which the device of the tensors, one for all, is the current one."""
-    _require_cuda(*tensors)
-    devices = {t.device.index for t in tensors if t is not None}
-    assert len(devices) == 1, f"tensors on several devices: {sorted(devices)}"
-    device = devices.pop()
-    return contextlib.nullcontext() if device == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def _place(*tensors) -> int:
+    """The CUDA device of the tensors, one for all."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            _require_cuda(*tensors)
+            raise AssertionError(f"tensors on several devices: {sorted({t.get_device() for t in tensors if t is not None})}")
+    if device < 0:
+        _require_cuda(*tensors)
+    return device
 
 
-def _one_type(*tensors) -> int:
-    dtype = tensors[0].dtype
+def _code(dtype) -> int:
     assert dtype in _CODES, f"fp16, bf16 or fp32 expected, got {dtype}"
-    assert all(t is None or t.dtype == dtype for t in tensors), f"one type expected, got {[t.dtype for t in tensors if t is not None]}"
     return _CODES[dtype]
 
 
 def _last_adjacent(t):
     """t, or a copy of it, whose last dimension is contiguous."""
-    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _pages(k_pages, v_pages, table, pos, G: int, D: int):
+def _pages(k_pages, v_pages, table, pos, dtype, G: int, D: int):
     """Checks a paged cache against what is stored in it; its arguments of the C ABI."""
     P, heads, page, dim = k_pages.shape
-    assert (heads, dim) == (G, D) and v_pages.shape == k_pages.shape, f"pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} for {G} heads of {D}"
-    assert v_pages.stride() == k_pages.stride() and k_pages.stride(3) == 1, "K and V pages have one layout, dimensions adjacent"
-    unit = 16 // k_pages.element_size()
-    assert D % unit == 0 and all(s % unit == 0 for s in k_pages.stride()[:3]), f"rows of a page start on multiples of {unit} elements"
-    assert k_pages.data_ptr() % 16 == 0 and v_pages.data_ptr() % 16 == 0, "pages start on multiples of 16 bytes"
+    ld_page, ld_head, ld_slot, one = strides = k_pages.stride()
     B, width = table.shape
-    assert table.dtype == torch.int32 and width >= 1 and (table.stride(1) == 1 or width == 1), "table: (B, width) int32, rows of adjacent entries"
+    k_at, v_at, unit = k_pages.data_ptr(), v_pages.data_ptr(), _UNIT[dtype]
+    assert k_pages.dtype is dtype and v_pages.dtype is dtype, f"pages of {k_pages.dtype} and {v_pages.dtype} for {dtype}"
+    assert heads == G and dim == D and v_pages.shape == k_pages.shape, f"pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} for {G} heads of {D}"
+    assert v_pages.stride() == strides and one == 1, "K and V pages have one layout, dimensions adjacent"
+    assert not (D | ld_page | ld_head | ld_slot) & unit, f"rows of a page start on multiples of {unit + 1} elements"
+    assert not (k_at | v_at) & 15, "pages start on multiples of 16 bytes"
+    assert table.dtype is torch.int32 and width >= 1 and (table.stride(1) == 1 or width == 1), "table: (B, width) int32, rows of adjacent entries"
     assert width * page < 2 ** 31, "more than 2^31 tokens per sequence"
-    assert pos.shape == (B,) and pos.dtype == torch.int64 and pos.is_contiguous(), "pos: (B,) int64"
-    return (k_pages.data_ptr(), v_pages.data_ptr(), *k_pages.stride()[:3], P, page, table.data_ptr(), table.stride(0), width,
-            pos.data_ptr())
+    assert pos.shape == (B,) and pos.dtype is torch.int64 and pos.is_contiguous(), "pos: (B,) int64"
+    return k_at, v_at, ld_page, ld_head, ld_slot, P, page, table.data_ptr(), table.stride(0), width, pos.data_ptr()
 
 
 def _cumulative(cu_seqlens) -> int:
-    assert cu_seqlens.dim() == 1 and cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.numel() >= 2, \
+    assert cu_seqlens.dim() == 1 and cu_seqlens.dtype is torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.numel() >= 2, \
         "cu_seqlens: (B + 1,) int32"
     return cu_seqlens.numel() - 1
 
@@ -906,29 +909,36 @@ def paged_append(q, k, v, k_pages, v_pages, table, pos, cu_seqlens=None, freqs=N
     Returns q rotated (T, H, D), or None without q, and with `keys` the rotated k (T, G, D), for packed_attention, else None. Rows of
     no sequence and rows at negative positions (padding of a batch) are not stored and come back as zeros. Table entries that are no
     page are not stored to but counted (paged_faults)."""
+    device = _place(k, v, q, k_pages, v_pages, table, pos, cu_seqlens, freqs)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return paged_append(q, k, v, k_pages, v_pages, table, pos, cu_seqlens, freqs, amp, interleaved, keys)
     T, G, D = k.shape
-    assert v.shape == k.shape and (q is None or (q.dim() == 3 and q.shape[0] == T and q.shape[2] == D)), "q (T, H, D), k and v (T, G, D)"
-    code = _one_type(k, v, q, k_pages, v_pages)
-    with _device_of(k, v, q, k_pages, v_pages, table, pos, cu_seqlens, freqs):
-        q, k, v = _last_adjacent(q), _last_adjacent(k), _last_adjacent(v)
-        pages = _pages(k_pages, v_pages, table, pos, G, D)
-        B = table.shape[0]
-        if cu_seqlens is None:
-            assert T == B, f"{T} rows of {B} sequences"
-        else:
-            assert _cumulative(cu_seqlens) == B, "cu_seqlens and table are of one batch"
-        half = 0
-        if freqs is not None:
-            _f32(freqs)
-            half = freqs.numel()
-            assert freqs.dim() == 1 and 2 * half <= D, f"{2 * half} rotary dimensions in heads of {D}"
-        H = 0 if q is None else q.shape[1]
-        q_out = None if q is None else torch.empty(T, H, D, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(T, G, D, dtype=k.dtype, device=k.device) if keys else None
-        if T:
-            call("djv_paged_append", code, _ptr(q_out), _ptr(k_out), _ptr(q), 0 if q is None else q.stride(0),
-                 0 if q is None else q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *pages,
-                 _ptr(cu_seqlens), _ptr(freqs), float(amp), half, int(interleaved), B, T, H, G, D, _stream())
+    dtype = k.dtype
+    code = _code(dtype)
+    assert v.shape == k.shape and v.dtype is dtype, "k and v: (T, G, D) of one type"
+    pages = _pages(k_pages, v_pages, table, pos, dtype, G, D)
+    B = table.shape[0]
+    if cu_seqlens is None:
+        assert T == B, f"{T} rows of {B} sequences"
+    else:
+        assert _cumulative(cu_seqlens) == B, "cu_seqlens and table are of one batch"
+    half = 0
+    if freqs is not None:
+        half = freqs.numel()
+        assert freqs.dim() == 1 and freqs.dtype is torch.float32 and freqs.is_contiguous(), "freqs: (half,) fp32"
+        assert 2 * half <= D, f"{2 * half} rotary dimensions in heads of {D}"
+    k, v = _last_adjacent(k), _last_adjacent(v)
+    H, q_out, query_args = 0, None, (None, 0, 0)
+    if q is not None:
+        rows, H, dim = q.shape
+        assert rows == T and dim == D and H >= 1 and q.dtype is dtype, f"q: ({T}, H, {D}) {dtype}"
+        q = _last_adjacent(q)
+        q_out, query_args = q.new_empty(T, H, D), (q.data_ptr(), q.stride(0), q.stride(1))
+    k_out = k.new_empty(T, G, D) if keys else None
+    if T:
+        call("djv_paged_append", code, _ptr(q_out), _ptr(k_out), *query_args, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+             v.stride(0), v.stride(1), *pages, _ptr(cu_seqlens), _ptr(freqs), float(amp), half, int(interleaved), B, T, H, G, D, _stream())
     return q_out, k_out
 
 
@@ -937,23 +947,28 @@ def paged_attention(q, k_pages, v_pages, table, pos, scale: float):
     0 .. pos[b] (int64), its own among them, in k_pages, v_pages (P, G, page, D) by table (B, width) int32; H a multiple of G, D at
     most 256. Returns (B, H, D). A sequence at position -1 gets zeros; table entries that are no page are not seen and counted
     (paged_faults)."""
+    device = _place(q, k_pages, v_pages, table, pos)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return paged_attention(q, k_pages, v_pages, table, pos, scale)
     B, H, D = q.shape
-    G = k_pages.shape[1]
-    assert H >= 1 and H % G == 0, f"{H} query heads over {G} key/value heads"
+    G, page = k_pages.shape[1:3]
+    dtype = q.dtype
+    code = _code(dtype)
+    assert H >= 1 and G >= 1 and H % G == 0, f"{H} query heads over {G} key/value heads"
     assert D <= 256, f"heads of {D}"
     assert table.shape[0] == B, "q and table are of one batch"
-    code = _one_type(q, k_pages, v_pages)
-    with _device_of(q, k_pages, v_pages, table, pos):
-        unit = 16 // q.element_size()
-        if q.stride(2) != 1 or q.stride(0) % unit or q.stride(1) % unit or q.data_ptr() % 16:
-            q = q.clone(memory_format=torch.contiguous_format)
-        pages = _pages(k_pages, v_pages, table, pos, G, D)
-        out = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
-        if B:
-            need = query("djv_paged_attention_scratch_bytes", code, B, H, G, D, k_pages.shape[2], table.shape[1])
-            scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None  # (one for each call: captured ones keep theirs)
-            call("djv_paged_attention", code, out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), *pages, B, H, G, D, float(scale),
-                 _ptr(scratch), need, _stream())
+    pages = _pages(k_pages, v_pages, table, pos, dtype, G, D)
+    ld, head, one = q.stride()
+    if one != 1 or (ld | head) & _UNIT[dtype] or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+        ld, head, one = q.stride()
+    out = q.new_empty(B, H, D)
+    if B:
+        need = query("djv_paged_attention_scratch_bytes", code, B, H, G, D, page, table.shape[1])
+        scratch = None if need == 0 else q.new_empty(need, dtype=torch.uint8)  # (one for each call: captured ones keep theirs)
+        call("djv_paged_attention", code, out.data_ptr(), q.data_ptr(), ld, head, *pages, B, H, G, D, float(scale), _ptr(scratch), need,
+             _stream())
     return out
 
 
@@ -966,23 +981,27 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     """Causal attention over whole prompts, packed row after row (djv_packed_attention): rows cu[b] .. cu[b + 1] - 1 of q (T, H, D), k
     and v (T, G, D) are sequence b, cu_seqlens (B + 1,) int32. H a multiple of G, D at most 256; any row and head strides. Returns
     (T, H, D). Rows of no sequence are zeros or, with `out` given (T, H, D, contiguous), left as they are."""
+    device = _place(q, k, v, cu_seqlens, out)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return packed_attention(q, k, v, cu_seqlens, scale, out)
     T, H, D = q.shape
     G = k.shape[1]
-    assert k.shape == v.shape == (T, G, D) and G >= 1, "q (T, H, D), k and v (T, G, D)"
+    dtype = q.dtype
+    code = _code(dtype)
+    assert k.shape == v.shape == (T, G, D) and G >= 1 and k.dtype is dtype and v.dtype is dtype, "q (T, H, D), k and v (T, G, D) of one type"
     assert H >= 1 and H % G == 0, f"{H} query heads over {G} key/value heads"
     assert 1 <= D <= 256, f"heads of {D}"
     B = _cumulative(cu_seqlens)
-    code = _one_type(q, k, v, out)
-    with _device_of(q, k, v, cu_seqlens, out):
-        q, k, v = _last_adjacent(q), _last_adjacent(k), _last_adjacent(v)
-        keep = out is not None
-        if keep:
-            assert out.shape == (T, H, D) and out.is_contiguous(), "out (T, H, D), contiguous"
-        else:
-            out = torch.empty(T, H, D, dtype=q.dtype, device=q.device)
-        if T:
-            call("djv_packed_attention", code, out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-                 v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens.data_ptr(), B, T, H, G, D, float(scale), int(keep), _stream())
+    q, k, v = _last_adjacent(q), _last_adjacent(k), _last_adjacent(v)
+    keep = out is not None
+    if keep:
+        assert out.shape == (T, H, D) and out.is_contiguous() and out.dtype is dtype, f"out: ({T}, {H}, {D}) {dtype}, contiguous"
+    else:
+        out = q.new_empty(T, H, D)
+    if T:
+        call("djv_packed_attention", code, out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
+             v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens.data_ptr(), B, T, H, G, D, float(scale), int(keep), _stream())
     return out
 
 
@@ -991,13 +1010,12 @@ def _bits(x: float) -> int:
     return struct.unpack("q", struct.pack("d", x))[0]
 
 
-def _setting(name: str, value, dtype, B: int, device):
-    """A setting of sample_tokens: (array or None, number)."""
+def _setting(name: str, value, dtype, B: int):
+    """A setting of sample_tokens: its array, or None."""
     if not torch.is_tensor(value):
-        return None, value
-    assert value.shape == (B,) and value.dtype == dtype and value.is_contiguous(), f"{name}: a number or ({B},) {dtype}"
-    assert value.device == device, f"{name} on {value.device}, logits on {device}"
-    return value.data_ptr(), 0
+        return None
+    assert value.shape == (B,) and value.dtype is dtype and value.is_contiguous(), f"{name}: a number or ({B},) {dtype}"
+    return value
 
 
 def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -1009,18 +1027,21 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     the others fp32). Returns (B,) int64, -1 for a row without entries."""
     assert logits.dim() == 2 and logits.shape[1] >= 1, f"logits (B, V), got {tuple(logits.shape)}"
     B, V = logits.shape
-    code = _one_type(logits)
-    assert uniform.shape == (B,) and uniform.dtype == torch.float32 and uniform.is_contiguous(), f"uniform ({B},) fp32"
-    with _device_of(logits, uniform):
-        if logits.stride(1) != 1 or logits.stride(0) < V:
-            logits = logits.contiguous()
-        dev = logits.device
-        t, t_all = _setting("temperature", temperature, torch.float32, B, dev)
-        k, k_all = _setting("top_k", top_k, torch.int32, B, dev)
-        p, p_all = _setting("top_p", top_p, torch.float32, B, dev)
-        m, m_all = _setting("min_p", min_p, torch.float32, B, dev)
-        token = torch.empty(B, dtype=torch.int64, device=dev)
-        if B:
-            call("djv_sample", code, token.data_ptr(), logits.data_ptr(), max(logits.stride(0), V), uniform.data_ptr(), t, _bits(t_all), k,
-                 min(int(k_all), 2 ** 31 - 1), p, _bits(p_all), m, _bits(m_all), B, V, _stream())
+    t, k = _setting("temperature", temperature, torch.float32, B), _setting("top_k", top_k, torch.int32, B)
+    p, m = _setting("top_p", top_p, torch.float32, B), _setting("min_p", min_p, torch.float32, B)
+    device = _place(logits, uniform, t, k, p, m)
+    if device != torch._C._cuda_getDevice():
+        with torch.cuda.device(device):
+            return sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
+    code = _code(logits.dtype)
+    assert uniform.shape == (B,) and uniform.dtype is torch.float32 and uniform.is_contiguous(), f"uniform: ({B},) fp32"
+    ld, one = logits.stride()
+    if one != 1 and V > 1 or ld < V:
+        logits = logits.contiguous()
+        ld = V
+    token = logits.new_empty(B, dtype=torch.int64)
+    if B:
+        call("djv_sample", code, token.data_ptr(), logits.data_ptr(), ld, uniform.data_ptr(), _ptr(t), 0 if t is not None else _bits(temperature),
+             _ptr(k), 0 if k is not None else min(int(top_k), 2 ** 31 - 1), _ptr(p), 0 if p is not None else _bits(top_p), _ptr(m),
+             0 if m is not None else _bits(min_p), B, V, _stream())
     return token
