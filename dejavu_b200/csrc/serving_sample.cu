@@ -1,25 +1,36 @@
 // Sampling of one token per row of logits: temperature, top-k, top-p, min-p, from a given random number.
 //
 // Entries are ordered without being sorted. (logit, index) is a 64-bit number, larger for what comes first, so that every cut is a
-// threshold on it and ties need no rule of their own. A row is swept a few times (from L2 after the first):
-//   1. its largest entry;  2. a histogram of 2048 equal steps of the logit, counts only;
-//   3. what lies in the step of the k-th entry: collected and sorted in shared memory, which gives the threshold of top-k;
-//   4. the same for top-p, where counts and the steps' borders bound the sums from both sides: the entries between the bounds are
+// threshold on it and ties need no rule of their own. A cluster of up to 8 blocks takes a row, each a slice of it in shared memory:
+//   1. the slices arrive, and the row's largest entry;
+//   2. a histogram of 2048 equal steps of the logit: how many entries, and how far into the step they are on average;
+//   3. top-k: what lies in the step of the k-th entry, or, where few enough do, in all steps up to it, is collected in the first block and
+//      sorted there; top-p: count and average bound a step's weight from both sides (the exponential is convex; the bounds are a 10^-4th
+//      apart, where the steps' borders alone would leave thousands of entries between them), the entries between the bounds are
 //      collected, those outside summed;
-//   5. the sum of what is kept, warp by warp in index order, and the place where the running sum passes u times it.
-// If too many entries are in the way (ties), the range is cut into 2048 steps again, now of the 64-bit number, until few are left.
-// Weights are 32-bit numbers with an error of at most 4e-7 (exp2f's, beside an exponent that is kept in two terms), sums 64-bit
-// ones. A comparison that comes out closer than the weights' errors allow makes the row start again with 64-bit weights: the token is
-// that of the 64-bit definition.
+//   4. if all that can be kept is in the list, the first block makes the rest of it alone; else the sum of what is kept, warp by warp in
+//      index order, and the place where the running sum passes u times it.
+// Rows of more ties than the list takes, and comparisons that come out closer than the weights' errors allow (one row in many
+// thousands), go to one block, which reads the row from L2 as often as it needs, narrows the range by 2048 steps of the 64-bit number at
+// a time, and has weights from exp in 64 bits: the token is that of the 64-bit definition.
+//
+// Weights: 2^(y/64) from a table of 64-bit numbers, 2^f for the rest |f| <= 1/128 by its series in 32 bits, off by 1e-9 at most; sums have 64
+// bits. (32-bit weights would leave every tenth row of a flat distribution undecided.)
+//
+// Bound by latency: a row is read once, then swept four times in shared memory between block and cluster barriers.
 #include <math.h>
 #include <string.h>
+
+#include <cooperative_groups.h>
+#include <utility>
 
 #include "serving.cuh"
 
 namespace djv {
 
-constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / WARP, SA_BINS = 2048, SA_LIST = 2048;
-constexpr double SA_CLOSE = 8e-7;   // what counts as close, of a sum of 32-bit weights: twice their relative error
+constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / WARP, SA_BINS = 2048, SA_LIST = 2048, SA_CLUSTER = 8;
+constexpr int SA_EACH = SA_BINS / SA_THREADS;  // steps, or entries of the list, of a thread
+constexpr double SA_CLOSE = 3e-9;   // what counts as close, of a sum: three times the weights' relative error
 constexpr float SA_FAR = 45.f;      // temperatures below the largest entry from where on nothing counts (e^-45 = 3e-20)
 
 struct SampleArgs {
@@ -53,14 +64,25 @@ __device__ __forceinline__ u64 place_of(uint32_t key, int i) { return (u64)key <
 
 struct SampleShared {
   u64 list[SA_LIST];
-  unsigned count[SA_BINS];
-  double mass[SA_BINS];
-  double part[SA_WARPS];
+  union {
+    struct {
+      unsigned count[SA_BINS];  // of this block's slice
+      unsigned upto[SA_BINS];   // of the row, in this step and those in front of it
+    };
+    double mass[SA_BINS];       // (of a block that works alone)
+  };
+  unsigned into[SA_BINS];       // of this block's slice: sum of how far into the step entries are, `fine` to a step
+  double table[64];           // 2^(j / 64)
+  double part[SA_WARPS], part2[SA_WARPS];
   u64 wide[SA_WARPS];
+  // written by the blocks of the cluster
+  u64 best[SA_CLUSTER], least[SA_CLUSTER];
+  double sums[SA_CLUSTER][2], kept[SA_CLUSTER];
   int listed;
+  u64 cut;                    // by the first block: entries whose place is lower are dropped
+  int done;                   // by the first block: 1: it has the token, or finds it alone
   int found[4];
   u64 lo, hi, place;
-  double sums[3];
 };
 
 // ---- what a block does together -------------------------------------------------------------------------------------
@@ -124,28 +146,66 @@ __device__ void sort_list(SampleShared &s, int n) {
     }
 }
 
-// ---- one row ----------------------------------------------------------------------------------------------------------
-template <typename T, bool VEC>
-struct SampleRow {
-  const T *row;
-  int V;
-  SampleShared &s;
+// Sum of v over the threads in front of this one; total receives the block's.
+__device__ __forceinline__ double block_before(double v, double *slots, double &total) {
+  const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
+  double sum = v;
+#pragma unroll
+  for (int o = 1; o < WARP; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
+  }
+  __syncthreads();
+  if (lane == WARP - 1) slots[warp] = sum;
+  __syncthreads();
+  double before = sum - v;
+  total = 0;
+#pragma unroll 4
+  for (int w = 0; w < SA_WARPS; ++w) {
+    if (w < warp) before += slots[w];
+    total += slots[w];
+  }
+  return before;
+}
+
+// The largest entry of a row and what follows from it.
+struct SampleScale {
   float top, inv;       // largest logit, steps per unit of the logit
   double temperature;
   float c_hi, c_lo;     // log2(e) / temperature
   float reach;          // entries further below the largest are dropped
 
-  template <bool EXACT>
-  __device__ __forceinline__ double weight(float x) const {
-    if (x == top) return 1.0;  // (+inf among them)
-    if (EXACT) return exp(((double)x - (double)top) / temperature);
-    const float t = x - top, v = t - x, e = (x - (t - v)) - (top + v);  // x - top = t + e
-    const float y = t * c_hi, rest = fmaf(t, c_hi, -y) + fmaf(t, c_lo, e * c_hi);
-    const float w = exp2f(y);
-    return fmaf(w, rest * 0.69314718f, w);
-  }
   __device__ __forceinline__ bool counts(float x) const { return x >= -3.402823466e38f && !(top - x > reach); }
   __device__ __forceinline__ int bin_of(float x) const { return min(SA_BINS - 1, (int)((top - x) * inv)); }
+  // the same, and how far into the step x is, in parts of a step
+  __device__ __forceinline__ int bin_of(float x, float fine, unsigned &into) const {
+    const float at = (top - x) * inv;  // (NaN where both are infinite)
+    const int bin = min(SA_BINS - 1, (int)at);
+    into = (unsigned)((at - bin) * fine);
+    return bin;
+  }
+  __device__ __forceinline__ double exact(float x) const { return x == top ? 1.0 : exp(((double)x - (double)top) / temperature); }
+  // x counts: y = (x - top) log2(e) / temperature >= -65 as the sum of two floats, y = k / 64 + f
+  __device__ __forceinline__ double weight(float x, const double *table) const {
+    if (x == top) return 1.0;  // (+inf among them)
+    const float t = x - top, v = t - x, e = (x - (t - v)) - (top + v);  // x - top = t + e
+    const float y = t * c_hi, rest = fmaf(t, c_hi, -y) + fmaf(t, c_lo, e * c_hi);
+    const float k = rintf(y * 64.f);
+    const float f = (fmaf(k, -0.015625f, y) + rest) * 0.69314718f;  // (the difference is exact)
+    const float q = fmaf(f * f, fmaf(f, fmaf(f, 0.041666668f, 0.16666667f), 0.5f), f);  // e^f - 1
+    const int n = (int)k;
+    const double w = table[n & 63];
+    return __longlong_as_double(__double_as_longlong(fma(w, (double)q, w)) + ((long long)(n >> 6) << 52));
+  }
+};
+
+// One row by one block, in 64 bits, from global memory: nothing is too close and nothing too much.
+template <typename T, bool VEC>
+struct SampleAlone {
+  const T *row;
+  int V;
+  SampleShared &s;
+  SampleScale z;
 
   template <typename F>
   __device__ __forceinline__ void all(F f) const {
@@ -154,20 +214,16 @@ struct SampleRow {
 
   // Of the entries between places lo and hi (inclusive), those in front first: the place of entry number `rank` (from 0), or, by
   // mass, of the last entry in front of which less than `mass` lies. Cuts the range until what is left fits the list.
-  template <bool EXACT, bool MASS>
-  __device__ u64 narrow(u64 lo, u64 hi, int rank, double mass, double total, bool &close) {
+  template <bool MASS>
+  __device__ u64 narrow(u64 lo, u64 hi, int rank, double mass) {
     for (;;) {
       __syncthreads();
-      if (threadIdx.x == 0) {
-        s.listed = 0;
-        s.lo = ~0ull;
-        s.hi = 0;
-      }
+      if (threadIdx.x == 0) s.listed = 0;
       __syncthreads();
       u64 first = 0, last = ~0ull;
       all([&](float x, int i) {
         const u64 p = place_of(order_of(x), i);
-        if (p < lo || p > hi || !counts(x)) return;
+        if (p < lo || p > hi || !z.counts(x)) return;
         first = p > first ? p : first;
         last = p < last ? p : last;
         const int at = atomicAdd(&s.listed, 1);
@@ -181,24 +237,23 @@ struct SampleRow {
       int shift = 0;
       while (((hi - lo) >> shift) >= SA_BINS) ++shift;
       for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) {
-        s.count[i] = 0;
-        s.mass[i] = 0;
+        if (MASS) s.mass[i] = 0;
+        else s.count[i] = 0;
       }
       __syncthreads();
       all([&](float x, int i) {
         const u64 p = place_of(order_of(x), i);
-        if (p < lo || p > hi || !counts(x)) return;
+        if (p < lo || p > hi || !z.counts(x)) return;
         const int bin = (int)((hi - p) >> shift);
-        if (MASS) atomicAdd(&s.mass[bin], weight<EXACT>(x));
+        if (MASS) atomicAdd(&s.mass[bin], z.exact(x));
         else atomicAdd(&s.count[bin], 1u);
       });
       __syncthreads();
       if (threadIdx.x == 0) {
         int bin = 0;
         if (MASS) {  // the last step in front of which less than `mass` lies and that holds anything
-          double run = 0;
+          double run = 0, before = 0;
           int best = 0;
-          double before = 0;
           for (; bin < SA_BINS; ++bin) {
             if (s.mass[bin] == 0) continue;
             if (bin > 0 && run >= mass) break;
@@ -207,9 +262,7 @@ struct SampleRow {
             run += s.mass[bin];
           }
           s.found[0] = best;
-          s.sums[0] = before;
-          // the step's borders have to be clear of the errors
-          s.found[1] = !EXACT && (fabs(before - mass) <= SA_CLOSE * total || fabs(run - mass) <= SA_CLOSE * total);
+          s.sums[0][0] = before;
         } else {
           int run = 0;
           while (bin < SA_BINS - 1 && run + (int)s.count[bin] <= rank) run += s.count[bin++];
@@ -219,161 +272,79 @@ struct SampleRow {
       }
       __syncthreads();
       const int bin = s.found[0];
-      if (MASS) {
-        mass -= s.sums[0];
-        close |= s.found[1] != 0;
-      } else {
-        rank -= s.found[1];
-      }
+      if (MASS) mass -= s.sums[0][0];
+      else rank -= s.found[1];
       const u64 step = 1ull << shift, up = hi - (u64)bin * step;
       lo = up - lo >= step ? up - (step - 1) : lo;
       hi = up;
     }
     const int n = s.listed;
     sort_list(s, n);
-    if (!MASS) {
-      const u64 p = s.list[rank];
-      __syncthreads();
-      return p;
-    }
-    // running sums of the list's weights, a warp 32 at a time
-    if (threadIdx.x < WARP) {
-      double run = 0;
-      u64 place = s.list[0];
-      bool near = false;
-      for (int i0 = 0; i0 < n; i0 += WARP) {
-        const int i = i0 + threadIdx.x;
-        const double w = i < n ? weight<EXACT>(logit_of((uint32_t)(s.list[i] >> 32))) : 0.0;
-        double sum = w;
-#pragma unroll
-        for (int o = 1; o < WARP; o <<= 1) {
-          const double up = __shfl_up_sync(0xffffffffu, sum, o);
-          if ((int)threadIdx.x >= o) sum += up;
+    if (threadIdx.x == 0) {
+      int at = min(rank, n - 1);
+      if (MASS) {
+        double run = 0;
+        at = 0;
+        for (int i = 0; i < n && (i == 0 || run < mass); ++i) {
+          at = i;
+          run += z.exact(logit_of((uint32_t)(s.list[i] >> 32)));
         }
-        const double before = run + sum - w;
-        const bool in = i < n && (before < mass || i == 0);
-        near |= __any_sync(0xffffffffu, i < n && i > 0 && fabs(before - mass) <= SA_CLOSE * total) != 0;
-        const unsigned kept = __ballot_sync(0xffffffffu, in);
-        if (kept) place = s.list[i0 + 31 - __clz(kept)];
-        if (kept != 0xffffffffu) break;
-        run += __shfl_sync(0xffffffffu, sum, WARP - 1);
       }
-      if (threadIdx.x == 0) {
-        s.place = place;
-        s.found[0] = near;
-      }
+      s.place = s.list[at];
     }
     __syncthreads();
     const u64 place = s.place;
-    if (!EXACT) close |= s.found[0] != 0;
     __syncthreads();
     return place;
   }
 
-  // The place of the last entry that top-p keeps. cut: the place of the last one that top-k keeps. counts of the steps: s.count,
-  // those of the last step with any kept entry among them.
-  template <bool EXACT>
-  __device__ u64 nucleus(u64 cut, double p, bool &close) {
-    // bounds of the running sums at the steps' borders, by warp 0
-    const float width = inv > 0.f ? 1.f / inv : 0.f;
-    if (threadIdx.x < WARP) {
-      const int lane = threadIdx.x;
-      double total_lo = 0, total_hi = 0;
-      for (int b = lane; b < SA_BINS; b += WARP) {
-        if (!s.count[b]) continue;
-        total_hi += s.count[b] * exp2((double)c_hi * -(b * (double)width) * (1 - 1e-6));
-        total_lo += s.count[b] * exp2((double)c_hi * -((b + 1) * (double)width) * (1 + 1e-6));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        total_lo += __shfl_xor_sync(0xffffffffu, total_lo, o);
-        total_hi += __shfl_xor_sync(0xffffffffu, total_hi, o);
-      }
-      total_lo *= 1 - 1e-5;
-      total_hi *= 1 + 1e-5;
-      // first: the first step at whose end the sum can have reached p of the total; last: the first at whose end it has to have
-      double run_lo = 0, run_hi = 0;
-      int first = -1, last = -1, end = 0;
-      for (int b0 = 0; b0 < SA_BINS && last < 0; b0 += WARP) {
-        const int b = b0 + lane;
-        const unsigned n = s.count[b];
-        double hi = n ? n * exp2((double)c_hi * -(b * (double)width) * (1 - 1e-6)) * (1 + 1e-5) : 0.0;
-        double lo = n ? n * exp2((double)c_hi * -((b + 1) * (double)width) * (1 + 1e-6)) * (1 - 1e-5) : 0.0;
-#pragma unroll
-        for (int o = 1; o < WARP; o <<= 1) {
-          const double x = __shfl_up_sync(0xffffffffu, hi, o), y = __shfl_up_sync(0xffffffffu, lo, o);
-          if (lane >= o) {
-            hi += x;
-            lo += y;
-          }
-        }
-        const unsigned can = __ballot_sync(0xffffffffu, run_hi + hi >= p * total_lo), must = __ballot_sync(0xffffffffu, run_lo + lo >= p * total_hi);
-        const unsigned any = __ballot_sync(0xffffffffu, n != 0);
-        if (first < 0 && can) first = b0 + __ffs(can) - 1;
-        if (last < 0 && must) last = b0 + __ffs(must) - 1;
-        if (any) end = b0 + 31 - __clz(any);
-        run_hi += __shfl_sync(0xffffffffu, hi, WARP - 1);
-        run_lo += __shfl_sync(0xffffffffu, lo, WARP - 1);
-      }
-      if (lane == 0) {
-        s.found[0] = first < 0 ? end : first;
-        s.found[1] = last < 0 ? SA_BINS - 1 : last;
-      }
+  __device__ int token(int k, double p, double min_p, double u) {
+    u64 cut = 0;
+    const u64 most = place_of(order_of(z.top), 0);
+    if (k > 0 && k < V) {
+      int n = 0;
+      all([&](float x, int) { n += z.counts(x); });
+      if ((int)block_total(n, s) > k) cut = narrow<false>(0, most, k - 1, 0);
     }
-    __syncthreads();
-    const int first = s.found[0], last = s.found[1];
-    double in_front = 0, between = 0, behind = 0;
-    u64 hi = 0, lo = ~0ull;
-    all([&](float x, int i) {
-      if (!counts(x)) return;
-      const u64 at = place_of(order_of(x), i);
-      if (at < cut) return;
-      const int bin = bin_of(x);
-      const double w = weight<EXACT>(x);
-      if (bin < first) {
-        in_front += w;
-      } else if (bin > last) {
-        behind += w;
-      } else {
-        between += w;
-        hi = at > hi ? at : hi;
-        lo = at < lo ? at : lo;
-      }
-    });
-    in_front = block_total(in_front, s);
-    between = block_total(between, s);
-    behind = block_total(behind, s);
-    hi = block_all(hi, s.wide, [](u64 a, u64 b) { return a > b ? a : b; });
-    lo = block_all(lo, s.wide, [](u64 a, u64 b) { return a < b ? a : b; });
-    const double total = in_front + between + behind;
-    if (lo > hi) return cut;  // nothing between the bounds: no entry is dropped
-    return narrow<EXACT, true>(lo, hi, 0, p * total - in_front, total, close);
+    if (p < 1) {
+      double sum = 0;
+      all([&](float x, int i) {
+        if (z.counts(x) && place_of(order_of(x), i) >= cut) sum += z.exact(x);
+      });
+      cut = narrow<true>(cut, most, 0, p * block_total(sum, s));
+    }
+    return draw(row, 0, V, cut, u, min_p, [&](float x) { return z.exact(x); }, [&](float x) { return z.exact(x); });
   }
 
-  // The token: the first index at which the running sum of what is kept passes u times its total.
-  template <bool EXACT>
-  __device__ int draw(u64 cut, double u, double min_p, bool &close) {
+  // The first index of from .. to - 1 at which the running sum of what is kept passes u times its total.
+  template <typename W, typename E>
+  __device__ int draw(const T *entries, int from, int to, u64 cut, double u, double min_p, W weight, E exact) {
     const int warp = threadIdx.x / WARP, lane = threadIdx.x % WARP;
     constexpr int N = VEC ? Chunk<T>::N : 1;
-    const int share = ((V + SA_WARPS - 1) / SA_WARPS + WARP * N - 1) / (WARP * N) * (WARP * N);
-    const int lo = min(V, warp * share), hi = min(V, lo + share);
+    const int share = ((to - from + SA_WARPS - 1) / SA_WARPS + WARP * N - 1) / (WARP * N) * (WARP * N);
+    const int lo = min(to, from + warp * share), hi = min(to, lo + share);
     auto kept = [&](float x, int i) -> double {
-      if (!counts(x) || place_of(order_of(x), i) < cut) return 0.0;
-      const double w = weight<EXACT>(x);
-      if (min_p > 0 && w < min_p * (1 + 1e-5) && (w < min_p * (1 - 1e-5) || weight<true>(x) < min_p)) return 0.0;
+      if (!z.counts(x) || place_of(order_of(x), i) < cut) return 0.0;
+      const double w = weight(x);
+      if (min_p > 0 && w < min_p * (1 + 1e-8) && (w < min_p * (1 - 1e-8) || exact(x) < min_p)) return 0.0;
       return w;
     };
     double sum = 0;
-    sweep<T, VEC>(row, lo, hi, lane, WARP, [&](float x, int i) { sum += kept(x, i); });
+    sweep<T, VEC>(entries, lo, hi, lane, WARP, [&](float x, int i) { sum += kept(x, i); });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     __syncthreads();
     if (lane == 0) s.part[warp] = sum;
-    if (threadIdx.x == 0) s.found[0] = -1;
     __syncthreads();
-    double total = 0, before = 0, target;
+    double total = 0;
     for (int w = 0; w < SA_WARPS; ++w) total += s.part[w];
-    target = u * total;
+    return locate(entries, lo, hi, 0.0, u * total, total, kept);
+  }
+
+  // s.part has the warps' sums, `before` is in front of the first: where the running sum passes target. found[1]: too close to tell.
+  template <typename K>
+  __device__ int locate(const T *entries, int lo, int hi, double before, double target, double total, K kept) {
+    const int warp = threadIdx.x / WARP, lane = threadIdx.x % WARP;
     int mine = SA_WARPS;  // the warp whose part the target falls into: the first whose running sum exceeds it
     int last = 0;         // the last warp that keeps anything
     for (int w = 0; w < SA_WARPS; ++w) {
@@ -389,11 +360,12 @@ struct SampleRow {
     if (warp == mine) {
       double run = before;
       int token = -1, latest = -1;
-      bool near = false;
+      bool near = fabs(before - target) <= SA_CLOSE * total;
       for (int i0 = lo; i0 < hi && token < 0; i0 += WARP) {
         const int i = i0 + lane;
-        const double w = i < hi ? kept(to_f(row[i]), i) : 0.0;
-        if (__ballot_sync(0xffffffffu, w > 0) == 0) continue;
+        const double w = i < hi ? kept(to_f(entries[i]), i) : 0.0;
+        const unsigned any = __ballot_sync(0xffffffffu, w > 0);
+        if (any == 0) continue;
         double sum = w;
 #pragma unroll
         for (int o = 1; o < WARP; o <<= 1) {
@@ -402,151 +374,465 @@ struct SampleRow {
         }
         const unsigned over = __ballot_sync(0xffffffffu, w > 0 && run + sum > target);
         near |= __any_sync(0xffffffffu, w > 0 && fabs(run + sum - target) <= SA_CLOSE * total) != 0;
-        latest = i0 + 31 - __clz(__ballot_sync(0xffffffffu, w > 0));
+        latest = i0 + 31 - __clz(any);
         if (over) token = i0 + __ffs(over) - 1;
         run += __shfl_sync(0xffffffffu, sum, WARP - 1);
       }
       if (lane == 0) {
         s.found[0] = token >= 0 ? token : latest;
-        s.found[1] = near || fabs(before - target) <= SA_CLOSE * total;
+        s.found[1] = near;
       }
     }
     __syncthreads();
-    const int token = s.found[0];
-    if (!EXACT && mine != SA_WARPS) close |= s.found[1] != 0;
-    __syncthreads();
-    return token;
+    return s.found[0];
   }
 };
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  SampleShared &s = *reinterpret_cast<SampleShared *>(smem_raw);
-  pdl_prologue();
-  const int b = blockIdx.x;
-  const double temperature = a.temperature ? (double)a.temperature[b] : a.temperature0;
-  const double p = a.top_p ? (double)a.top_p[b] : a.top_p0, min_p = a.min_p ? (double)a.min_p[b] : a.min_p0;
-  const int k = a.top_k ? a.top_k[b] : a.top_k0;
-  const double u = a.u[b];
-  SampleRow<T, VEC> r{static_cast<const T *>(a.logits) + b * a.ld, a.V, s};
-  u64 best = 0;
-  uint32_t least = 0xffffffffu;
-  r.all([&](float x, int i) {
-    const uint32_t key = order_of(x);
-    const u64 place = place_of(key, i);
-    if (key <= SA_NONE) return;
-    best = place > best ? place : best;
-    least = min(least, key);
-  });
-  best = block_all(best, s.wide, [](u64 x, u64 y) { return x > y ? x : y; });
-  const int arg = best ? (int)~(uint32_t)best : -1;
-  if (arg < 0 || !(temperature > 0) || k == 1) {
-    if (threadIdx.x == 0) a.token[b] = arg;
-    return;
-  }
-  const uint32_t bottom = (uint32_t)block_all((u64)least, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
-  r.top = logit_of((uint32_t)(best >> 32));
-  r.temperature = temperature;
-  const double c = 1.4426950408889634 / temperature;
-  r.c_hi = (float)c;
-  r.c_lo = (float)(c - (double)r.c_hi);
-  r.reach = (float)fmin(SA_FAR * temperature, 3e38);
-  const float range = fminf(r.top - logit_of(bottom), r.reach);
-  r.inv = range > 0.f && range < 3e38f ? SA_BINS / range * 0.99999f : 0.f;
-  const bool by_rank = k > 0 && k < a.V, by_mass = p < 1;
-  bool close = false;
-  u64 cut = 0;
-  if (by_rank || by_mass) {
-    for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) s.count[i] = 0;
-    __syncthreads();
-    r.all([&](float x, int) {
-      if (r.counts(x)) atomicAdd(&s.count[r.bin_of(x)], 1u);
-    });
-    __syncthreads();
-  }
-  if (by_rank) {
-    if (threadIdx.x < WARP) {
-      const int lane = threadIdx.x;
-      int run = 0, bin = -1, before = 0;
-      for (int b0 = 0; b0 < SA_BINS && bin < 0; b0 += WARP) {
-        int n = s.count[b0 + lane], sum = n;
+// The sorted list holds all entries that can be kept, n of them, `behind` is the weight of the others that top-p counts: the token.
+// found[1]: too close to tell. By all of a block.
+__device__ int sample_list(SampleShared &s, const SampleScale &z, int n, double behind, double p, double min_p, double u) {
+  const int at = threadIdx.x * SA_EACH;
+  double w[SA_EACH], mine = 0, total;
+  if (threadIdx.x == 0) s.found[1] = 0;
 #pragma unroll
-        for (int o = 1; o < WARP; o <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, sum, o);
-          if (lane >= o) sum += up;
-        }
-        const unsigned over = __ballot_sync(0xffffffffu, run + sum >= k);
-        if (over) {
-          bin = b0 + __ffs(over) - 1;
-          before = run + __shfl_sync(0xffffffffu, sum - n, __ffs(over) - 1);
-        }
-        run += __shfl_sync(0xffffffffu, sum, WARP - 1);
-      }
-      if (lane == 0) {
-        s.found[2] = bin;
-        s.found[3] = before;
-      }
-    }
-    __syncthreads();
-    const int bin = s.found[2], before = s.found[3];
-    if (bin >= 0) {  // else there are fewer than k
-      u64 first = 0, last = ~0ull;
-      r.all([&](float x, int i) {
-        if (!r.counts(x) || r.bin_of(x) != bin) return;
-        const u64 at = place_of(order_of(x), i);
-        first = at > first ? at : first;
-        last = at < last ? at : last;
-      });
-      first = block_all(first, s.wide, [](u64 x, u64 y) { return x > y ? x : y; });
-      last = block_all(last, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
-      bool none = false;
-      // (the histogram is needed again)
-      cut = r.template narrow<true, false>(last, first, k - 1 - before, 0, 0, none);
-      if (by_mass) {
-        for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) s.count[i] = 0;
-        __syncthreads();
-        r.all([&](float x, int i) {
-          if (r.counts(x) && place_of(order_of(x), i) >= cut) atomicAdd(&s.count[r.bin_of(x)], 1u);
-        });
-        __syncthreads();
-      }
-    }
+  for (int e = 0; e < SA_EACH; ++e) {
+    w[e] = at + e < n ? z.weight(logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
+    mine += w[e];
   }
-  const u64 by_k = cut;
-  if (by_mass) cut = r.template nucleus<false>(by_k, p, close);
-  int token = -1;
-  if (!close) token = r.template draw<false>(cut, u, min_p, close);
-  if (close) {
-    if (by_mass) {
-      // the steps' counts may have been used up
-      for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) s.count[i] = 0;
-      __syncthreads();
-      r.all([&](float x, int i) {
-        if (r.counts(x) && place_of(order_of(x), i) >= by_k) atomicAdd(&s.count[r.bin_of(x)], 1u);
-      });
-      __syncthreads();
-      cut = r.template nucleus<true>(by_k, p, close);
+  double run = block_before(mine, s.part, total);
+  const double mass = p * (total + behind);
+  int left = 0;
+  bool near = false;
+#pragma unroll
+  for (int e = 0; e < SA_EACH; ++e) {
+    bool in = at + e < n;
+    if (in && p < 1 && at + e > 0) {
+      in = run < mass;
+      near |= fabs(run - mass) <= SA_CLOSE * (total + behind);
     }
-    token = r.template draw<true>(cut, u, min_p, close);
+    if (in && min_p > 0 && w[e] < min_p * (1 + 1e-8)) in = w[e] >= min_p * (1 - 1e-8) && z.exact(logit_of((uint32_t)(s.list[at + e] >> 32))) >= min_p;
+    left += in;
+    run += w[e];
   }
-  if (threadIdx.x == 0) a.token[b] = token;
+  n = (int)block_total(left, s);  // (what is kept are the first ones)
+  // by index: the halves of a place change sides
+  for (int i = threadIdx.x; i < n; i += SA_THREADS) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
+  __syncthreads();
+  sort_list(s, n);
+  mine = 0;
+#pragma unroll
+  for (int e = 0; e < SA_EACH; ++e) {
+    w[e] = at + e < n ? z.weight(logit_of((uint32_t)s.list[at + e]), s.table) : 0.0;
+    mine += w[e];
+  }
+  run = block_before(mine, s.part, total);
+  const double target = u * total;
+  int over = n - 1;  // (rounding: the last one)
+#pragma unroll
+  for (int e = SA_EACH - 1; e >= 0; --e) {
+    double upto = run;
+    for (int x = 0; x <= e; ++x) upto += w[x];
+    if (at + e >= n) continue;
+    near |= fabs(upto - target) <= SA_CLOSE * total;
+    if (upto > target) over = min(over, at + e);
+  }
+  over = (int)block_all((u64)over, s.wide, [](u64 a, u64 b) { return a < b ? a : b; });
+  if (near) s.found[1] = 1;
+  __syncthreads();
+  return (int)~(uint32_t)(s.list[over] >> 32);
 }
 
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int slice, int stored) {
+  namespace cg = cooperative_groups;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  SampleShared &s = *reinterpret_cast<SampleShared *>(smem_raw);
+  T *const copy = reinterpret_cast<T *>(smem_raw + (sizeof(SampleShared) + 15) / 16 * 16);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / C;
+  auto started = cluster.barrier_arrive();
+  pdl_prologue();
+  const double temperature = a.temperature ? (double)a.temperature[b] : a.temperature0;
+  const double p = a.top_p ? (double)a.top_p[b] : a.top_p0, min_p = fmin(a.min_p ? (double)a.min_p[b] : a.min_p0, 1.0), u = a.u[b];
+  const int k = a.top_k ? a.top_k[b] : a.top_k0;
+  const T *const row = static_cast<const T *>(a.logits) + b * a.ld;
+  const int from = min(a.V, rank * slice), to = min(a.V, from + slice);
+  const T *const entries = stored ? copy - from : row;  // entries[i], from <= i < to
+  SampleShared &first = *cluster.map_shared_rank(&s, 0);
+  SampleAlone<T, VEC> r{row, a.V, s, {}};
+  SampleScale &z = r.z;
+  auto mine = [&](auto f) { sweep<T, VEC>(entries, from, to, threadIdx.x, SA_THREADS, f); };
+
+  // 1. the slice, and the row's largest and smallest entries
+  u64 best = 0, least = ~0ull;
+  {
+    auto see = [&](float x, int i) {
+      const uint32_t key = order_of(x);
+      if (key <= SA_NONE) return;
+      const u64 place = place_of(key, i);
+      best = place > best ? place : best;
+      least = key < least ? key : least;
+    };
+    constexpr int N = Chunk<T>::N;
+    if (VEC && stored) {
+      for (int i0 = from + (int)threadIdx.x * N; i0 < to; i0 += 4 * SA_THREADS * N) {
+        uint4 v[4];
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+          if (i0 + d * SA_THREADS * N + N <= to) v[d] = ld_stream16(row + i0 + d * SA_THREADS * N);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int i = i0 + d * SA_THREADS * N;
+          if (i + N <= to) {
+            float x[N];
+            unpack_chunk<T>(v[d], x);
+            *reinterpret_cast<uint4 *>(copy + (i - from)) = v[d];
+#pragma unroll
+            for (int e = 0; e < N; ++e) see(x[e], i + e);
+          } else {
+            for (int e = i; e < to; ++e) {
+              copy[e - from] = row[e];
+              see(to_f(row[e]), e);
+            }
+          }
+        }
+      }
+    } else {
+      sweep<T, VEC>(row, from, to, threadIdx.x, SA_THREADS, [&](float x, int i) {
+        if (stored) copy[i - from] = row[i];
+        see(x, i);
+      });
+    }
+  }
+  if (threadIdx.x < 64) s.table[threadIdx.x] = exp2(threadIdx.x * 0.015625);
+  for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) s.count[i] = s.into[i] = 0;
+  if (threadIdx.x == 0) s.listed = 0;
+  best = block_all(best, s.wide, [](u64 x, u64 y) { return x > y ? x : y; });
+  least = block_all(least, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
+  cluster.barrier_wait(std::move(started));  // (all blocks of the cluster have started)
+  if ((int)threadIdx.x < C) {
+    SampleShared &other = *cluster.map_shared_rank(&s, threadIdx.x);
+    other.best[rank] = best;
+    other.least[rank] = least;
+  }
+  cluster.sync();
+  for (int c = 0; c < C; ++c) {
+    best = s.best[c] > best ? s.best[c] : best;
+    least = s.least[c] < least ? s.least[c] : least;
+  }
+  const int arg = best ? (int)~(uint32_t)best : -1;
+  if (arg < 0 || !(temperature > 0) || k == 1) {
+    if (rank == 0 && threadIdx.x == 0) a.token[b] = arg;
+    return;
+  }
+  z.top = logit_of((uint32_t)(best >> 32));
+  z.temperature = temperature;
+  const double c = 1.4426950408889634 / temperature;
+  z.c_hi = (float)c;
+  z.c_lo = (float)(c - (double)z.c_hi);
+  z.reach = (float)fmin(SA_FAR * temperature, 3e38);
+  const float range = fminf(z.top - logit_of((uint32_t)least), z.reach);
+  z.inv = range > 0.f && range < 3e38f ? SA_BINS / range * 0.99999f : 0.f;
+  bool by_rank = k > 0 && k < a.V;
+  const bool by_mass = p < 1;
+  u64 cut = 0;
+
+  // One block goes on alone; the others have nothing left to do.
+  auto alone = [&]() {
+    const int token = r.token(k, p, min_p, u);
+    if (threadIdx.x == 0) a.token[b] = token;
+  };
+  // Entries of steps lo .. hi at or in front of the cut go to the first block's list; weights in front of them and behind, if wanted, to
+  // its sums. Returns the list's length and the sums, in the first block.
+  auto collect = [&](int lo, int hi, bool sums, double &in_front, double &behind) -> int {
+    double x0 = 0, x1 = 0;
+    mine([&](float x, int i) {
+      if (!z.counts(x)) return;
+      const int bin = z.bin_of(x);
+      const u64 place = place_of(order_of(x), i);
+      if (place < cut) return;
+      if (bin >= lo && bin <= hi) {
+        const int at = atomicAdd(&first.listed, 1);
+        if (at < SA_LIST) first.list[at] = place;
+      } else if (sums) {
+        const double w = z.weight(x, s.table);
+        if (bin < lo) x0 += w;
+        else x1 += w;
+      }
+    });
+    if (sums) {
+      x0 = block_total(x0, s);
+      x1 = block_total(x1, s);
+      if (threadIdx.x == 0) {
+        first.sums[rank][0] = x0;
+        first.sums[rank][1] = x1;
+      }
+    }
+    cluster.sync();
+    in_front = behind = 0;
+    if (rank != 0) return 0;
+    if (sums)
+      for (int c = 0; c < C; ++c) {
+        in_front += s.sums[c][0];
+        behind += s.sums[c][1];
+      }
+    return s.listed;
+  };
+  // The first block tells all the cut, or that they are not needed any more.
+  auto tell = [&](u64 value, bool done) {
+    if (rank == 0) {
+      __syncthreads();  // (the list has been read)
+      if (threadIdx.x == 0) s.listed = 0;
+      if ((int)threadIdx.x < C) {
+        SampleShared &other = *cluster.map_shared_rank(&s, threadIdx.x);
+        other.cut = value;
+        other.done = done;
+      }
+    }
+    cluster.sync();
+    cut = s.cut;
+    return s.done != 0;
+  };
+  // The first block makes the rest of what it has in the list.
+  auto finish = [&](int n, double behind) {
+    sort_list(s, n);
+    const int token = sample_list(s, z, by_rank ? min(n, k) : n, behind, p, min_p, u);
+    const bool close = s.found[1] != 0;
+    __syncthreads();
+    if (close) alone();
+    else if (threadIdx.x == 0) a.token[b] = token;
+  };
+
+  if (by_rank || by_mass) {
+    // 2. counts of the steps: of the slice, then of the row and running
+    const int fine = 1 << min(12, __clz(a.V) - 1);  // (the sum over the row stays below 2^31)
+    mine([&](float x, int) {
+      if (!z.counts(x)) return;
+      unsigned into;
+      const int bin = z.bin_of(x, (float)fine, into);
+      atomicAdd(&s.count[bin], 1u);
+      if (by_mass) atomicAdd(&s.into[bin], into);
+    });
+    cluster.sync();
+    unsigned n[SA_EACH] = {}, sum = 0, into[SA_EACH] = {};
+    const int at = threadIdx.x * SA_EACH;
+    for (int c = 0; c < C; ++c) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(&cluster.map_shared_rank(&s, c)->count[at]);
+      n[0] += v.x;
+      n[1] += v.y;
+      n[2] += v.z;
+      n[3] += v.w;
+      if (by_mass) {
+        const uint4 y = *reinterpret_cast<const uint4 *>(&cluster.map_shared_rank(&s, c)->into[at]);
+        into[0] += y.x;
+        into[1] += y.y;
+        into[2] += y.z;
+        into[3] += y.w;
+      }
+    }
+    static_assert(SA_EACH == 4, "one 16-byte load of counts");
+    sum = n[0] + n[1] + n[2] + n[3];
+    double total;
+    unsigned run = (unsigned)block_before(sum, s.part, total);
+    if (threadIdx.x == 0) s.found[2] = s.found[3] = SA_BINS - 1;
+    __syncthreads();
+    int rank_bin = SA_BINS;
+    by_rank = by_rank && total > k;
+    {
+      unsigned upto = run;
+#pragma unroll
+      for (int e = 0; e < SA_EACH; ++e) {
+        if (by_rank && (int)upto < k && (int)(upto + n[e]) >= k) s.found[2] = at + e;
+        upto += n[e];
+        s.upto[at + e] = upto;
+      }
+    }
+    __syncthreads();
+    if (by_rank) rank_bin = s.found[2];
+    const int rank_upto = by_rank ? (int)s.upto[rank_bin] : 0, rank_before = by_rank && rank_bin ? (int)s.upto[rank_bin - 1] : 0;
+    double in_front, behind;
+    if (by_rank) {
+      // 3. top-k
+      const bool whole = rank_upto <= SA_LIST;
+      if (!whole && rank_upto - rank_before > SA_LIST) {
+        cluster.sync();  // (counts have been read)
+        if (rank == 0) alone();
+        return;
+      }
+      const int listed = collect(whole ? 0 : rank_bin, rank_bin, false, in_front, behind);
+      if (whole) {
+        if (rank == 0) finish(listed, 0);
+        return;
+      }
+      u64 place = 0;
+      if (rank == 0) {
+        sort_list(s, listed);
+        place = s.list[k - 1 - rank_before];
+      }
+      tell(place, false);
+    }
+    if (by_mass) {
+      // top-p: bounds of the running sums at the steps' borders. A step's n entries at f_i of it (0 .. 1) weigh E 2^(-c f_i) each, E at its
+      // beginning: together at least E n 2^(-c F), with F the average, and at most E n (1 - F (1 - 2^-c)). What (top - x) * inv is rounded by
+      // is below 2048 * 2^-22 of a step; all in all the bounds are widened by 1e-5.
+      const double width = z.inv > 0.f ? 1.0 / z.inv : 0.0, per = c * width, full = exp2(-per);
+      double lo[SA_EACH], hi[SA_EACH], lo_sum = 0, hi_sum = 0, lo_total, hi_total;
+#pragma unroll
+      for (int e = 0; e < SA_EACH; ++e) {
+        const int bin = at + e;
+        lo[e] = hi[e] = 0;
+        if (n[e] && bin <= rank_bin) {
+          const double begin = exp2(-per * bin);
+          if (bin < rank_bin) {
+            const double f = (double)into[e] / ((double)n[e] * fine);
+            hi[e] = begin * n[e] * (1 - f * (1 - full)) * (1 + 1e-5);
+            lo[e] = begin * n[e] * exp2(-per * (f + 1.0 / fine)) * (1 - 1e-5);
+          } else {  // only the first ones of the step
+            hi[e] = begin * (k - rank_before) * (1 + 1e-5);
+            lo[e] = begin * (k - rank_before) * full * (1 - 1e-5);
+          }
+          if (z.inv == 0.f) lo[e] = 0;  // (no steps: equal entries, or a range that floats do not hold)
+        }
+        hi_sum += hi[e];
+        lo_sum += lo[e];
+      }
+      double hi_run = block_before(hi_sum, s.part, hi_total), lo_run = block_before(lo_sum, s.part2, lo_total);
+      // can: the first step at whose end the sum can have reached p of the total; must: the first at whose end it has to have
+      int can = SA_BINS - 1, must = SA_BINS - 1;
+#pragma unroll
+      for (int e = SA_EACH - 1; e >= 0; --e) {
+        double x = hi_run, y = lo_run;
+        for (int f = 0; f <= e; ++f) {
+          x += hi[f];
+          y += lo[f];
+        }
+        if (x >= p * lo_total) can = at + e;
+        if (y >= p * hi_total) must = at + e;
+      }
+      can = (int)block_all((u64)can, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
+      must = (int)block_all((u64)must, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
+      int most = (int)s.upto[must], least_n = can ? (int)s.upto[can - 1] : 0;
+      if (by_rank) {
+        most = min(most, k);
+        least_n = min(least_n, k);
+      }
+      const bool whole = most <= SA_LIST;
+      if (!whole && most - least_n > SA_LIST) {
+        cluster.sync();
+        if (rank == 0) alone();
+        return;
+      }
+      const int listed = collect(whole ? 0 : can, must, true, in_front, behind);
+      if (whole) {
+        if (rank == 0) {
+          by_rank = false;  // (the cut is in the list)
+          finish(listed, behind);
+        }
+        return;
+      }
+      u64 place = cut;
+      bool close = false;
+      if (rank == 0 && listed > 0) {
+        sort_list(s, listed);
+        double w[SA_EACH], sum = 0, between;
+#pragma unroll
+        for (int e = 0; e < SA_EACH; ++e) {
+          w[e] = at + e < listed ? z.weight(logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
+          sum += w[e];
+        }
+        double before = in_front + block_before(sum, s.part, between);
+        const double all = in_front + between + behind, mass = p * all;
+        bool near = false;
+        int last = 0;
+#pragma unroll
+        for (int e = 0; e < SA_EACH; ++e) {
+          if (at + e < listed && at + e > 0) {
+            near |= fabs(before - mass) <= SA_CLOSE * all;
+            if (before < mass) last = at + e;
+          }
+          before += w[e];
+        }
+        last = (int)block_all((u64)last, s.wide, [](u64 x, u64 y) { return x > y ? x : y; });
+        close = block_all((u64)near, s.wide, [](u64 x, u64 y) { return x | y; }) != 0;
+        place = s.list[last];
+      }
+      if (tell(place, close)) {
+        if (rank == 0) alone();
+        return;
+      }
+    }
+  }
+
+  // 4. the sums of what is kept, in index order
+  {
+    const int warp = threadIdx.x / WARP, lane = threadIdx.x % WARP;
+    constexpr int N = VEC ? Chunk<T>::N : 1;
+    const int share = ((to - from + SA_WARPS - 1) / SA_WARPS + WARP * N - 1) / (WARP * N) * (WARP * N);
+    const int lo = min(to, from + warp * share), hi = min(to, lo + share);
+    auto kept = [&](float x, int i) -> double {
+      if (!z.counts(x) || place_of(order_of(x), i) < cut) return 0.0;
+      const double w = z.weight(x, s.table);
+      if (min_p > 0 && w < min_p * (1 + 1e-8) && (w < min_p * (1 - 1e-8) || z.exact(x) < min_p)) return 0.0;
+      return w;
+    };
+    double sum = 0;
+    sweep<T, VEC>(entries, lo, hi, lane, WARP, [&](float x, int i) { sum += kept(x, i); });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) s.part[warp] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < SA_WARPS; ++w) sum += s.part[w];
+    if ((int)threadIdx.x < C) cluster.map_shared_rank(&s, threadIdx.x)->kept[rank] = sum;
+    cluster.sync();
+    double total = 0, before = 0;
+    for (int c = 0; c < C; ++c) total += s.kept[c];
+    const double target = u * total;
+    int owner = C, last = 0;
+    double mine_before = 0;
+    for (int c = 0; c < C; ++c) {
+      if (s.kept[c] > 0) last = c;
+      if (owner == C && before + s.kept[c] > target) {
+        owner = c;
+        mine_before = before;
+      }
+      before += s.kept[c];
+    }
+    if (owner == C) {  // (rounding: the last entry that is kept)
+      owner = last;
+      mine_before = before;
+    }
+    if (rank != owner) return;
+    const int token = r.locate(entries, lo, hi, mine_before, target, total, kept);
+    const bool close = s.found[1] != 0;
+    __syncthreads();
+    if (close) alone();
+    else if (threadIdx.x == 0) a.token[b] = token;
+  }
+}
+
+// Blocks of a row: as many as keep the device busy with B rows, more where a slice would leave room for one block per multiprocessor.
 template <typename T>
 static cudaError_t launch_sample(const SampleArgs &a, int B, bool vec, cudaStream_t st) {
-  constexpr int smem = sizeof(SampleShared);
+  constexpr int N = Chunk<T>::N, fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16, most = 200 * 1024;
+  int C = 1;
+  while (C < SA_CLUSTER && ((long long)B * C * 2 <= 2 * sm_count() || (long long)(a.V + C - 1) / C * sizeof(T) > 64 * 1024)) C *= 2;
+  while (C > 1 && a.V / C < 512) C /= 2;
+  const int slice = ceil_div(ceil_div(a.V, C), N) * N;
+  const bool stored = (long long)slice * sizeof(T) <= most - fixed;
+  const int smem = fixed + (stored ? slice * (int)sizeof(T) : 0);
   static DevicePrep prep;
   const int(*unused)[4];
   cudaError_t e = prep.get(
       [&](int(&)[4]) {
-        cudaError_t f = cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        return f != cudaSuccess ? f : cudaFuncSetAttribute(sample_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t f = cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+        return f != cudaSuccess ? f : cudaFuncSetAttribute(sample_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       },
       unused);
   if (e != cudaSuccess) return e;
-  return vec ? djv::launch_kernel(sample_kernel<T, true>, dim3(B), dim3(SA_THREADS), smem, st, a)
-             : djv::launch_kernel(sample_kernel<T, false>, dim3(B), dim3(SA_THREADS), smem, st, a);
+  return djv::launch_kernel_cluster(vec ? sample_kernel<T, true> : sample_kernel<T, false>, dim3(B * C), dim3(SA_THREADS), smem, st, dim3(C, 1, 1),
+                                    a, slice, (int)stored);
 }
 
 static double double_of(long long bits) {
@@ -564,7 +850,7 @@ extern "C" int djv_sample(int dtype, long long *token, const void *logits, long 
                           const float *min_p, long long min_p_bits, int B, int V, void *stream) {
   DJV_REQUIRE(is_dtype(dtype), "sample: dtype %d", dtype);
   DJV_REQUIRE(token && logits && u, "sample: null pointer");
-  DJV_REQUIRE(B >= 0 && V >= 1 && V <= (1 << 30) && ld >= V, "sample: B=%d V=%d ld=%lld", B, V, ld);
+  DJV_REQUIRE(B >= 0 && B <= (1 << 27) && V >= 1 && V <= (1 << 30) && ld >= V, "sample: B=%d V=%d ld=%lld", B, V, ld);
   const SampleArgs a{token, logits, ld, u, temperature, double_of(temperature_bits), top_k, top_k_all, top_p, double_of(top_p_bits),
                      min_p, double_of(min_p_bits), V};
   DJV_REQUIRE((temperature || (a.temperature0 >= 0 && a.temperature0 < 1e30)) && (top_k || top_k_all >= 0) && (top_p || a.top_p0 >= 0) &&

@@ -870,26 +870,31 @@ def _code(dtype) -> int:
     return _CODES[dtype]
 
 
-def _last_adjacent(t):
-    """t, or a copy of it, whose last dimension is contiguous."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _rows(t):
+    """t (T, heads, D), or a copy of it, whose last dimension is contiguous; its address, row stride and head stride."""
+    ld, head, one = t.stride()
+    if one != 1 and t.shape[2] != 1:
+        t = t.contiguous()
+        ld, head, one = t.stride()
+    return t, (t.data_ptr(), ld, head)
 
 
 def _pages(k_pages, v_pages, table, pos, dtype, G: int, D: int):
     """Checks a paged cache against what is stored in it; its arguments of the C ABI."""
-    P, heads, page, dim = k_pages.shape
+    P, heads, page, dim = shape = k_pages.shape
     ld_page, ld_head, ld_slot, one = strides = k_pages.stride()
     B, width = table.shape
     k_at, v_at, unit = k_pages.data_ptr(), v_pages.data_ptr(), _UNIT[dtype]
     assert k_pages.dtype is dtype and v_pages.dtype is dtype, f"pages of {k_pages.dtype} and {v_pages.dtype} for {dtype}"
-    assert heads == G and dim == D and v_pages.shape == k_pages.shape, f"pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} for {G} heads of {D}"
+    assert heads == G and dim == D and v_pages.shape == shape, f"pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} for {G} heads of {D}"
     assert v_pages.stride() == strides and one == 1, "K and V pages have one layout, dimensions adjacent"
     assert not (D | ld_page | ld_head | ld_slot) & unit, f"rows of a page start on multiples of {unit + 1} elements"
     assert not (k_at | v_at) & 15, "pages start on multiples of 16 bytes"
-    assert table.dtype is torch.int32 and width >= 1 and (table.stride(1) == 1 or width == 1), "table: (B, width) int32, rows of adjacent entries"
+    ld_table, next_entry = table.stride()
+    assert table.dtype is torch.int32 and width >= 1 and (next_entry == 1 or width == 1), "table: (B, width) int32, rows of adjacent entries"
     assert width * page < 2 ** 31, "more than 2^31 tokens per sequence"
-    assert pos.shape == (B,) and pos.dtype is torch.int64 and pos.is_contiguous(), "pos: (B,) int64"
-    return k_at, v_at, ld_page, ld_head, ld_slot, P, page, table.data_ptr(), table.stride(0), width, pos.data_ptr()
+    assert pos.dim() == 1 and pos.numel() == B and pos.dtype is torch.int64 and pos.is_contiguous(), "pos: (B,) int64"
+    return k_at, v_at, ld_page, ld_head, ld_slot, P, page, table.data_ptr(), ld_table, width, pos.data_ptr()
 
 
 def _cumulative(cu_seqlens) -> int:
@@ -913,10 +918,10 @@ def paged_append(q, k, v, k_pages, v_pages, table, pos, cu_seqlens=None, freqs=N
     if device != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
             return paged_append(q, k, v, k_pages, v_pages, table, pos, cu_seqlens, freqs, amp, interleaved, keys)
-    T, G, D = k.shape
+    T, G, D = shape = k.shape
     dtype = k.dtype
     code = _code(dtype)
-    assert v.shape == k.shape and v.dtype is dtype, "k and v: (T, G, D) of one type"
+    assert v.shape == shape and v.dtype is dtype, "k and v: (T, G, D) of one type"
     pages = _pages(k_pages, v_pages, table, pos, dtype, G, D)
     B = table.shape[0]
     if cu_seqlens is None:
@@ -928,17 +933,18 @@ def paged_append(q, k, v, k_pages, v_pages, table, pos, cu_seqlens=None, freqs=N
         half = freqs.numel()
         assert freqs.dim() == 1 and freqs.dtype is torch.float32 and freqs.is_contiguous(), "freqs: (half,) fp32"
         assert 2 * half <= D, f"{2 * half} rotary dimensions in heads of {D}"
-    k, v = _last_adjacent(k), _last_adjacent(v)
-    H, q_out, query_args = 0, None, (None, 0, 0)
+    k, k_args = _rows(k)
+    v, v_args = _rows(v)
+    H, q_out, q_args = 0, None, (None, 0, 0)
     if q is not None:
         rows, H, dim = q.shape
         assert rows == T and dim == D and H >= 1 and q.dtype is dtype, f"q: ({T}, H, {D}) {dtype}"
-        q = _last_adjacent(q)
-        q_out, query_args = q.new_empty(T, H, D), (q.data_ptr(), q.stride(0), q.stride(1))
+        q, q_args = _rows(q)
+        q_out = q.new_empty(T, H, D)
     k_out = k.new_empty(T, G, D) if keys else None
     if T:
-        call("djv_paged_append", code, _ptr(q_out), _ptr(k_out), *query_args, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-             v.stride(0), v.stride(1), *pages, _ptr(cu_seqlens), _ptr(freqs), float(amp), half, int(interleaved), B, T, H, G, D, _stream())
+        call("djv_paged_append", code, _ptr(q_out), _ptr(k_out), *q_args, *k_args, *v_args, *pages, _ptr(cu_seqlens), _ptr(freqs), float(amp),
+             half, int(interleaved), B, T, H, G, D, _stream())
     return q_out, k_out
 
 
@@ -993,15 +999,15 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     assert H >= 1 and H % G == 0, f"{H} query heads over {G} key/value heads"
     assert 1 <= D <= 256, f"heads of {D}"
     B = _cumulative(cu_seqlens)
-    q, k, v = _last_adjacent(q), _last_adjacent(k), _last_adjacent(v)
+    (q, q_args), (k, k_args), (v, v_args) = _rows(q), _rows(k), _rows(v)
     keep = out is not None
     if keep:
         assert out.shape == (T, H, D) and out.is_contiguous() and out.dtype is dtype, f"out: ({T}, {H}, {D}) {dtype}, contiguous"
     else:
         out = q.new_empty(T, H, D)
     if T:
-        call("djv_packed_attention", code, out.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-             v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens.data_ptr(), B, T, H, G, D, float(scale), int(keep), _stream())
+        call("djv_packed_attention", code, out.data_ptr(), *q_args, *k_args, *v_args, cu_seqlens.data_ptr(), B, T, H, G, D, float(scale),
+             int(keep), _stream())
     return out
 
 
