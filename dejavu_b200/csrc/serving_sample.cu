@@ -66,19 +66,24 @@ struct SampleShared {
   u64 list[SA_LIST];
   union {
     struct {
-      unsigned count[SA_BINS];  // of this block's slice
+      union {
+        unsigned count[SA_BINS];  // of this block's slice
+        int owned[SA_LIST];       // later: its entries between the bounds of top-p
+      };
       unsigned upto[SA_BINS];   // of the row, in this step and those in front of it
     };
     double mass[SA_BINS];       // (of a block that works alone)
   };
   unsigned into[SA_BINS];       // of this block's slice: sum of how far into the step entries are, `fine` to a step
   double table[64];           // 2^(j / 64)
-  double part[SA_WARPS], part2[SA_WARPS];
+  double part[SA_WARPS], part2[SA_WARPS], part3[SA_WARPS];
   u64 wide[SA_WARPS];
+  float narrow[SA_WARPS];
   // written by the blocks of the cluster
-  u64 best[SA_CLUSTER], least[SA_CLUSTER];
+  u64 best[SA_CLUSTER];
+  float least[SA_CLUSTER];
   double sums[SA_CLUSTER][2], kept[SA_CLUSTER];
-  int listed;
+  int listed, own;
   u64 cut;                    // by the first block: entries whose place is lower are dropped
   int done;                   // by the first block: 1: it has the token, or finds it alone
   int found[4];
@@ -93,9 +98,9 @@ __device__ __forceinline__ V block_all(V v, V *slots, F f) {
   __syncthreads();
   if (threadIdx.x % WARP == 0) slots[threadIdx.x / WARP] = v;
   __syncthreads();
-  v = slots[0];
-#pragma unroll 4
-  for (int w = 1; w < SA_WARPS; ++w) v = f(v, slots[w]);
+  v = slots[threadIdx.x % SA_WARPS];
+#pragma unroll
+  for (int o = SA_WARPS / 2; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
 __device__ __forceinline__ double block_total(double v, SampleShared &s) {
@@ -126,24 +131,60 @@ __device__ __forceinline__ void sweep(const T *row, int lo, int hi, int at, int 
       if (i + e < hi) f(to_f(row[i + e]), i + e);
 }
 
-// Sorts list[0 .. n), largest first; n <= SA_LIST.
-__device__ void sort_list(SampleShared &s, int n) {
-  int size = 32;
+// The places of a warp's 64 entries, two to a lane (lane and lane + 32), through the steps j <= 32 of a bitonic merge of blocks of k.
+__device__ __forceinline__ void merge_in_warp(u64 &x, u64 &y, int first, int k, int from) {
+  const int lane = threadIdx.x % WARP;
+  if (from >= 32) {
+    const bool falls = ((first + lane) & k) == 0;
+    if ((x < y) == falls) {
+      const u64 t = x;
+      x = y;
+      y = t;
+    }
+    from = 16;
+  }
+  for (int j = from; j > 0; j >>= 1) {
+    const u64 a = __shfl_xor_sync(0xffffffffu, x, j), b = __shfl_xor_sync(0xffffffffu, y, j);
+    const bool low = (lane & j) == 0;  // of a pair, the one that gets the larger where the block falls
+    if ((low == (((first + lane) & k) == 0)) == (a > x)) x = a;
+    if ((low == (((first + 32 + lane) & k) == 0)) == (b > y)) y = b;
+  }
+}
+
+// Sorts list[0 .. n), largest first; n <= SA_LIST; entries are different, the filling is 0. Steps inside 64 entries stay in a warp.
+__device__ __noinline__ void sort_list(u64 *list, int n) {
+  int size = 64;
   while (size < n) size *= 2;
-  for (int i = n + threadIdx.x; i < size; i += SA_THREADS) s.list[i] = 0;
+  const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
+  for (int i = n + threadIdx.x; i < size; i += SA_THREADS) list[i] = 0;
   __syncthreads();
-  for (int k = 2; k <= size; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
+  for (int at = warp * 64; at < size; at += SA_WARPS * 64) {
+    u64 x = list[at + lane], y = list[at + 32 + lane];
+    for (int k = 2; k <= 64; k *= 2) merge_in_warp(x, y, at, k, k / 2);
+    list[at + lane] = x;
+    list[at + 32 + lane] = y;
+  }
+  __syncthreads();
+  for (int k = 128; k <= size; k *= 2) {
+    for (int j = k / 2; j >= 64; j /= 2) {
       for (int i = threadIdx.x; i < size / 2; i += SA_THREADS) {
         const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const u64 x = s.list[a], y = s.list[b];
+        const u64 x = list[a], y = list[b];
         if ((x < y) == ((a & k) == 0)) {
-          s.list[a] = y;
-          s.list[b] = x;
+          list[a] = y;
+          list[b] = x;
         }
       }
       __syncthreads();
     }
+    for (int at = warp * 64; at < size; at += SA_WARPS * 64) {
+      u64 x = list[at + lane], y = list[at + 32 + lane];
+      merge_in_warp(x, y, at, k, 32);
+      list[at + lane] = x;
+      list[at + 32 + lane] = y;
+    }
+    __syncthreads();
+  }
 }
 
 // Sum of v over the threads in front of this one; total receives the block's.
@@ -158,14 +199,15 @@ __device__ __forceinline__ double block_before(double v, double *slots, double &
   __syncthreads();
   if (lane == WARP - 1) slots[warp] = sum;
   __syncthreads();
-  double before = sum - v;
-  total = 0;
-#pragma unroll 4
-  for (int w = 0; w < SA_WARPS; ++w) {
-    if (w < warp) before += slots[w];
-    total += slots[w];
+  double run = slots[lane % SA_WARPS];
+#pragma unroll
+  for (int o = 1; o < SA_WARPS; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, run, o, SA_WARPS);
+    if (lane % SA_WARPS >= o) run += up;
   }
-  return before;
+  total = __shfl_sync(0xffffffffu, run, SA_WARPS - 1);
+  const double front = __shfl_sync(0xffffffffu, run, warp ? warp - 1 : 0);
+  return (warp ? front : 0.0) + (sum - v);
 }
 
 // The largest entry of a row and what follows from it.
@@ -175,27 +217,22 @@ struct SampleScale {
   float c_hi, c_lo;     // log2(e) / temperature
   float reach;          // entries further below the largest are dropped
 
-  __device__ __forceinline__ bool counts(float x) const { return x >= -3.402823466e38f && !(top - x > reach); }
-  __device__ __forceinline__ int bin_of(float x) const { return min(SA_BINS - 1, (int)((top - x) * inv)); }
-  // the same, and how far into the step x is, in parts of a step
-  __device__ __forceinline__ int bin_of(float x, float fine, unsigned &into) const {
-    const float at = (top - x) * inv;  // (NaN where both are infinite)
-    const int bin = min(SA_BINS - 1, (int)at);
-    into = (unsigned)((at - bin) * fine);
-    return bin;
-  }
+  __device__ __forceinline__ bool counts(float x) const { return top - x <= reach || x == top; }
+  // for x that counts: the steps in front of x, a number below SA_BINS
+  __device__ __forceinline__ float step_of(float x) const { return x == top ? 0.f : (top - x) * inv; }
   __device__ __forceinline__ double exact(float x) const { return x == top ? 1.0 : exp(((double)x - (double)top) / temperature); }
-  // x counts: y = (x - top) log2(e) / temperature >= -65 as the sum of two floats, y = k / 64 + f
+  // For x that counts (for others a number that means nothing): y = (x - top) log2(e) / temperature >= -65 as the sum of two floats,
+  // y = k / 64 + f
   __device__ __forceinline__ double weight(float x, const double *table) const {
-    if (x == top) return 1.0;  // (+inf among them)
     const float t = x - top, v = t - x, e = (x - (t - v)) - (top + v);  // x - top = t + e
-    const float y = t * c_hi, rest = fmaf(t, c_hi, -y) + fmaf(t, c_lo, e * c_hi);
+    const float y = fmaxf(t * c_hi, -100.f), rest = fmaf(t, c_hi, -y) + fmaf(t, c_lo, e * c_hi);
     const float k = rintf(y * 64.f);
     const float f = (fmaf(k, -0.015625f, y) + rest) * 0.69314718f;  // (the difference is exact)
     const float q = fmaf(f * f, fmaf(f, fmaf(f, 0.041666668f, 0.16666667f), 0.5f), f);  // e^f - 1
     const int n = (int)k;
     const double w = table[n & 63];
-    return __longlong_as_double(__double_as_longlong(fma(w, (double)q, w)) + ((long long)(n >> 6) << 52));
+    const double scaled = __longlong_as_double(__double_as_longlong(fma(w, (double)q, w)) + ((long long)(n >> 6) << 52));
+    return x == top ? 1.0 : scaled;  // (+inf among them)
   }
 };
 
@@ -279,7 +316,7 @@ struct SampleAlone {
       hi = up;
     }
     const int n = s.listed;
-    sort_list(s, n);
+    sort_list(s.list, n);
     if (threadIdx.x == 0) {
       int at = min(rank, n - 1);
       if (MASS) {
@@ -418,7 +455,7 @@ __device__ int sample_list(SampleShared &s, const SampleScale &z, int n, double 
   // by index: the halves of a place change sides
   for (int i = threadIdx.x; i < n; i += SA_THREADS) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;
   __syncthreads();
-  sort_list(s, n);
+  sort_list(s.list, n);
   mine = 0;
 #pragma unroll
   for (int e = 0; e < SA_EACH; ++e) {
@@ -450,141 +487,211 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   T *const copy = reinterpret_cast<T *>(smem_raw + (sizeof(SampleShared) + 15) / 16 * 16);
   cg::cluster_group cluster = cg::this_cluster();
   const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), b = blockIdx.x / C;
+  const int tid = threadIdx.x, warp = tid / WARP, lane = tid % WARP;
   auto started = cluster.barrier_arrive();
   pdl_prologue();
   const double temperature = a.temperature ? (double)a.temperature[b] : a.temperature0;
   const double p = a.top_p ? (double)a.top_p[b] : a.top_p0, min_p = fmin(a.min_p ? (double)a.min_p[b] : a.min_p0, 1.0), u = a.u[b];
   const int k = a.top_k ? a.top_k[b] : a.top_k0;
   const T *const row = static_cast<const T *>(a.logits) + b * a.ld;
+  constexpr int N = VEC ? Chunk<T>::N : 1;
   const int from = min(a.V, rank * slice), to = min(a.V, from + slice);
   const T *const entries = stored ? copy - from : row;  // entries[i], from <= i < to
+  // a warp's share of the slice, in index order
+  const int share = ((to - from + SA_WARPS - 1) / SA_WARPS + WARP * N - 1) / (WARP * N) * (WARP * N);
+  const int lo = min(to, from + warp * share), hi = min(to, lo + share);
   SampleShared &first = *cluster.map_shared_rank(&s, 0);
   SampleAlone<T, VEC> r{row, a.V, s, {}};
   SampleScale &z = r.z;
-  auto mine = [&](auto f) { sweep<T, VEC>(entries, from, to, threadIdx.x, SA_THREADS, f); };
+  // f(x, index) for the warp's entries (a short body: all of it stays in the instruction cache)
+  auto mine = [&](auto f) {
+    for (int i = lo + lane * N; i < hi; i += WARP * N) {
+      if (VEC && i + N <= hi) {
+        float x[N];
+        unpack_chunk<T>(*reinterpret_cast<const uint4 *>(entries + i), x);
+#pragma unroll
+        for (int e = 0; e < N; ++e) f(x[e], i + e);
+      } else {
+        for (int e = i; e < min(hi, i + N); ++e) f(to_f(entries[e]), e);
+      }
+    }
+  };
 
   // 1. the slice, and the row's largest and smallest entries
-  u64 best = 0, least = ~0ull;
+  float top = -INFINITY, bottom = INFINITY;
+  int top_at = 0;
   {
     auto see = [&](float x, int i) {
-      const uint32_t key = order_of(x);
-      if (key <= SA_NONE) return;
-      const u64 place = place_of(key, i);
-      best = place > best ? place : best;
-      least = key < least ? key : least;
+      if (x > top) {  // (not -inf, not NaN; of equal ones the first)
+        top = x;
+        top_at = i;
+      }
+      if (x > -INFINITY) bottom = fminf(bottom, x);
     };
-    constexpr int N = Chunk<T>::N;
-    if (VEC && stored) {
-      for (int i0 = from + (int)threadIdx.x * N; i0 < to; i0 += 4 * SA_THREADS * N) {
-        uint4 v[4];
+    if (VEC) {
+      constexpr int DEEP = 4;
+      for (int i0 = lo + lane * N; i0 < hi; i0 += DEEP * WARP * N) {
+        uint4 v[DEEP];
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
-          if (i0 + d * SA_THREADS * N + N <= to) v[d] = ld_stream16(row + i0 + d * SA_THREADS * N);
-#pragma unroll
-        for (int d = 0; d < 4; ++d) {
-          const int i = i0 + d * SA_THREADS * N;
-          if (i + N <= to) {
+        for (int d = 0; d < DEEP; ++d)
+          if (i0 + d * WARP * N + N <= hi) v[d] = ld_stream16(row + i0 + d * WARP * N);
+#pragma unroll 1
+        for (int d = 0; d < DEEP; ++d) {
+          const int i = i0 + d * WARP * N;
+          if (i + N <= hi) {
             float x[N];
-            unpack_chunk<T>(v[d], x);
-            *reinterpret_cast<uint4 *>(copy + (i - from)) = v[d];
+            unpack_chunk<T>(v[0], x);
+            if (stored) *reinterpret_cast<uint4 *>(copy + (i - from)) = v[0];
 #pragma unroll
             for (int e = 0; e < N; ++e) see(x[e], i + e);
+#pragma unroll
+            for (int e = 0; e + 1 < DEEP; ++e) v[e] = v[e + 1];
           } else {
-            for (int e = i; e < to; ++e) {
-              copy[e - from] = row[e];
+            for (int e = i; e < hi; ++e) {
+              if (stored) copy[e - from] = row[e];
               see(to_f(row[e]), e);
             }
           }
         }
       }
     } else {
-      sweep<T, VEC>(row, from, to, threadIdx.x, SA_THREADS, [&](float x, int i) {
+      for (int i = lo + lane; i < hi; i += WARP) {
         if (stored) copy[i - from] = row[i];
-        see(x, i);
-      });
+        see(to_f(row[i]), i);
+      }
     }
   }
-  if (threadIdx.x < 64) s.table[threadIdx.x] = exp2(threadIdx.x * 0.015625);
-  for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) s.count[i] = s.into[i] = 0;
-  if (threadIdx.x == 0) s.listed = 0;
+  if (tid < 64) s.table[tid] = exp2(tid * 0.015625);
+  for (int i = tid; i < SA_BINS; i += SA_THREADS) s.count[i] = s.into[i] = 0;
+  if (tid == 0) s.listed = s.own = 0;
+  u64 best = top > -INFINITY ? place_of(order_of(top), top_at) : 0;
   best = block_all(best, s.wide, [](u64 x, u64 y) { return x > y ? x : y; });
-  least = block_all(least, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
+  bottom = block_all(bottom, s.narrow, [](float x, float y) { return fminf(x, y); });
   cluster.barrier_wait(std::move(started));  // (all blocks of the cluster have started)
-  if ((int)threadIdx.x < C) {
-    SampleShared &other = *cluster.map_shared_rank(&s, threadIdx.x);
+  if (tid < C) {
+    SampleShared &other = *cluster.map_shared_rank(&s, tid);
     other.best[rank] = best;
-    other.least[rank] = least;
+    other.least[rank] = bottom;
   }
   cluster.sync();
-  for (int c = 0; c < C; ++c) {
-    best = s.best[c] > best ? s.best[c] : best;
-    least = s.least[c] < least ? s.least[c] : least;
+#pragma unroll
+  for (int c = 0; c < SA_CLUSTER; ++c) {
+    if (c < C) {
+      best = s.best[c] > best ? s.best[c] : best;
+      bottom = fminf(bottom, s.least[c]);
+    }
   }
   const int arg = best ? (int)~(uint32_t)best : -1;
   if (arg < 0 || !(temperature > 0) || k == 1) {
-    if (rank == 0 && threadIdx.x == 0) a.token[b] = arg;
+    if (rank == 0 && tid == 0) a.token[b] = arg;
     return;
   }
   z.top = logit_of((uint32_t)(best >> 32));
   z.temperature = temperature;
-  const double c = 1.4426950408889634 / temperature;
-  z.c_hi = (float)c;
-  z.c_lo = (float)(c - (double)z.c_hi);
+  const double log2_unit = 1.4426950408889634 / temperature;
+  z.c_hi = (float)log2_unit;
+  z.c_lo = (float)(log2_unit - (double)z.c_hi);
   z.reach = (float)fmin(SA_FAR * temperature, 3e38);
-  const float range = fminf(z.top - logit_of((uint32_t)least), z.reach);
+  const float range = fminf(z.top - bottom, z.reach);
   z.inv = range > 0.f && range < 3e38f ? SA_BINS / range * 0.99999f : 0.f;
   bool by_rank = k > 0 && k < a.V;
   const bool by_mass = p < 1;
   u64 cut = 0;
+  int rank_bin = SA_BINS;  // the step with the last entry that top-k keeps
 
   // One block goes on alone; the others have nothing left to do.
   auto alone = [&]() {
     const int token = r.token(k, p, min_p, u);
-    if (threadIdx.x == 0) a.token[b] = token;
+    if (tid == 0) a.token[b] = token;
   };
-  // Entries of steps lo .. hi at or in front of the cut go to the first block's list; weights in front of them and behind, if wanted, to
-  // its sums. Returns the list's length and the sums, in the first block.
-  auto collect = [&](int lo, int hi, bool sums, double &in_front, double &behind) -> int {
-    double x0 = 0, x1 = 0;
+  // The block's own list (indices; fewer than SA_LIST, as the counts say): begun, an entry, and sent to the first block's list.
+  auto begin_list = [&]() {
+    if (tid == 0) s.own = 0;
+    __syncthreads();
+  };
+  auto own = [&](int i) { s.owned[atomicAdd(&s.own, 1) & (SA_LIST - 1)] = i; };
+  auto send_list = [&]() {
+    __syncthreads();
+    const int n = s.own;
+    if (tid == 0) s.found[0] = n ? atomicAdd(&first.listed, n) : 0;
+    __syncthreads();
+    const int at = s.found[0];
+    for (int i = tid; i < n && at + i < SA_LIST; i += SA_THREADS) {
+      const int j = s.owned[i];
+      first.list[at + i] = place_of(order_of(to_f(entries[j])), j);
+    }
+  };
+  // Entries of steps from .. to - 1 go to the first block's list.
+  auto collect = [&](float from, float to) {
+    begin_list();
     mine([&](float x, int i) {
-      if (!z.counts(x)) return;
-      const int bin = z.bin_of(x);
-      const u64 place = place_of(order_of(x), i);
-      if (place < cut) return;
-      if (bin >= lo && bin <= hi) {
-        const int at = atomicAdd(&first.listed, 1);
-        if (at < SA_LIST) first.list[at] = place;
-      } else if (sums) {
-        const double w = z.weight(x, s.table);
-        if (bin < lo) x0 += w;
-        else x1 += w;
-      }
+      const float at = z.step_of(x);
+      if (at >= from && at < to && z.counts(x)) own(i);
     });
-    if (sums) {
-      x0 = block_total(x0, s);
-      x1 = block_total(x1, s);
-      if (threadIdx.x == 0) {
-        first.sums[rank][0] = x0;
-        first.sums[rank][1] = x1;
+    send_list();
+    cluster.sync();
+  };
+  const bool by_min = min_p > 0;
+  auto enough = [&](float x, double w) { return w >= min_p * (1 + 1e-8) || (w >= min_p * (1 - 1e-8) && z.exact(x) >= min_p); };
+  // Weights of the entries that top-k keeps: in front of step `from` and from step `to` on (to the first block's sums), and, in s.part, of the
+  // first ones that min-p keeps too, warp by warp. Those between go to the lists. (No branches around the weights, so that those
+  // of a chunk overlap.)
+  auto weigh = [&](float from, float to) {
+    begin_list();
+    double x0 = 0, x1 = 0, x2 = 0;
+    for (int i = lo + lane * N; i < hi; i += WARP * N) {
+      float x[N];
+      if (VEC && i + N <= hi) {
+        unpack_chunk<T>(*reinterpret_cast<const uint4 *>(entries + i), x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = i + e < hi ? to_f(entries[i + e]) : -INFINITY;
+      }
+      unsigned between = 0;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float at = z.step_of(x[e]);
+        bool keep = z.counts(x[e]);
+        if (rank_bin < SA_BINS) keep = keep && (at < rank_bin || (at < rank_bin + 1 && place_of(order_of(x[e]), i + e) >= cut));
+        const bool mid = keep && at >= from && at < to;
+        double w = z.weight(x[e], s.table);
+        w = keep && !mid ? w : 0.0;
+        x0 += at < from ? w : 0.0;
+        x1 += at < from ? 0.0 : w;
+        if (by_min && at < from && w > 0 && enough(x[e], w)) x2 += w;
+        between |= (unsigned)mid << e;
+      }
+      while (between) {
+        own(i + __ffs(between) - 1);
+        between &= between - 1;
       }
     }
-    cluster.sync();
-    in_front = behind = 0;
-    if (rank != 0) return 0;
-    if (sums)
-      for (int c = 0; c < C; ++c) {
-        in_front += s.sums[c][0];
-        behind += s.sums[c][1];
-      }
-    return s.listed;
+    if (!by_min) x2 = x0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      x0 += __shfl_xor_sync(0xffffffffu, x0, o);
+      x1 += __shfl_xor_sync(0xffffffffu, x1, o);
+      x2 += __shfl_xor_sync(0xffffffffu, x2, o);
+    }
+    if (lane == 0) {
+      s.part[warp] = x2;
+      s.part2[warp] = x0;
+      s.part3[warp] = x1;
+    }
+    send_list();
+    if (tid < 2) {
+      double sum = 0;
+      for (int w = 0; w < SA_WARPS; ++w) sum += tid ? s.part3[w] : s.part2[w];
+      first.sums[rank][tid] = sum;
+    }
   };
   // The first block tells all the cut, or that they are not needed any more.
   auto tell = [&](u64 value, bool done) {
     if (rank == 0) {
       __syncthreads();  // (the list has been read)
-      if (threadIdx.x == 0) s.listed = 0;
-      if ((int)threadIdx.x < C) {
-        SampleShared &other = *cluster.map_shared_rank(&s, threadIdx.x);
+      if (tid == 0) s.listed = 0;
+      if (tid < C) {
+        SampleShared &other = *cluster.map_shared_rank(&s, tid);
         other.cut = value;
         other.done = done;
       }
@@ -593,50 +700,52 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     cut = s.cut;
     return s.done != 0;
   };
-  // The first block makes the rest of what it has in the list.
-  auto finish = [&](int n, double behind) {
-    sort_list(s, n);
-    const int token = sample_list(s, z, by_rank ? min(n, k) : n, behind, p, min_p, u);
+  // The first block makes the rest of what it has in the list, `behind` is the weight of the others that top-p counts.
+  auto finish = [&](int most, double behind) {
+    const int n = s.listed;
+    sort_list(s.list, n);
+    const int token = sample_list(s, z, min(n, most), behind, p, min_p, u);
     const bool close = s.found[1] != 0;
     __syncthreads();
     if (close) alone();
-    else if (threadIdx.x == 0) a.token[b] = token;
+    else if (tid == 0) a.token[b] = token;
   };
 
   if (by_rank || by_mass) {
     // 2. counts of the steps: of the slice, then of the row and running
-    const int fine = 1 << min(12, __clz(a.V) - 1);  // (the sum over the row stays below 2^31)
+    const float fine = (float)(1 << min(12, __clz(a.V) - 1));  // (the sum over the row stays below 2^31)
     mine([&](float x, int) {
       if (!z.counts(x)) return;
-      unsigned into;
-      const int bin = z.bin_of(x, (float)fine, into);
+      const float at = z.step_of(x);
+      const int bin = min(SA_BINS - 1, (int)at);
       atomicAdd(&s.count[bin], 1u);
-      if (by_mass) atomicAdd(&s.into[bin], into);
+      if (by_mass) atomicAdd(&s.into[bin], (unsigned)((at - bin) * fine));
     });
     cluster.sync();
-    unsigned n[SA_EACH] = {}, sum = 0, into[SA_EACH] = {};
-    const int at = threadIdx.x * SA_EACH;
-    for (int c = 0; c < C; ++c) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(&cluster.map_shared_rank(&s, c)->count[at]);
-      n[0] += v.x;
-      n[1] += v.y;
-      n[2] += v.z;
-      n[3] += v.w;
-      if (by_mass) {
-        const uint4 y = *reinterpret_cast<const uint4 *>(&cluster.map_shared_rank(&s, c)->into[at]);
-        into[0] += y.x;
-        into[1] += y.y;
-        into[2] += y.z;
-        into[3] += y.w;
+    static_assert(SA_EACH == 4, "16-byte loads of counts");
+    const int at = tid * SA_EACH;
+    unsigned n[SA_EACH] = {}, into[SA_EACH] = {};
+#pragma unroll
+    for (int c0 = 0; c0 < SA_CLUSTER; c0 += 4) {
+      uint4 x[4], y[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        x[c] = y[c] = make_uint4(0, 0, 0, 0);
+        if (c0 + c < C) {
+          const SampleShared &other = *cluster.map_shared_rank(&s, c0 + c);
+          x[c] = *reinterpret_cast<const uint4 *>(&other.count[at]);
+          if (by_mass) y[c] = *reinterpret_cast<const uint4 *>(&other.into[at]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        n[0] += x[c].x, n[1] += x[c].y, n[2] += x[c].z, n[3] += x[c].w;
+        into[0] += y[c].x, into[1] += y[c].y, into[2] += y[c].z, into[3] += y[c].w;
       }
     }
-    static_assert(SA_EACH == 4, "one 16-byte load of counts");
-    sum = n[0] + n[1] + n[2] + n[3];
+    auto read = cluster.barrier_arrive();
     double total;
-    unsigned run = (unsigned)block_before(sum, s.part, total);
-    if (threadIdx.x == 0) s.found[2] = s.found[3] = SA_BINS - 1;
-    __syncthreads();
-    int rank_bin = SA_BINS;
+    const unsigned run = (unsigned)block_before(n[0] + n[1] + n[2] + n[3], s.part, total);
     by_rank = by_rank && total > k;
     {
       unsigned upto = run;
@@ -650,23 +759,22 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     __syncthreads();
     if (by_rank) rank_bin = s.found[2];
     const int rank_upto = by_rank ? (int)s.upto[rank_bin] : 0, rank_before = by_rank && rank_bin ? (int)s.upto[rank_bin - 1] : 0;
-    double in_front, behind;
+    cluster.barrier_wait(std::move(read));  // (nobody reads counts any more)
     if (by_rank) {
       // 3. top-k
       const bool whole = rank_upto <= SA_LIST;
       if (!whole && rank_upto - rank_before > SA_LIST) {
-        cluster.sync();  // (counts have been read)
         if (rank == 0) alone();
         return;
       }
-      const int listed = collect(whole ? 0 : rank_bin, rank_bin, false, in_front, behind);
+      collect(whole ? 0 : rank_bin, rank_bin + 1);
       if (whole) {
-        if (rank == 0) finish(listed, 0);
+        if (rank == 0) finish(k, 0);
         return;
       }
       u64 place = 0;
       if (rank == 0) {
-        sort_list(s, listed);
+        sort_list(s.list, s.listed);
         place = s.list[k - 1 - rank_before];
       }
       tell(place, false);
@@ -675,141 +783,140 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
       // top-p: bounds of the running sums at the steps' borders. A step's n entries at f_i of it (0 .. 1) weigh E 2^(-c f_i) each, E at its
       // beginning: together at least E n 2^(-c F), with F the average, and at most E n (1 - F (1 - 2^-c)). What (top - x) * inv is rounded by
       // is below 2048 * 2^-22 of a step; all in all the bounds are widened by 1e-5.
-      const double width = z.inv > 0.f ? 1.0 / z.inv : 0.0, per = c * width, full = exp2(-per);
-      double lo[SA_EACH], hi[SA_EACH], lo_sum = 0, hi_sum = 0, lo_total, hi_total;
+      const double width = z.inv > 0.f ? 1.0 / z.inv : 0.0, per = log2_unit * width, full = exp2(-per);
+      double begin = exp2(-per * at);
+      double low[SA_EACH], high[SA_EACH], low_total, high_total;
 #pragma unroll
       for (int e = 0; e < SA_EACH; ++e) {
         const int bin = at + e;
-        lo[e] = hi[e] = 0;
+        low[e] = high[e] = 0;
         if (n[e] && bin <= rank_bin) {
-          const double begin = exp2(-per * bin);
           if (bin < rank_bin) {
-            const double f = (double)into[e] / ((double)n[e] * fine);
-            hi[e] = begin * n[e] * (1 - f * (1 - full)) * (1 + 1e-5);
-            lo[e] = begin * n[e] * exp2(-per * (f + 1.0 / fine)) * (1 - 1e-5);
+            const double f = __fdividef((float)into[e], (float)n[e] * fine);
+            high[e] = begin * n[e] * (1 - f * (1 - full)) * (1 + 1e-5);
+            low[e] = begin * n[e] * exp2f((float)(-per * (f + 1.0 / fine))) * (1 - 1e-5);
           } else {  // only the first ones of the step
-            hi[e] = begin * (k - rank_before) * (1 + 1e-5);
-            lo[e] = begin * (k - rank_before) * full * (1 - 1e-5);
+            high[e] = begin * (k - rank_before) * (1 + 1e-5);
+            low[e] = begin * (k - rank_before) * full * (1 - 1e-5);
           }
-          if (z.inv == 0.f) lo[e] = 0;  // (no steps: equal entries, or a range that floats do not hold)
+          if (z.inv == 0.f) low[e] = 0;  // (no steps: equal entries, or a range that floats do not hold)
         }
-        hi_sum += hi[e];
-        lo_sum += lo[e];
+        begin *= full;
       }
-      double hi_run = block_before(hi_sum, s.part, hi_total), lo_run = block_before(lo_sum, s.part2, lo_total);
+      double high_run = block_before(high[0] + high[1] + high[2] + high[3], s.part, high_total);
+      double low_run = block_before(low[0] + low[1] + low[2] + low[3], s.part2, low_total);
       // can: the first step at whose end the sum can have reached p of the total; must: the first at whose end it has to have
-      int can = SA_BINS - 1, must = SA_BINS - 1;
+      unsigned can = SA_BINS - 1, must = SA_BINS - 1;
 #pragma unroll
-      for (int e = SA_EACH - 1; e >= 0; --e) {
-        double x = hi_run, y = lo_run;
-        for (int f = 0; f <= e; ++f) {
-          x += hi[f];
-          y += lo[f];
-        }
-        if (x >= p * lo_total) can = at + e;
-        if (y >= p * hi_total) must = at + e;
+      for (int e = 0; e < SA_EACH; ++e) {
+        high_run += high[e];
+        low_run += low[e];
+        if (can == SA_BINS - 1 && high_run >= p * low_total) can = at + e;
+        if (must == SA_BINS - 1 && low_run >= p * high_total) must = at + e;
       }
-      can = (int)block_all((u64)can, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
-      must = (int)block_all((u64)must, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
-      int most = (int)s.upto[must], least_n = can ? (int)s.upto[can - 1] : 0;
+      const u64 both = block_all((u64)can << 32 | can, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
+      must = (unsigned)block_all((u64)must, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
+      can = (unsigned)both;
+      int most = (int)s.upto[must], least = can ? (int)s.upto[can - 1] : 0;
       if (by_rank) {
         most = min(most, k);
-        least_n = min(least_n, k);
+        least = min(least, k);
       }
-      const bool whole = most <= SA_LIST;
-      if (!whole && most - least_n > SA_LIST) {
-        cluster.sync();
+      const bool whole = most <= SA_LIST / 4;  // (a longer list is sorted in more time than it saves)
+      if (!whole && most - least > SA_LIST) {
         if (rank == 0) alone();
         return;
       }
-      const int listed = collect(whole ? 0 : can, must, true, in_front, behind);
+      weigh(whole ? 0.f : (float)can, (float)must + 1.f);
+      cluster.sync();
       if (whole) {
         if (rank == 0) {
-          by_rank = false;  // (the cut is in the list)
-          finish(listed, behind);
+          double behind = 0;
+          for (int c = 0; c < C; ++c) behind += s.sums[c][1];
+          finish(SA_LIST, behind);
         }
         return;
       }
       u64 place = cut;
       bool close = false;
-      if (rank == 0 && listed > 0) {
-        sort_list(s, listed);
-        double w[SA_EACH], sum = 0, between;
+      if (rank == 0 && s.listed > 0) {
+        const int length = s.listed;
+        double in_front = 0, behind = 0, w[SA_EACH], sum = 0, between;
+        for (int c = 0; c < C; ++c) {
+          in_front += s.sums[c][0];
+          behind += s.sums[c][1];
+        }
+        sort_list(s.list, length);
 #pragma unroll
         for (int e = 0; e < SA_EACH; ++e) {
-          w[e] = at + e < listed ? z.weight(logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
+          w[e] = at + e < length ? z.weight(logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
           sum += w[e];
         }
-        double before = in_front + block_before(sum, s.part, between);
+        double before = in_front + block_before(sum, s.part2, between);
         const double all = in_front + between + behind, mass = p * all;
         bool near = false;
-        int last = 0;
+        unsigned last = 0;
 #pragma unroll
         for (int e = 0; e < SA_EACH; ++e) {
-          if (at + e < listed && at + e > 0) {
+          if (at + e < length && at + e > 0) {
             near |= fabs(before - mass) <= SA_CLOSE * all;
             if (before < mass) last = at + e;
           }
           before += w[e];
         }
-        last = (int)block_all((u64)last, s.wide, [](u64 x, u64 y) { return x > y ? x : y; });
-        close = block_all((u64)near, s.wide, [](u64 x, u64 y) { return x | y; }) != 0;
-        place = s.list[last];
+        const u64 found = block_all((u64)near << 32 | last, s.wide, [](u64 x, u64 y) { return max(x >> 32, y >> 32) << 32 | max((unsigned)x, (unsigned)y); });
+        close = (found >> 32) != 0;
+        place = s.list[(unsigned)found];
       }
       if (tell(place, close)) {
         if (rank == 0) alone();
         return;
       }
+      // the block's own entries between the bounds, as far as they are kept, join their warps' sums
+      for (int i = tid; i < s.own; i += SA_THREADS) {
+        const int j = s.owned[i];
+        const float x = to_f(entries[j]);
+        if (place_of(order_of(x), j) < cut) continue;
+        const double w = z.weight(x, s.table);
+        if (!by_min || enough(x, w)) atomicAdd(&s.part[(j - from) / share], w);
+      }
+      __syncthreads();
     }
   }
+  if (!by_mass) weigh(INFINITY, INFINITY);
 
   // 4. the sums of what is kept, in index order
-  {
-    const int warp = threadIdx.x / WARP, lane = threadIdx.x % WARP;
-    constexpr int N = VEC ? Chunk<T>::N : 1;
-    const int share = ((to - from + SA_WARPS - 1) / SA_WARPS + WARP * N - 1) / (WARP * N) * (WARP * N);
-    const int lo = min(to, from + warp * share), hi = min(to, lo + share);
-    auto kept = [&](float x, int i) -> double {
-      if (!z.counts(x) || place_of(order_of(x), i) < cut) return 0.0;
-      const double w = z.weight(x, s.table);
-      if (min_p > 0 && w < min_p * (1 + 1e-8) && (w < min_p * (1 - 1e-8) || z.exact(x) < min_p)) return 0.0;
-      return w;
-    };
-    double sum = 0;
-    sweep<T, VEC>(entries, lo, hi, lane, WARP, [&](float x, int i) { sum += kept(x, i); });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    __syncthreads();
-    if (lane == 0) s.part[warp] = sum;
-    __syncthreads();
-    sum = 0;
-    for (int w = 0; w < SA_WARPS; ++w) sum += s.part[w];
-    if ((int)threadIdx.x < C) cluster.map_shared_rank(&s, threadIdx.x)->kept[rank] = sum;
-    cluster.sync();
-    double total = 0, before = 0;
-    for (int c = 0; c < C; ++c) total += s.kept[c];
-    const double target = u * total;
-    int owner = C, last = 0;
-    double mine_before = 0;
-    for (int c = 0; c < C; ++c) {
-      if (s.kept[c] > 0) last = c;
-      if (owner == C && before + s.kept[c] > target) {
-        owner = c;
-        mine_before = before;
-      }
-      before += s.kept[c];
+  __syncthreads();
+  double sum = 0;
+  for (int w = 0; w < SA_WARPS; ++w) sum += s.part[w];
+  if (tid < C) cluster.map_shared_rank(&s, tid)->kept[rank] = sum;
+  cluster.sync();
+  double total = 0, before = 0, in_front = 0;
+  for (int c = 0; c < C; ++c) total += s.kept[c];
+  const double target = u * total;
+  int owner = C, last = 0;
+  for (int c = 0; c < C; ++c) {
+    if (s.kept[c] > 0) last = c;
+    if (owner == C && before + s.kept[c] > target) {
+      owner = c;
+      in_front = before;
     }
-    if (owner == C) {  // (rounding: the last entry that is kept)
-      owner = last;
-      mine_before = before;
-    }
-    if (rank != owner) return;
-    const int token = r.locate(entries, lo, hi, mine_before, target, total, kept);
-    const bool close = s.found[1] != 0;
-    __syncthreads();
-    if (close) alone();
-    else if (threadIdx.x == 0) a.token[b] = token;
+    before += s.kept[c];
   }
+  if (owner == C) {  // (rounding: the last entry that is kept)
+    owner = last;
+    in_front = before;
+  }
+  if (rank != owner) return;
+  const int token = r.locate(entries, lo, hi, in_front, target, total, [&](float x, int i) -> double {
+    if (!z.counts(x) || place_of(order_of(x), i) < cut) return 0.0;
+    const double w = z.weight(x, s.table);
+    return !by_min || enough(x, w) ? w : 0.0;
+  });
+  const bool close = s.found[1] != 0;
+  __syncthreads();
+  if (close) alone();
+  else if (tid == 0) a.token[b] = token;
 }
 
 // Blocks of a row: as many as keep the device busy with B rows, more where a slice would leave room for one block per multiprocessor.
