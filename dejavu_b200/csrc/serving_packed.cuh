@@ -21,11 +21,23 @@ int packed_tc(int dtype, const PackedArgs &a, cudaStream_t st);
 struct PackedTile {
   int first, q0, rows;  // the sequence's first row, the tile's first query in it, its queries (<= 0: no tile)
   int rest;             // 1: rows of no sequence
+  int b;                // the sequence
 };
 
 // Tiles of Q rows that B sequences of T rows in all can make, those of no sequence among them.
 template <int Q>
 inline int packed_tiles(int T, int B) { return T / Q + B + 2 < T + 2 ? T / Q + B + 2 : T + 2; }
+
+// Tiles of Q rows that the sequences make. Whole warp.
+template <int Q>
+__device__ __forceinline__ int packed_total(const PackedArgs &a) {
+  int t = 0;
+  for (int b = threadIdx.x % WARP; b < a.B; b += WARP) {
+    const int lo = max(0, min(a.cu[b], a.T));
+    t += (max(0, min(a.cu[b + 1], a.T) - lo) + Q - 1) / Q;
+  }
+  return __reduce_add_sync(0xffffffffu, t);
+}
 
 // Tile number `index`: tiles of the sequences in order, then of the rows in front of the first and behind the last. Whole warp. Whatever
 // cu holds, rows are within 0 .. T - 1.
@@ -52,15 +64,15 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedArgs &a, int index
       const int who = __ffs(here) - 1;
       const int first = __shfl_sync(0xffffffffu, lo, who), rows = __shfl_sync(0xffffffffu, n, who);
       const int before = seen + __shfl_sync(0xffffffffu, s - t, who), q0 = (index - before) * Q;
-      return {first, q0, min(Q, rows - q0), 0};
+      return {first, q0, min(Q, rows - q0), 0, b0 + who};
     }
     seen += __shfl_sync(0xffffffffu, s, WARP - 1);
   }
   const int head = max(0, min(a.cu[0], a.T)), tail = max(0, min(a.cu[a.B], a.T));
   const int at = (index - seen) * Q;
   const int in_head = (head + Q - 1) / Q * Q;
-  if (at < in_head) return {0, at, min(Q, head - at), 1};
-  return {tail, at - in_head, min(Q, a.T - tail - (at - in_head)), 1};
+  if (at < in_head) return {0, at, min(Q, head - at), 1, -1};
+  return {tail, at - in_head, min(Q, a.T - tail - (at - in_head)), 1, -1};
 }
 
 }  // namespace djv

@@ -2,15 +2,19 @@
 //
 // Persistent blocks, one per multiprocessor, walk items of 256 queries of one head: two tiles of 128 that share the key and value
 // tiles they pass, so that one tile's softmax runs while the tensor cores work for the other. Roles:
-//   warps 0-3, 4-7  softmax and results of a query tile each, a thread per row: S (TMEM, fp32) -> weights in the inputs' type, over S
-//   warp 8          one thread loads: Q tiles, and K and V tiles of 128 keys into a ring, by TMA
-//   warp 9          one thread issues the products: S = Q K^T, O (TMEM) += P V
-//   warps 10, 11    look through the value tiles that hold keys some row does not see (the last one or two of an item)
+//   warps 0-7, 8-15 softmax and results of a query tile each, two threads per row, 64 keys each: S (TMEM, fp32) -> weights in the inputs'
+//                   type, over S
+//   warp 16         one thread loads: Q tiles, and K and V tiles of 128 keys into a ring, by TMA
+//   warp 17         one thread issues the products: S = Q K^T, O (TMEM) += P V
+//   warps 18, 19    look through the value tiles that hold keys some row does not see (the last one or two of an item)
 // With one score tile per query tile in TMEM (S 2 x 128 + O 2 x 128 columns are all there is) a tile's steps are a chain: QK, softmax, PV;
 // the two tiles' chains interleave.
 //
 // O is only rescaled when a row's maximum grows by more than 2^8 (the division by the sum makes up for the rest), by the softmax
-// threads themselves: the barrier that says S is there also says that the product before it is complete.
+// threads themselves: the barrier that says S is there also says that the product before it is complete. Whether any row of a tile has
+// grown is a barrier with a vote; only then do a row's two threads tell one another their maxima.
+//
+// Items go out in the order of falling work, back and forth over the blocks; sequences may have any lengths.
 //
 // What a row does not see must not reach it: scores are masked by comparison, but a weight of 0 times an infinity would be NaN. So
 // entries of those value tiles that are not finite are set to 0 before the products, and joined again at the end for the rows that
@@ -22,8 +26,64 @@
 
 namespace djv {
 
-constexpr int PT_THREADS = 384, PT_M = 128, PT_N = 128, PT_Q = 2 * PT_M;  // rows of a query tile, of a key tile, of an item
-constexpr int PT_LOADER = 8, PT_ISSUER = 9, PT_SCAN = 10;
+constexpr int PT_THREADS = 640, PT_M = 128, PT_N = 128, PT_Q = 2 * PT_M;  // rows of a query tile, of a key tile, of an item
+constexpr int PT_SOFT = 16, PT_LOADER = 16, PT_ISSUER = 17, PT_SCAN = 18;  // softmax warps, and the others
+constexpr int PT_TABLE = 1024;  // items per head that are put in order
+
+// whether `mine` holds for any of a tile's 256 threads; a barrier of them
+__device__ __forceinline__ bool any_of_tile(int t, bool mine) {
+  int any;
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      "setp.ne.s32 p, %2, 0;\n"
+      "barrier.cta.red.or.pred q, %1, 256, p;\n"
+      "selp.s32 %0, 1, 0, q;\n"
+      "}\n"
+      : "=r"(any)
+      : "r"(t + 1), "r"((int)mine)
+      : "memory");
+  return any != 0;
+}
+// Products and commits by one thread of a warp that runs as one: what they are given stays in uniform registers (from one thread's own
+// branch every operand of every product would have to be moved there, 60 to 130 cycles for each).
+__device__ __forceinline__ void warp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void warp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void warp_commit(uint64_t *bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tile_sync(int t) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(t + 1) : "memory"); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 
 __device__ unsigned g_packed_timeouts;  // bounded waits that ran out (never, in a healthy run)
 
@@ -57,14 +117,16 @@ struct Exponent<__half> {
   static constexpr uint32_t MASK = 0x7c007c00u, ONE = 0x04000400u;
 };
 
-template <typename T, int KB, int STAGES>  // KB: blocks of 64 elements in a row
+template <typename T, int KB, int STAGES, bool FULL>  // KB: blocks of 64 elements in a row; FULL: all of them are in use
 __global__ void __launch_bounds__(PT_THREADS, 1)
 packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, PackedArgs a, int tiles) {
+                 const __grid_constant__ CUtensorMap map_v, PackedArgs a, int most) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2],
       clean[STAGES], taken[2][2], drained;
   __shared__ uint32_t tmem_slot;
+  __shared__ float exch[2][2][PT_M];  // maxima, and in the end sums, of the two halves of a row
+  __shared__ int2 table[PT_TABLE];    // sequence and item in it, by falling work
   __shared__ int odd[2][2][2];  // by the item's parity: what each of the two warps found in each of the two value tiles
   constexpr uint32_t TILE = KB * PT_N * 128;
   const int tid = threadIdx.x, warp = tid / WARP, lane = tid % WARP;
@@ -75,10 +137,10 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], PT_M);
+      mbar_init(&p_full[t], 2 * PT_M);
       mbar_init(&o_full[t], 1);
-      mbar_init(&taken[0][t], 4);
-      mbar_init(&taken[1][t], 4);
+      mbar_init(&taken[0][t], 8);
+      mbar_init(&taken[1][t], 8);
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -90,26 +152,57 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   }
   if (warp == PT_ISSUER) tmem_alloc(&tmem_slot, 512);
   pdl_prologue();
+  // How many items there are, and if they are few their order: by falling number in the sequence, which is what they take.
+  // (Offsets that do not ascend can make more than `most`, which is all that offsets that do can make: the rest is left out.)
+  const int total = packed_total<PT_Q>(a), tiles = total < 0 || total > most ? most : total;
+  const bool ordered = tiles == total && tiles <= PT_TABLE && (long long)tiles * a.B <= 64 * 1024;
+  if (ordered) {
+    for (int i = warp; i < tiles; i += PT_THREADS / WARP) {
+      const PackedTile w = packed_tile<PT_Q>(a, i);
+      const int q = w.q0 / PT_Q;
+      int before = 0;
+      for (int b = lane; b < a.B; b += WARP) {
+        const int lo = max(0, min(a.cu[b], a.T)), n = max(0, min(a.cu[b + 1], a.T) - lo), t = (n + PT_Q - 1) / PT_Q;
+        before += max(0, t - q - 1) + (b < w.b && t > q);
+      }
+      before = __reduce_add_sync(0xffffffffu, before);
+      if (lane == 0) table[before] = make_int2(w.b, q);
+    }
+  }
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tm = tmem_slot;
   const int items = tiles * a.H;
-  // Items in the order of falling work (later queries see more keys), dealt out back and forth
+  // items are dealt out back and forth
   auto item_of = [&](int round) {
     const int i = round * (int)gridDim.x + ((round & 1) ? (int)gridDim.x - 1 - (int)blockIdx.x : (int)blockIdx.x);
     return i < items ? i : -1;
   };
-  auto tile_of = [&](int item) { return packed_tile<PT_Q>(a, tiles - 1 - item / a.H); };  // whole warp
+  auto tile_of = [&](int item) {  // whole warp
+    if (!ordered) return packed_tile<PT_Q>(a, tiles - 1 - item / a.H);
+    const int2 x = table[item / a.H];
+    const int first = max(0, min(a.cu[x.x], a.T)), q0 = x.y * PT_Q;
+    return PackedTile{first, q0, min(PT_Q, min(a.cu[x.x + 1], a.T) - first - q0), 0, x.x};
+  };
   const int rounds = (items + (int)gridDim.x - 1) / (int)gridDim.x;
   bool dead = false;  // a wait ran out: wait no more, finish and report
 
-  if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    const int t = warp / 4, r = tid % PT_M;
-    const uint32_t lane_base = (uint32_t)(warp % 4 * 32) << 16, tm_s = tm + t * PT_N + lane_base, tm_o = tm + 2 * PT_N + t * (KB * 64) + lane_base;
+  if (warp < PT_SOFT) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int t = warp / 8, half = warp / 4 % 2, r = tid % PT_M;
+    const uint32_t lane_base = (uint32_t)(warp % 4 * 32) << 16;
+    // the thread's scores, over which it puts its weights, and its half of the columns of O
+    const uint32_t tm_s = tm + t * PT_N + half * 64 + lane_base, tm_o = tm + 2 * PT_N + t * (KB * 64) + lane_base;
     const float c = a.scale * 1.4426950408889634f, ca = c == 0.f ? 1e-30f : fabsf(c);  // scores in units of log 2
     const uint64_t ca2 = pack2(ca, ca);
+    if (!a.keep_rest) {  // rows of no sequence
+      const int head = max(0, min(a.cu[0], a.T)), tail = max(head, min(a.cu[a.B], a.T)), pieces = a.H * a.D / 8;
+      for (int i = blockIdx.x; i < head + a.T - tail; i += gridDim.x) {
+        uint4 *row = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + (long long)(i < head ? i : i - head + tail) * a.H * a.D);
+        for (int d = tid; d < pieces; d += PT_SOFT * WARP) row[d] = make_uint4(0, 0, 0, 0);
+      }
+    }
     int steps = 0, done = 0;  // phases of s_full and o_full
     int parity = 0;
     for (int round = 0; round < rounds; ++round) {
@@ -117,13 +210,6 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (item < 0) break;
       const PackedTile w = tile_of(item);
       const int h = item % a.H, rows = w.rows - t * PT_M;  // of this query tile
-      if (w.rows <= 0) continue;
-      T *out = static_cast<T *>(a.out) + ((long long)(w.first + w.q0 + t * PT_M + r) * a.H + h) * a.D;
-      if (w.rest) {
-        if (!a.keep_rest && r < rows)
-          for (int d = 0; d < a.D; d += 8) *reinterpret_cast<uint4 *>(out + d) = make_uint4(0, 0, 0, 0);
-        continue;
-      }
       parity ^= 1;
       if (rows <= 0) continue;
       const int last = w.q0 / PT_N + t;  // the key tile of the row's own key
@@ -132,39 +218,42 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!dead) dead = !mbar_wait(&s_full[t], steps & 1);
         __syncwarp();
         tmem_fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) tmem_ld32(s[q], tm_s + q * 32);
+        uint32_t s[2][32];
+        tmem_ld32(s[0], tm_s);
+        tmem_ld32(s[1], tm_s + 32);
         tmem_wait_ld();
         if (c < 0.f) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[q][e] ^= 0x80000000u;
         }
         if (j == last) {  // keys behind the row's own
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < 2; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (q * 32 + e > r) s[q][e] = 0xff800000u;
+              if (half * 64 + q * 32 + e > r) s[q][e] = 0xff800000u;
         }
         float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < 2; ++q)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mm[e % 4] = fmaxf(mm[e % 4], __uint_as_float(s[q][e]));
-        const float mx = fmaxf(fmaxf(mm[0], mm[1]), fmaxf(mm[2], mm[3])) * ca;
-        if (j == 0) {
-          m = mx == -INFINITY ? 0.f : mx;
-        } else {
-          const bool grow = mx > m + 8.f;
-          if (__any_sync(0xffffffffu, grow)) {
+          for (int e = 0; e < 32; e += 2) mm[e / 2 % 4] = max3(mm[e / 2 % 4], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
+        float mx = fmaxf(max3(mm[0], mm[1], mm[2]), mm[3]) * ca;
+        if (any_of_tile(t, j == 0 || mx > m + 8.f)) {
+          exch[t][half][r] = mx;
+          tile_sync(t);
+          mx = fmaxf(mx, exch[t][half ^ 1][r]);
+          if (j == 0) {
+            m = mx == -INFINITY ? 0.f : mx;
+          } else {
+            const bool grow = mx > m + 8.f;
             const float corr = grow ? exp2_approx(m - mx) : 1.f;
             if (grow) m = mx;
             l *= corr;
-#pragma unroll
-            for (int q = 0; q < KB * 64; q += 16) {
+#pragma unroll 1
+            for (int q = half * 16; q < KB * 64; q += 32) {
               uint32_t o[16];
               tmem_ld16(o, tm_o + q);
               tmem_wait_ld();
@@ -173,11 +262,12 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               tmem_st16(tm_o + q, o);
             }
           }
+          tile_sync(t);  // (before the next maxima are written)
         }
         const uint64_t nm2 = pack2(-m, -m);
         uint64_t l2[2] = {0, 0};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 2; ++q) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -197,6 +287,10 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         tmem_fence_before();
         mbar_arrive(&p_full[t]);
       }
+      exch[t][half][r] = l;
+      tile_sync(t);
+      l += exch[t][half ^ 1][r];
+      tile_sync(t);
       if (!dead) dead = !mbar_wait(&o_full[t], done & 1);
       ++done;
       __syncwarp();
@@ -205,8 +299,9 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const bool odd0 = (odd[parity][0][0] | odd[parity][0][1]) != 0, odd1 = (odd[parity][1][0] | odd[parity][1][1]) != 0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&taken[parity][t]);
+      T *out = static_cast<T *>(a.out) + ((long long)(w.first + w.q0 + t * PT_M + r) * a.H + h) * a.D;
 #pragma unroll 1
-      for (int q = 0; q < a.D; q += 16) {
+      for (int q = half * 16; q < a.D; q += 32) {
         uint32_t o[16];
         tmem_ld16(o, tm_o + q);
         tmem_wait_ld();
@@ -240,7 +335,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_fence_before();  // (the next item's first product into O waits for this thread's next weights)
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     int slot = 0;              // ring slots passed so far; slot n is stage n % STAGES in its n / STAGES-th use
     int used[2] = {0, 0};      // items that used query tile 0, 1
     unsigned looked = 0;       // phases of clean, a bit each
@@ -250,7 +345,6 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const int item = item_of(round);
       if (item < 0) break;
       const PackedTile w = tile_of(item);
-      if (w.rows <= 0 || w.rest) continue;
       const int h = item % a.H, g = h / (a.H / a.G), d0 = w.q0 / PT_N;
       const bool both = w.rows > PT_M;
       const int n = d0 + (both ? 2 : 1);  // key tiles
@@ -281,65 +375,83 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         dead = __shfl_sync(0xffffffffu, (int)dead, 0) != 0;
       } else if (warp == PT_ISSUER) {
-        if (lane == 0) {
-          constexpr bool FP16 = sizeof(T) == 2 && !__is_same(T, bf16);
-          const uint32_t idesc_s = mma_idesc(PT_M, PT_N, false, false, FP16), idesc_o = mma_idesc(PT_M, (a.D + 15) / 16 * 16, false, true, FP16);
-          const int k_steps = (a.D + 15) / 16;
-          auto wait = [&](uint64_t *bar, int phase) {
-            if (!dead) dead = !mbar_wait(bar, phase & 1);
-            tmem_fence_after();
-          };
-          auto scores = [&](int t, int at) {
-            const uint64_t q = desc_k_major(q_sm + t * TILE, PT_M, 0), k = desc_k_major(ring + at % STAGES * TILE, PT_N, 0);
+        constexpr bool FP16 = !__is_same(T, bf16);
+        const uint32_t idesc_s = mma_idesc(PT_M, PT_N, false, false, FP16), idesc_o = mma_idesc(PT_M, FULL ? KB * 64 : (a.D + 15) / 16 * 16, false, true, FP16);
+        const int k_steps = FULL ? KB * 4 : (a.D + 15) / 16;
+        const uint64_t q0 = desc_k_major(q_sm, PT_M, 0), k0 = desc_k_major(ring, PT_N, 0), v0 = desc_mn_major(ring, PT_N, 0);
+        auto wait = [&](uint64_t *bar, int phase) {
+          if (!dead && !mbar_try_wait(bar, phase & 1)) dead = !mbar_wait(bar, phase & 1);
+          __syncwarp();
+          tmem_fence_after();
+        };
+        auto scores = [&](int t, int at) {
+          const uint64_t q = q0 + t * (TILE / 16), k = k0 + at % STAGES * (TILE / 16);
 #pragma unroll
-            for (int x = 0; x < KB * 4; ++x) {
-              const uint32_t step = (x / 4) * (PT_N * 128 / 16) + (x % 4) * 2;  // descriptor units of 16 bytes
-              if (x < k_steps) mma_ss(tm + t * PT_N, q + step, k + step, idesc_s, x > 0);
-            }
-            mma_commit(&s_full[t]);
-          };
-          // slots of this item: K0, V0, K1, V1, ...
-          const int first = slot;
-          wait(&full[first % STAGES], first / STAGES);
-          for (int t = 0; t < (both ? 2 : 1); ++t) {
-            wait(&q_full[t], used[t]);
-            ++used[t];
-            scores(t, first);
+          for (int x = 0; x < KB * 4; ++x) {
+            const uint32_t step = (x / 4) * (PT_N * 128 / 16) + (x % 4) * 2;  // descriptor units of 16 bytes
+            if (FULL || x < k_steps) warp_mma_ss(tm + t * PT_N, q + step, k + step, idesc_s, x > 0);
           }
-          mma_commit(&empty[first % STAGES]);
-          for (int j = 0; j < n; ++j) {
-            const int vs = first + 2 * j + 1, ks = vs + 1;
-            wait(&full[vs % STAGES], vs / STAGES);
-            if (j >= d0) {
-              wait(&clean[vs % STAGES], looked >> (vs % STAGES));
-              looked ^= 1u << (vs % STAGES);
-            }
-            bool more = false;
-            for (int t = 0; t < (both ? 2 : 1); ++t) {
-              const int last = d0 + t;
-              if (j > last) continue;
-              wait(&p_full[t], stepped[t]);
-              ++stepped[t];
-              const uint64_t v = desc_mn_major(ring + vs % STAGES * TILE, PT_N, 0);
+          warp_commit(&s_full[t]);
+        };
+        auto values = [&](int t, int at, bool begun) {
+          const uint64_t v = v0 + at % STAGES * (TILE / 16);
 #pragma unroll
-              for (int x = 0; x < PT_N / 16; ++x)
-                mma_ts(tm + 2 * PT_N + t * (KB * 64), tm + t * PT_N + x * 8, v + (uint64_t)(x * 128), idesc_o, j > 0 || x > 0);
-              if (j == last) {
-                mma_commit(&o_full[t]);
-                continue;
-              }
-              if (!more) wait(&full[ks % STAGES], ks / STAGES);
-              more = true;
-              scores(t, ks);
-              if (j + 1 == last) mma_commit(&q_empty[t]);
-            }
-            mma_commit(&empty[vs % STAGES]);
-            if (more) mma_commit(&empty[ks % STAGES]);
+          for (int x = 0; x < PT_N / 16; ++x)
+            warp_mma_ts(tm + 2 * PT_N + t * (KB * 64), tm + t * PT_N + x / 4 * 64 + x % 4 * 8, v + (uint64_t)(x * 128), idesc_o,
+                        x > 0 ? 1u : (uint32_t)begun);
+        };
+        // slots of this item: K0, V0, K1, V1, ... Those of the next step are waited for behind this step's products.
+        const int first = slot;
+        auto arrive = [&](int j) {  // V of step j, K of step j + 1
+          const int vs = first + 2 * j + 1;
+          wait(&full[vs % STAGES], vs / STAGES);
+          if (j >= d0) {
+            wait(&clean[vs % STAGES], looked >> (vs % STAGES));
+            looked ^= 1u << (vs % STAGES);
           }
-          if (d0 == 0) mma_commit(&q_empty[0]);  // (a tile with one key tile)
-          slot += 2 * n;
+          if (j + 1 < n) wait(&full[(vs + 1) % STAGES], (vs + 1) / STAGES);
+        };
+        wait(&full[first % STAGES], first / STAGES);
+        for (int t = 0; t < (both ? 2 : 1); ++t) {
+          wait(&q_full[t], used[t]);
+          ++used[t];
+          scores(t, first);
         }
-        dead = __shfl_sync(0xffffffffu, (int)dead, 0) != 0;
+        warp_commit(&empty[first % STAGES]);
+        arrive(0);
+        for (int j = 0; j < n; ++j) {
+          const int vs = first + 2 * j + 1;
+          if (j <= d0) {
+            wait(&p_full[0], stepped[0]);
+            ++stepped[0];
+            values(0, vs, j > 0);
+            if (j < d0) {
+              scores(0, vs + 1);
+              if (j + 1 == d0) warp_commit(&q_empty[0]);
+            } else {
+              warp_commit(&o_full[0]);
+              if (j == 0) warp_commit(&q_empty[0]);  // (a tile with one key tile)
+            }
+          }
+          if (both) {
+            wait(&p_full[1], stepped[1]);
+            ++stepped[1];
+            values(1, vs, j > 0);
+          }
+          warp_commit(&empty[vs % STAGES]);
+          if (j + 1 < n) {
+            if (both) {
+              scores(1, vs + 1);
+              if (j == d0) warp_commit(&q_empty[1]);
+            }
+            warp_commit(&empty[(vs + 1) % STAGES]);
+            arrive(j + 1);
+          } else if (both) {
+            warp_commit(&o_full[1]);
+          }
+        }
+        slot += 2 * n;
+        dead = __any_sync(0xffffffffu, dead);
       } else {
         const int me = tid - PT_SCAN * WARP, mine = warp - PT_SCAN;
         for (int t = 0; t < 2; ++t) {  // what was found in the item before the last has been read
@@ -386,8 +498,8 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       for (int t = 0; t < 2; ++t)
         if (used[t]) mbar_wait(&q_full[t], (used[t] - 1) & 1);
     }
-    if (warp == PT_ISSUER && lane == 0 && dead) {
-      mma_commit(&drained);
+    if (warp == PT_ISSUER && dead) {
+      warp_commit(&drained);
       mbar_wait(&drained, 0);
     }
   }
@@ -420,7 +532,7 @@ bool packed_tc_supported(int dtype, const PackedArgs &a) {
          rows_fit(a.v, a.ldv, a.hv, a.G) && aligned16(a.out) && (long long)packed_tiles<PT_Q>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
 }
 
-template <typename T, int KB>
+template <typename T, int KB, bool FULL>
 static int launch_packed_tc(const PackedArgs &a, cudaStream_t st) {
   constexpr int STAGES = KB == 1 ? 8 : 4, smem = 1024 + (2 + STAGES) * KB * PT_N * 128;
   constexpr bool FP16 = !__is_same(T, bf16);
@@ -433,11 +545,11 @@ static int launch_packed_tc(const PackedArgs &a, cudaStream_t st) {
   static DevicePrep prep;
   const int(*unused)[4];
   cudaError_t e = prep.get(
-      [&](int(&)[4]) { return cudaFuncSetAttribute(packed_tc_kernel<T, KB, STAGES>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); },
+      [&](int(&)[4]) { return cudaFuncSetAttribute(packed_tc_kernel<T, KB, STAGES, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); },
       unused);
-  const int tiles = packed_tiles<PT_Q>(a.T, a.B), items = tiles * a.H, grid = items < sm_count() ? items : sm_count();
+  const int tiles = packed_tiles<PT_Q>(a.T, a.B), grid = tiles * a.H < sm_count() ? tiles * a.H : sm_count();  // (no fewer than there can be)
   if (e == cudaSuccess)
-    e = djv::launch_kernel(packed_tc_kernel<T, KB, STAGES>, dim3(grid), dim3(PT_THREADS), smem, st, q, k, v, a, tiles);
+    e = djv::launch_kernel(packed_tc_kernel<T, KB, STAGES, FULL>, dim3(grid), dim3(PT_THREADS), smem, st, q, k, v, a, tiles);
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_error("packed_attention: CUDA error %d (%s)", (int)e, cudaGetErrorString(e));
@@ -448,8 +560,12 @@ static int launch_packed_tc(const PackedArgs &a, cudaStream_t st) {
 }
 
 int packed_tc(int dtype, const PackedArgs &a, cudaStream_t st) {
-  if (dtype == DJV_DTYPE_F16) return a.D <= 64 ? launch_packed_tc<__half, 1>(a, st) : launch_packed_tc<__half, 2>(a, st);
-  return a.D <= 64 ? launch_packed_tc<bf16, 1>(a, st) : launch_packed_tc<bf16, 2>(a, st);
+  const auto of = [&](auto t) {
+    using T = decltype(t);
+    if (a.D <= 64) return a.D == 64 ? launch_packed_tc<T, 1, true>(a, st) : launch_packed_tc<T, 1, false>(a, st);
+    return a.D == 128 ? launch_packed_tc<T, 2, true>(a, st) : launch_packed_tc<T, 2, false>(a, st);
+  };
+  return dtype == DJV_DTYPE_F16 ? of(__half()) : of(bf16());
 }
 
 unsigned packed_timeouts() {
