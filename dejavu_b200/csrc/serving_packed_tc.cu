@@ -28,7 +28,7 @@ namespace djv {
 
 constexpr int PT_THREADS = 640, PT_M = 128, PT_N = 128, PT_Q = 2 * PT_M;  // rows of a query tile, of a key tile, of an item
 constexpr int PT_SOFT = 16, PT_LOADER = 16, PT_ISSUER = 17, PT_SCAN = 18;  // softmax warps, and the others
-constexpr int PT_EVERY = 4;     // of so many pairs of weights one is made on the FMA units
+constexpr int PT_EVERY = 6;     // of so many pairs of weights one is made on the FMA units
 constexpr int PT_TABLE = 1024;  // items per head that are put in order
 
 // whether `mine` holds for any of a tile's 256 threads; a barrier of them
@@ -358,11 +358,17 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         }
         if (r < rows) {
+          uint32_t p[8];
 #pragma unroll
-          for (int e = 0; e < 16; e += 8)
-            if (q + e < a.D)
-              *reinterpret_cast<uint4 *>(out + q + e) = make_uint4(pack_pair<T>(f[e], f[e + 1]), pack_pair<T>(f[e + 2], f[e + 3]),
-                                                                   pack_pair<T>(f[e + 4], f[e + 5]), pack_pair<T>(f[e + 6], f[e + 7]));
+          for (int e = 0; e < 8; ++e) p[e] = pack_pair<T>(f[2 * e], f[2 * e + 1]);
+          if (FULL) {  // a sector in one: every lane writes to a line of its own
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + q), "r"(p[0]), "r"(p[1]), "r"(p[2]), "r"(p[3]),
+                         "r"(p[4]), "r"(p[5]), "r"(p[6]), "r"(p[7])
+                         : "memory");
+          } else {
+            if (q < a.D) *reinterpret_cast<uint4 *>(out + q) = make_uint4(p[0], p[1], p[2], p[3]);
+            if (q + 8 < a.D) *reinterpret_cast<uint4 *>(out + q + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+          }
         }
         __syncwarp();
       }
@@ -503,20 +509,30 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             continue;
           }
           uint4 *v = reinterpret_cast<uint4 *>(base + 2 * TILE + vs % STAGES * TILE);
-          bool any = false;
+          // the largest magnitude, two 16-bit numbers at a time: infinities and NaN are above all others
+          uint32_t large[4] = {0, 0, 0, 0};
+#pragma unroll 4
           for (int i = me; i < (int)(TILE / 16); i += 2 * WARP) {
-            uint4 x = v[i];
-            uint32_t *e = reinterpret_cast<uint32_t *>(&x);
-            bool here = false;
+            const uint4 y = v[i];
+            large[0] = __vmaxu2(large[0], y.x & 0x7fff7fffu);
+            large[1] = __vmaxu2(large[1], y.y & 0x7fff7fffu);
+            large[2] = __vmaxu2(large[2], y.z & 0x7fff7fffu);
+            large[3] = __vmaxu2(large[3], y.w & 0x7fff7fffu);
+          }
+          const uint32_t most = __vmaxu2(__vmaxu2(large[0], large[1]), __vmaxu2(large[2], large[3]));
+          bool any = (((most & Exponent<T>::MASK) + Exponent<T>::ONE) & 0x80008000u) != 0;
+          if (any) {
+            for (int i = me; i < (int)(TILE / 16); i += 2 * WARP) {
+              uint4 y = v[i];
+              uint32_t *e = reinterpret_cast<uint32_t *>(&y);
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint32_t top = ((e[y] & Exponent<T>::MASK) + Exponent<T>::ONE) & 0x80008000u;
-              here |= top != 0;
-              if (top & 0x8000u) e[y] &= 0xffff0000u;
-              if (top & 0x80000000u) e[y] &= 0x0000ffffu;
+              for (int z = 0; z < 4; ++z) {
+                const uint32_t top = ((e[z] & Exponent<T>::MASK) + Exponent<T>::ONE) & 0x80008000u;
+                if (top & 0x8000u) e[z] &= 0xffff0000u;
+                if (top & 0x80000000u) e[z] &= 0x0000ffffu;
+              }
+              v[i] = y;
             }
-            if (here) v[i] = x;
-            any |= here;
           }
           any = __any_sync(0xffffffffu, any);
           if (lane == 0) odd[parity][j - d0][mine] = any;
@@ -563,7 +579,7 @@ static bool rows_fit(const void *p, long long ld, long long hs, int heads) {
 }
 bool packed_tc_supported(int dtype, const PackedArgs &a) {
   return dtype != DJV_DTYPE_F32 && a.D % 8 == 0 && a.D <= 128 && rows_fit(a.q, a.ldq, a.hq, a.H) && rows_fit(a.k, a.ldk, a.hk, a.G) &&
-         rows_fit(a.v, a.ldv, a.hv, a.G) && aligned16(a.out) && (long long)packed_tiles<PT_Q>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
+         rows_fit(a.v, a.ldv, a.hv, a.G) && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (long long)packed_tiles<PT_Q>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
 }
 
 template <typename T, int KB, bool FULL>
