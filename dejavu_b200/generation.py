@@ -1,4 +1,4 @@
-"""Greedy generation with a CUDA-graph decode step, with the call surface the reference's benchmarks use:
+"""Generation with a CUDA-graph decode step, greedy or sampled, with the call surface the reference's benchmarks use:
 
     update_graph_cache(model, cache, batch_size, seqlen_og, max_seqlen, tensor_parallel=1)
     model.generate(input_ids=, max_length=, fused_ft_kernel=, cg=, vocab_size=, return_dict_in_generate=,
@@ -219,12 +219,18 @@ class GenerationMixin:
     @torch.inference_mode()
     def generate(self, input_ids, max_length, top_k=1, top_p=0.0, temperature=1.0, fused_ft_kernel=True,
                  cg=False, vocab_size=None, return_dict_in_generate=False, output_scores=False, timing=False,
-                 prompt_chunk=None, **kwargs):
-        """Greedy decoding (top_k=1 is the only sampler the benchmarks use). Returns an object with
+                 prompt_chunk=None, min_p=0.0, generator=None, **kwargs):
+        """Greedy decoding with top_k=1 (what the benchmarks use); else every token is sampled (ops.sample_tokens) at `temperature`
+        among the top_k (0: all) largest logits, of those the ones that make up top_p of the probability (0 or 1: all), of those the ones
+        with at least min_p of the largest one's, with random numbers from `generator` (of the device; None: the default
+        one; ranks of a tensor-parallel group have theirs seeded alike). Returns an object with
         .sequences (B, max_length) and, when asked, .scores (list of (B, vocab) logits per new token).
         prompt_chunk: the prompt runs in portions of at most that many tokens (models that take portions)."""
-        assert top_k == 1, "only greedy decoding is implemented"
+        if top_k < 0 or not 0 <= top_p <= 1 or not 0 <= min_p <= 1 or not temperature >= 0:
+            raise ValueError(f"top_k {top_k}, top_p {top_p}, min_p {min_p}, temperature {temperature}")
         assert prompt_chunk is None or getattr(self, "takes_portions", False), "this model takes a prompt in one piece"
+        from . import ops
+
         B, seqlen_og = input_ids.shape
         device = input_ids.device
         if timing:
@@ -251,7 +257,11 @@ class GenerationMixin:
                 logits = logits[..., :vocab_size]
             if output_scores:
                 scores.append(logits.clone())
-            token = logits.argmax(dim=-1, keepdim=True)
+            if top_k == 1:
+                token = logits.argmax(dim=-1, keepdim=True)
+            else:
+                token = ops.sample_tokens(logits, torch.rand(B, device=device, generator=generator), temperature, top_k, top_p or 1.0,
+                                          min_p)[:, None]
             sequences.append(token)
             if ip.sequence_len_offset >= max_length - 1:
                 break

@@ -661,3 +661,34 @@ def test_serving_operators_refuse_what_does_not_fit(ops):
         with pytest.raises((AssertionError, RuntimeError)):
             call()
             print("taken:", i)
+
+
+# ---- in the generation loop --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cg", [False, True])
+def test_generate_samples(ops, cg):
+    """Every new token is the one that its logits, the settings and the generator's numbers give; top_k=1 stays greedy."""
+    from dejavu_b200.gpt import GPTLMHeadModel, opt_config
+
+    cfg = opt_config("opt-125m", n_layer=2, n_embd=256, hidden_size=256, n_head=4, n_inner=1024, vocab_size=512, max_position_embeddings=64,
+                     mlp_sparse=False, att_sparse=False)
+    model = GPTLMHeadModel(cfg, device="cuda", dtype=F16).eval().init_random(0, std=0.3)
+    ids = torch.randint(0, 512, (3, 7), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    settings = {"top_k": 20, "top_p": 0.9, "min_p": 0.01, "temperature": 1.5}
+    kw = {"max_length": 20, "cg": cg, "vocab_size": 500, "return_dict_in_generate": True, "output_scores": True}
+    out = model.generate(ids, generator=torch.Generator("cuda").manual_seed(5), **settings, **kw)
+    g = torch.Generator("cuda").manual_seed(5)
+    assert out.sequences.shape == (3, 20) and len(out.scores) == 13
+    for i, scores in enumerate(out.scores):
+        u = torch.rand(3, device="cuda", generator=g).tolist()
+        for b in range(3):
+            assert int(out.sequences[b, 7 + i]) == S.sample(scores[b].cpu(), u[b], 1.5, 20, 0.9, 0.01)
+    again = model.generate(ids, generator=torch.Generator("cuda").manual_seed(5), **settings, **kw)
+    assert torch.equal(out.sequences, again.sequences)
+    greedy = model.generate(ids, **kw)
+    assert torch.equal(greedy.sequences[:, 7:], torch.stack([s.argmax(-1) for s in greedy.scores], 1))
+    cold = model.generate(ids, top_k=0, temperature=0.0, **kw)
+    assert torch.equal(cold.sequences, greedy.sequences)
+    for bad in ({"top_k": -1}, {"top_p": 1.5}, {"min_p": -0.1}, {"temperature": -1.0}, {"temperature": math.nan}):
+        with pytest.raises(ValueError):
+            model.generate(ids, **{"top_k": 0, **bad}, **kw)
