@@ -74,8 +74,8 @@ struct SampleShared {
     };
     double mass[SA_BINS];       // (of a block that works alone)
   };
-  unsigned into[SA_BINS];       // of this block's slice: sum of how far into the step entries are, `fine` to a step
-  double table[64];           // 2^(j / 64)
+  unsigned into[SA_BINS], all_into[SA_BINS];  // sum of how far into the step entries are, in parts; of the slice, of the row
+  float2 table[64];           // 2^(j / 64), as the sum of two floats
   double part[SA_WARPS], part2[SA_WARPS], part3[SA_WARPS];
   u64 wide[SA_WARPS];
   float narrow[SA_WARPS];
@@ -106,6 +106,13 @@ __device__ __forceinline__ V block_all(V v, V *slots, F f) {
 __device__ __forceinline__ double block_total(double v, SampleShared &s) {
   return block_all(v, s.part, [](double a, double b) { return a + b; });
 }
+// (Out of line, like other things that are used in several places: a row goes through most of the code once, and fetching that is a
+// large part of its time.)
+__device__ __noinline__ u64 block_most(u64 v, u64 *slots) {
+  return block_all(v, slots, [](u64 a, u64 b) { return a > b ? a : b; });
+}
+__device__ __forceinline__ u64 block_least(u64 v, u64 *slots) { return ~block_most(~v, slots); }
+__device__ __noinline__ double power_of_2(double x) { return exp2(x); }
 
 // f(x, index) for the row's entries from lo to hi (multiples of the chunk, or the row's end), a thread every `step`-th chunk
 template <typename T, bool VEC, typename F>
@@ -188,7 +195,7 @@ __device__ __noinline__ void sort_list(u64 *list, int n) {
 }
 
 // Sum of v over the threads in front of this one; total receives the block's.
-__device__ __forceinline__ double block_before(double v, double *slots, double &total) {
+__device__ __noinline__ double block_before(double v, double *slots, double &total) {
   const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
   double sum = v;
 #pragma unroll
@@ -213,27 +220,55 @@ __device__ __forceinline__ double block_before(double v, double *slots, double &
 // The largest entry of a row and what follows from it.
 struct SampleScale {
   float top, inv;       // largest logit, steps per unit of the logit
+  float fine, inv_fine; // parts of a step, and per unit of the logit
+  int fine_bits;
   double temperature;
   float c_hi, c_lo;     // log2(e) / temperature
   float reach;          // entries further below the largest are dropped
 
   __device__ __forceinline__ bool counts(float x) const { return top - x <= reach || x == top; }
-  // for x that counts: the steps in front of x, a number below SA_BINS
-  __device__ __forceinline__ float step_of(float x) const { return x == top ? 0.f : (top - x) * inv; }
+  // For x that counts: how many parts of a step, `fine` of them to one, are in front of it, rounded, plus 2^23: a number whose lowest bits
+  // are the part and those above the step, and which compares with parts(step).
+  __device__ __forceinline__ float part_of(float x) const { return x == top ? 8388608.f : fmaf(top - x, inv_fine, 8388608.f); }
+  __device__ __forceinline__ float parts(float step) const { return fmaf(step, fine, 8388608.f); }
   __device__ __forceinline__ double exact(float x) const { return x == top ? 1.0 : exp(((double)x - (double)top) / temperature); }
   // For x that counts (for others a number that means nothing): y = (x - top) log2(e) / temperature >= -65 as the sum of two floats,
   // y = k / 64 + f
-  __device__ __forceinline__ double weight(float x, const double *table) const {
+  __device__ __forceinline__ int reduced(float x, float &q) const {  // k, and 2^f - 1
     const float t = x - top, v = t - x, e = (x - (t - v)) - (top + v);  // x - top = t + e
     const float y = fmaxf(t * c_hi, -100.f), rest = fmaf(t, c_hi, -y) + fmaf(t, c_lo, e * c_hi);
     const float k = rintf(y * 64.f);
     const float f = (fmaf(k, -0.015625f, y) + rest) * 0.69314718f;  // (the difference is exact)
-    const float q = fmaf(f * f, fmaf(f, fmaf(f, 0.041666668f, 0.16666667f), 0.5f), f);  // e^f - 1
-    const int n = (int)k;
-    const double w = table[n & 63];
+    q = fmaf(f * f, fmaf(f, fmaf(f, 0.041666668f, 0.16666667f), 0.5f), f);
+    return (int)k;
+  }
+  __device__ __forceinline__ double weight(float x, const float2 *table) const {
+    float q;
+    const int n = reduced(x, q);
+    const double w = (double)table[n & 63].x + (double)table[n & 63].y;
     const double scaled = __longlong_as_double(__double_as_longlong(fma(w, (double)q, w)) + ((long long)(n >> 6) << 52));
     return x == top ? 1.0 : scaled;  // (+inf among them)
   }
+  // the same as the sum of two floats
+  __device__ __forceinline__ float2 weight_pair(float x, const float2 *table) const {
+    float q;
+    const int n = reduced(x, q);
+    const float2 w = table[n & 63];
+    const float scale = __uint_as_float((uint32_t)((n >> 6) + 127) << 23), rest = fmaf(w.x, q, w.y), hi = w.x + rest;
+    return x == top ? make_float2(1.f, 0.f) : make_float2(hi * scale, (rest - (hi - w.x)) * scale);
+  }
+};
+
+// A sum of such pairs, with 40 bits and more: what the larger part loses joins the smaller one. (Additions of 64-bit numbers take
+// ten times as long as one of 32 bits.)
+struct PairSum {
+  float hi = 0.f, lo = 0.f;
+  __device__ __forceinline__ void add(float2 w) {
+    const float s = hi + w.x, back = s - hi;
+    lo += ((hi - (s - back)) + (w.x - back)) + w.y;
+    hi = s;
+  }
+  __device__ __forceinline__ double value() const { return (double)hi + (double)lo; }
 };
 
 // One row by one block, in 64 bits, from global memory: nothing is too close and nothing too much.
@@ -269,8 +304,8 @@ struct SampleAlone {
       __syncthreads();
       const int n = s.listed;
       if (n <= SA_LIST) break;
-      hi = block_all(first, s.wide, [](u64 a, u64 b) { return a > b ? a : b; });
-      lo = block_all(last, s.wide, [](u64 a, u64 b) { return a < b ? a : b; });
+      hi = block_most(first, s.wide);
+      lo = block_least(last, s.wide);
       int shift = 0;
       while (((hi - lo) >> shift) >= SA_BINS) ++shift;
       for (int i = threadIdx.x; i < SA_BINS; i += SA_THREADS) {
@@ -335,7 +370,7 @@ struct SampleAlone {
     return place;
   }
 
-  __device__ int token(int k, double p, double min_p, double u) {
+  __device__ __noinline__ int token(int k, double p, double min_p, double u) {
     u64 cut = 0;
     const u64 most = place_of(order_of(z.top), 0);
     if (k > 0 && k < V) {
@@ -427,7 +462,7 @@ struct SampleAlone {
 
 // The sorted list holds all entries that can be kept, n of them, `behind` is the weight of the others that top-p counts: the token.
 // found[1]: too close to tell. By all of a block.
-__device__ int sample_list(SampleShared &s, const SampleScale &z, int n, double behind, double p, double min_p, double u) {
+__device__ __noinline__ int sample_list(SampleShared &s, const SampleScale &z, int n, double behind, double p, double min_p, double u) {
   const int at = threadIdx.x * SA_EACH;
   double w[SA_EACH], mine = 0, total;
   if (threadIdx.x == 0) s.found[1] = 0;
@@ -473,7 +508,7 @@ __device__ int sample_list(SampleShared &s, const SampleScale &z, int n, double 
     near |= fabs(upto - target) <= SA_CLOSE * total;
     if (upto > target) over = min(over, at + e);
   }
-  over = (int)block_all((u64)over, s.wide, [](u64 a, u64 b) { return a < b ? a : b; });
+  over = (int)block_least((u64)over, s.wide);
   if (near) s.found[1] = 1;
   __syncthreads();
   return (int)~(uint32_t)(s.list[over] >> 32);
@@ -503,17 +538,30 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   SampleShared &first = *cluster.map_shared_rank(&s, 0);
   SampleAlone<T, VEC> r{row, a.V, s, {}};
   SampleScale &z = r.z;
-  // f(x, index) for the warp's entries (a short body: all of it stays in the instruction cache)
-  auto mine = [&](auto f) {
-    for (int i = lo + lane * N; i < hi; i += WARP * N) {
-      if (VEC && i + N <= hi) {
-        float x[N];
-        unpack_chunk<T>(*reinterpret_cast<const uint4 *>(entries + i), x);
-#pragma unroll
-        for (int e = 0; e < N; ++e) f(x[e], i + e);
+  // four entries at a time, whatever their type: short code
+  constexpr int FOUR = VEC ? 4 : 1;
+  auto four = [&](int i, float (&x)[FOUR]) {
+    if (VEC && i + FOUR <= hi) {
+      if (sizeof(T) == 4) {
+        *reinterpret_cast<uint4 *>(x) = *reinterpret_cast<const uint4 *>(entries + i);
       } else {
-        for (int e = i; e < min(hi, i + N); ++e) f(to_f(entries[e]), e);
+        T y[4];
+        *reinterpret_cast<uint2 *>(y) = *reinterpret_cast<const uint2 *>(entries + i);
+#pragma unroll
+        for (int e = 0; e < FOUR; ++e) x[e] = to_f(y[e]);
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < FOUR; ++e) x[e] = i + e < hi ? to_f(entries[i + e]) : -INFINITY;
+    }
+  };
+  // f(x, index) for the warp's entries, and for some of -inf behind its last
+  auto mine = [&](auto f) {
+    for (int i = lo + lane * FOUR; i < hi; i += WARP * FOUR) {
+      float x[FOUR];
+      four(i, x);
+#pragma unroll
+      for (int e = 0; e < FOUR; ++e) f(x[e], i + e);
     }
   };
 
@@ -561,11 +609,15 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
       }
     }
   }
-  if (tid < 64) s.table[tid] = exp2(tid * 0.015625);
+  if (tid < 64) {
+    const double w = power_of_2(tid * 0.015625);
+    const float high = (float)w;
+    s.table[tid] = make_float2(high, (float)(w - (double)high));
+  }
   for (int i = tid; i < SA_BINS; i += SA_THREADS) s.count[i] = s.into[i] = 0;
   if (tid == 0) s.listed = s.own = 0;
   u64 best = top > -INFINITY ? place_of(order_of(top), top_at) : 0;
-  best = block_all(best, s.wide, [](u64 x, u64 y) { return x > y ? x : y; });
+  best = block_most(best, s.wide);
   bottom = block_all(bottom, s.narrow, [](float x, float y) { return fminf(x, y); });
   cluster.barrier_wait(std::move(started));  // (all blocks of the cluster have started)
   if (tid < C) {
@@ -594,6 +646,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   z.reach = (float)fmin(SA_FAR * temperature, 3e38);
   const float range = fminf(z.top - bottom, z.reach);
   z.inv = range > 0.f && range < 3e38f ? SA_BINS / range * 0.99999f : 0.f;
+  z.fine_bits = min(12, __clz(a.V) - 1);  // (the sum of parts over the row stays below 2^31)
+  z.fine = (float)(1 << z.fine_bits);
+  z.inv_fine = z.inv * z.fine;
   bool by_rank = k > 0 && k < a.V;
   const bool by_mass = p < 1;
   u64 cut = 0;
@@ -624,8 +679,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   // Entries of steps from .. to - 1 go to the first block's list.
   auto collect = [&](float from, float to) {
     begin_list();
+    from = z.parts(from);
+    to = z.parts(to);
     mine([&](float x, int i) {
-      const float at = z.step_of(x);
+      const float at = z.part_of(x);
       if (at >= from && at < to && z.counts(x)) own(i);
     });
     send_list();
@@ -638,35 +695,32 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   // of a chunk overlap.)
   auto weigh = [&](float from, float to) {
     begin_list();
-    double x0 = 0, x1 = 0, x2 = 0;
-    for (int i = lo + lane * N; i < hi; i += WARP * N) {
-      float x[N];
-      if (VEC && i + N <= hi) {
-        unpack_chunk<T>(*reinterpret_cast<const uint4 *>(entries + i), x);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = i + e < hi ? to_f(entries[i + e]) : -INFINITY;
-      }
+    from = z.parts(from);  // (infinite ones stay so)
+    to = z.parts(to);
+    const float rank_from = z.parts((float)rank_bin), rank_to = z.parts((float)rank_bin + 1);
+    PairSum front, behind, enough_too;
+    for (int i = lo + lane * FOUR; i < hi; i += WARP * FOUR) {
+      float x[FOUR];
+      four(i, x);
       unsigned between = 0;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const float at = z.step_of(x[e]);
+      for (int e = 0; e < FOUR; ++e) {
+        const float at = z.part_of(x[e]);
         bool keep = z.counts(x[e]);
-        if (rank_bin < SA_BINS) keep = keep && (at < rank_bin || (at < rank_bin + 1 && place_of(order_of(x[e]), i + e) >= cut));
-        const bool mid = keep && at >= from && at < to;
-        double w = z.weight(x[e], s.table);
-        w = keep && !mid ? w : 0.0;
-        x0 += at < from ? w : 0.0;
-        x1 += at < from ? 0.0 : w;
-        if (by_min && at < from && w > 0 && enough(x[e], w)) x2 += w;
-        between |= (unsigned)mid << e;
+        if (rank_bin < SA_BINS) keep = keep && (at < rank_from || (at < rank_to && place_of(order_of(x[e]), i + e) >= cut));
+        const float2 w = z.weight_pair(x[e], s.table);
+        const bool first_ones = keep && at < from, last_ones = keep && at >= to;
+        front.add(first_ones ? w : make_float2(0.f, 0.f));
+        behind.add(last_ones ? w : make_float2(0.f, 0.f));
+        if (by_min && first_ones && enough(x[e], (double)w.x + (double)w.y)) enough_too.add(w);
+        between |= (unsigned)(keep && !first_ones && !last_ones) << e;
       }
       while (between) {
         own(i + __ffs(between) - 1);
         between &= between - 1;
       }
     }
-    if (!by_min) x2 = x0;
+    double x0 = front.value(), x1 = behind.value(), x2 = by_min ? enough_too.value() : x0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       x0 += __shfl_xor_sync(0xffffffffu, x0, o);
@@ -711,39 +765,44 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     else if (tid == 0) a.token[b] = token;
   };
 
+  float weigh_from = INFINITY, weigh_to = INFINITY;  // (without top-p all that top-k keeps)
+  bool all_listed = false;
   if (by_rank || by_mass) {
     // 2. counts of the steps: of the slice, then of the row and running
-    const float fine = (float)(1 << min(12, __clz(a.V) - 1));  // (the sum over the row stays below 2^31)
     mine([&](float x, int) {
       if (!z.counts(x)) return;
-      const float at = z.step_of(x);
-      const int bin = min(SA_BINS - 1, (int)at);
-      atomicAdd(&s.count[bin], 1u);
-      if (by_mass) atomicAdd(&s.into[bin], (unsigned)((at - bin) * fine));
+      const unsigned at = __float_as_uint(z.part_of(x)) & 0x7fffffu;
+      atomicAdd(&s.count[at >> z.fine_bits], 1u);
+      if (by_mass) atomicAdd(&s.into[at >> z.fine_bits], at & ((1u << z.fine_bits) - 1));
     });
     cluster.sync();
-    static_assert(SA_EACH == 4, "16-byte loads of counts");
-    const int at = tid * SA_EACH;
-    unsigned n[SA_EACH] = {}, into[SA_EACH] = {};
+    // a block adds up its share of the steps, for all
+    const int steps = SA_BINS / C, at = tid * SA_EACH;
+    for (int i = tid; i < steps * (by_mass ? 2 : 1); i += SA_THREADS) {
+      const bool second = i >= steps;
+      const int bin = rank * steps + (second ? i - steps : i);
+      unsigned v[SA_CLUSTER], sum = 0;
 #pragma unroll
-    for (int c0 = 0; c0 < SA_CLUSTER; c0 += 4) {
-      uint4 x[4], y[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        x[c] = y[c] = make_uint4(0, 0, 0, 0);
-        if (c0 + c < C) {
-          const SampleShared &other = *cluster.map_shared_rank(&s, c0 + c);
-          x[c] = *reinterpret_cast<const uint4 *>(&other.count[at]);
-          if (by_mass) y[c] = *reinterpret_cast<const uint4 *>(&other.into[at]);
+      for (int c = 0; c < SA_CLUSTER; ++c) {
+        v[c] = 0;
+        if (c < C) {
+          const SampleShared &other = *cluster.map_shared_rank(&s, c);
+          v[c] = second ? other.into[bin] : other.count[bin];
         }
       }
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        n[0] += x[c].x, n[1] += x[c].y, n[2] += x[c].z, n[3] += x[c].w;
-        into[0] += y[c].x, into[1] += y[c].y, into[2] += y[c].z, into[3] += y[c].w;
-      }
+      for (int c = 0; c < SA_CLUSTER; ++c) sum += v[c];
+#pragma unroll
+      for (int c = 0; c < SA_CLUSTER; ++c)
+        if (c < C) {
+          SampleShared &other = *cluster.map_shared_rank(&s, c);
+          (second ? other.all_into : other.upto)[bin] = sum;
+        }
     }
-    auto read = cluster.barrier_arrive();
+    cluster.sync();
+    static_assert(SA_EACH == 4, "16-byte loads of counts");
+    const uint4 n4 = *reinterpret_cast<const uint4 *>(&s.upto[at]);
+    const unsigned n[SA_EACH] = {n4.x, n4.y, n4.z, n4.w};
     double total;
     const unsigned run = (unsigned)block_before(n[0] + n[1] + n[2] + n[3], s.part, total);
     by_rank = by_rank && total > k;
@@ -759,7 +818,6 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     __syncthreads();
     if (by_rank) rank_bin = s.found[2];
     const int rank_upto = by_rank ? (int)s.upto[rank_bin] : 0, rank_before = by_rank && rank_bin ? (int)s.upto[rank_bin - 1] : 0;
-    cluster.barrier_wait(std::move(read));  // (nobody reads counts any more)
     if (by_rank) {
       // 3. top-k
       const bool whole = rank_upto <= SA_LIST;
@@ -781,10 +839,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     }
     if (by_mass) {
       // top-p: bounds of the running sums at the steps' borders. A step's n entries at f_i of it (0 .. 1) weigh E 2^(-c f_i) each, E at its
-      // beginning: together at least E n 2^(-c F), with F the average, and at most E n (1 - F (1 - 2^-c)). What (top - x) * inv is rounded by
-      // is below 2048 * 2^-22 of a step; all in all the bounds are widened by 1e-5.
-      const double width = z.inv > 0.f ? 1.0 / z.inv : 0.0, per = log2_unit * width, full = exp2(-per);
-      double begin = exp2(-per * at);
+      // beginning: together at least E n 2^(-c F), with F the average, and at most E n (1 - F (1 - 2^-c)). For the half a
+      // part that places are rounded by, and 32-bit arithmetic, the bounds are widened.
+      const double width = z.inv > 0.f ? 1.0 / z.inv : 0.0, per = log2_unit * width, full = power_of_2(-per);
+      const double wider = 1 + 1e-5 + per / z.fine, less = fmax(0.0, 2 - wider);
+      double begin = power_of_2(-per * at);
       double low[SA_EACH], high[SA_EACH], low_total, high_total;
 #pragma unroll
       for (int e = 0; e < SA_EACH; ++e) {
@@ -792,12 +851,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
         low[e] = high[e] = 0;
         if (n[e] && bin <= rank_bin) {
           if (bin < rank_bin) {
-            const double f = __fdividef((float)into[e], (float)n[e] * fine);
-            high[e] = begin * n[e] * (1 - f * (1 - full)) * (1 + 1e-5);
-            low[e] = begin * n[e] * exp2f((float)(-per * (f + 1.0 / fine))) * (1 - 1e-5);
+            const double f = __fdividef((float)s.all_into[bin], (float)n[e] * z.fine);
+            high[e] = begin * n[e] * (1 - f * (1 - full)) * wider;
+            low[e] = begin * n[e] * exp2f((float)(-per * (f + 1.0 / z.fine))) * less;
           } else {  // only the first ones of the step
-            high[e] = begin * (k - rank_before) * (1 + 1e-5);
-            low[e] = begin * (k - rank_before) * full * (1 - 1e-5);
+            high[e] = begin * (k - rank_before) * wider;
+            low[e] = begin * (k - rank_before) * full * less;
           }
           if (z.inv == 0.f) low[e] = 0;  // (no steps: equal entries, or a range that floats do not hold)
         }
@@ -814,9 +873,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
         if (can == SA_BINS - 1 && high_run >= p * low_total) can = at + e;
         if (must == SA_BINS - 1 && low_run >= p * high_total) must = at + e;
       }
-      const u64 both = block_all((u64)can << 32 | can, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
-      must = (unsigned)block_all((u64)must, s.wide, [](u64 x, u64 y) { return x < y ? x : y; });
-      can = (unsigned)both;
+      can = (unsigned)block_least(can, s.wide);
+      must = (unsigned)block_least(must, s.wide);
       int most = (int)s.upto[must], least = can ? (int)s.upto[can - 1] : 0;
       if (by_rank) {
         most = min(most, k);
@@ -827,16 +885,24 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
         if (rank == 0) alone();
         return;
       }
-      weigh(whole ? 0.f : (float)can, (float)must + 1.f);
-      cluster.sync();
-      if (whole) {
-        if (rank == 0) {
-          double behind = 0;
-          for (int c = 0; c < C; ++c) behind += s.sums[c][1];
-          finish(SA_LIST, behind);
-        }
-        return;
+      all_listed = whole;
+      weigh_from = whole ? 0.f : (float)can;
+      weigh_to = (float)must + 1.f;
+    }
+  }
+  weigh(weigh_from, weigh_to);
+  if (by_mass) {
+    cluster.sync();
+    if (all_listed) {
+      if (rank == 0) {
+        double behind = 0;
+        for (int c = 0; c < C; ++c) behind += s.sums[c][1];
+        finish(SA_LIST, behind);
       }
+      return;
+    }
+    {
+        const int at = tid * SA_EACH;
       u64 place = cut;
       bool close = false;
       if (rank == 0 && s.listed > 0) {
@@ -883,7 +949,6 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
       __syncthreads();
     }
   }
-  if (!by_mass) weigh(INFINITY, INFINITY);
 
   // 4. the sums of what is kept, in index order
   __syncthreads();
@@ -919,15 +984,17 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   else if (tid == 0) a.token[b] = token;
 }
 
-// Blocks of a row: as many as keep the device busy with B rows, more where a slice would leave room for one block per multiprocessor.
+// Blocks of a row: as many as are resident at once with B rows, two to a multiprocessor; slices that are small enough stay in shared memory,
+// others are read from L2 in every sweep. (256 rows of 50272 entries: 91 us with four blocks per row, in four waves.)
 template <typename T>
 static cudaError_t launch_sample(const SampleArgs &a, int B, bool vec, cudaStream_t st) {
   constexpr int N = Chunk<T>::N, fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16, most = 200 * 1024;
-  int C = 1;
-  while (C < SA_CLUSTER && ((long long)B * C * 2 <= 2 * sm_count() || (long long)(a.V + C - 1) / C * sizeof(T) > 64 * 1024)) C *= 2;
-  while (C > 1 && a.V / C < 512) C /= 2;
+  int C = SA_CLUSTER;
+  // (not so few that a slice finds no room beside another one)
+  while (C > 1 && (a.V / C < 512 || ((long long)B * C > 2 * sm_count() && (long long)(a.V / C) * 2 * sizeof(T) <= 112 * 1024 - fixed))) C /= 2;
   const int slice = ceil_div(ceil_div(a.V, C), N) * N;
-  const bool stored = (long long)slice * sizeof(T) <= most - fixed;
+  const int room = (B * C <= sm_count() ? most : 112 * 1024) - fixed;
+  const bool stored = (long long)slice * sizeof(T) <= room;
   const int smem = fixed + (stored ? slice * (int)sizeof(T) : 0);
   static DevicePrep prep;
   const int(*unused)[4];
