@@ -749,14 +749,17 @@ struct DecodePlan {
   size_t scratch;
   bool split;
 };
-constexpr int DE_LEAST = 4;  // units of a block, where items are split
+// Units of an item up to which it is not split (256 tokens that one block reads take no longer than a second kernel does: 137 tokens of 12
+// heads 10 us whole, 14 split), and units that a block gets at least where items are split (2000 tokens of 8 heads, cold: 16 us
+// with two of them tokens, 18 with three, 21 with five).
+constexpr int DE_WHOLE = DECODE_ITEM + 3, DE_LEAST = DECODE_ITEM + 2;
 template <typename T, int DP>
 static DecodePlan decode_plan(int B, int H, int G, int page, int width) {
   constexpr int ROWS = DecodeRows<T>::N;
   DecodePlan p;
   p.groups = ceil_div(H / G, ROWS);
   const long long items = (long long)B * G * p.groups, most = units_of((long long)width * page);  // units of an item
-  p.split = most > DE_LEAST;
+  p.split = most > DE_WHOLE;
   p.least = DE_LEAST;
   const long long resident = (long long)sm_count() * DecodeRing<T, DP>::BLOCKS, needed = (items * most + DE_LEAST - 1) / DE_LEAST;
   p.blocks = (int)(p.split ? (needed < resident ? needed : resident) : items);

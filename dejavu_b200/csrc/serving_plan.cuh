@@ -53,14 +53,14 @@ DJV_HOST_DEVICE int sequence_of(const int *cu, int B, int t) {
 }
 
 // How the cached tokens of a batch are dealt out to blocks: sequence b of n tokens is `share` items (key/value heads times groups of
-// query heads), each of units_of(n) units: one for its beginning and end, which take about as long as 64 tokens do, and one for every
-// DECODE_UNIT tokens. All units stand in a row, sequence by sequence and item by item, and every block takes `per` of them, so that
-// an item may begin in one block and end in another.
-constexpr int DECODE_UNIT = 64;
-DJV_HOST_DEVICE long long units_of(long long tokens) { return tokens <= 0 ? 1 : (tokens + DECODE_UNIT - 1) / DECODE_UNIT + 1; }
+// query heads), each of units_of(n) units: DECODE_ITEM for its beginning and end, which take about as long as so many times DECODE_UNIT
+// tokens do, and one for every DECODE_UNIT tokens. All units stand in a row, sequence by sequence and item by item, and every block
+// takes `per` of them, so that an item may begin in one block and end in another.
+constexpr int DECODE_UNIT = 64, DECODE_ITEM = 2;
+DJV_HOST_DEVICE long long units_of(long long tokens) { return (tokens <= 0 ? 0 : (tokens + DECODE_UNIT - 1) / DECODE_UNIT) + DECODE_ITEM; }
 // Tokens of an item in front of its unit u.
 DJV_HOST_DEVICE long long tokens_before(long long u, long long tokens) {
-  const long long t = u <= 1 ? 0 : (u - 1) * DECODE_UNIT;
+  const long long t = u <= DECODE_ITEM ? 0 : (u - DECODE_ITEM) * DECODE_UNIT;
   return t < tokens ? t : (tokens < 0 ? 0 : tokens);
 }
 DJV_HOST_DEVICE long long units_per_block(long long units, int blocks, int least) {

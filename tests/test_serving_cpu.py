@@ -198,10 +198,10 @@ def test_units_of_a_batch_are_dealt_out_once(tmp_path):
           for (int b = 0; b < 4; ++b) {
             base[b] = total;
             const long long u = units_of(tokens[b]);
-            CHECK(u >= 1 && tokens_before(0, tokens[b]) == 0 && tokens_before(1, tokens[b]) == 0 && tokens_before(u, tokens[b]) == tokens[b])
+            CHECK(u >= 1 && tokens_before(0, tokens[b]) == 0 && tokens_before(DECODE_ITEM, tokens[b]) == 0 && tokens_before(u, tokens[b]) == tokens[b])
             for (long long i = 0; i < u; ++i) {
               const long long n = tokens_before(i + 1, tokens[b]) - tokens_before(i, tokens[b]);
-              CHECK(n >= (i > 0) && n <= (i > 0 ? DECODE_UNIT : 0))
+              CHECK(n >= (i >= DECODE_ITEM) && n <= (i >= DECODE_ITEM ? DECODE_UNIT : 0))
             }
             total += units_of(tokens[b]) * share;
           }
