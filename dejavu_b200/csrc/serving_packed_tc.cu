@@ -2,17 +2,15 @@
 //
 // Persistent blocks, one per multiprocessor, walk items of 256 queries of one head: two tiles of 128 that share the key and value
 // tiles they pass, so that one tile's softmax runs while the tensor cores work for the other. Roles:
-//   warps 0-7, 8-15 softmax and results of a query tile each, two threads per row, 64 keys each: S (TMEM, fp32) -> weights in the inputs'
-//                   type, over S
-//   warp 16         one thread loads: Q tiles, and K and V tiles of 128 keys into a ring, by TMA
-//   warp 17         one thread issues the products: S = Q K^T, O (TMEM) += P V
-//   warps 18, 19    look through the value tiles that hold keys some row does not see (the last one or two of an item)
+//   warps 0-3, 4-7  softmax and results of a query tile each, a thread per row: S (TMEM, fp32) -> weights in the inputs' type, over S
+//   warp 8          one thread loads: Q tiles, and K and V tiles of 128 keys into a ring, by TMA
+//   warp 9          issues the products: S = Q K^T, O (TMEM) += P V
+//   warps 10, 11    look through the value tiles that hold keys some row does not see (the last one or two of an item)
 // With one score tile per query tile in TMEM (S 2 x 128 + O 2 x 128 columns are all there is) a tile's steps are a chain: QK, softmax, PV;
 // the two tiles' chains interleave.
 //
 // O is only rescaled when a row's maximum grows by more than 2^8 (the division by the sum makes up for the rest), by the softmax
-// threads themselves: the barrier that says S is there also says that the product before it is complete. Whether any row of a tile has
-// grown is a barrier with a vote; only then do a row's two threads tell one another their maxima.
+// threads themselves: the barrier that says S is there also says that the product before it is complete.
 //
 // Items go out in the order of falling work, back and forth over the blocks; sequences may have any lengths.
 //
@@ -26,26 +24,10 @@
 
 namespace djv {
 
-constexpr int PT_THREADS = 640, PT_M = 128, PT_N = 128, PT_Q = 2 * PT_M;  // rows of a query tile, of a key tile, of an item
-constexpr int PT_SOFT = 16, PT_LOADER = 16, PT_ISSUER = 17, PT_SCAN = 18;  // softmax warps, and the others
-constexpr int PT_EVERY = 6;     // of so many pairs of weights one is made on the FMA units
+constexpr int PT_THREADS = 384, PT_M = 128, PT_N = 128, PT_Q = 2 * PT_M;  // rows of a query tile, of a key tile, of an item
+constexpr int PT_SOFT = 8, PT_LOADER = 8, PT_ISSUER = 9, PT_SCAN = 10;  // softmax warps, and the others
 constexpr int PT_TABLE = 1024;  // items per head that are put in order
 
-// whether `mine` holds for any of a tile's 256 threads; a barrier of them
-__device__ __forceinline__ bool any_of_tile(int t, bool mine) {
-  int any;
-  asm volatile(
-      "{\n"
-      ".reg .pred p, q;\n"
-      "setp.ne.s32 p, %2, 0;\n"
-      "barrier.cta.red.or.pred q, %1, 256, p;\n"
-      "selp.s32 %0, 1, 0, q;\n"
-      "}\n"
-      : "=r"(any)
-      : "r"(t + 1), "r"((int)mine)
-      : "memory");
-  return any != 0;
-}
 // Products and commits by one thread of a warp that runs as one: what they are given stays in uniform registers (from one thread's own
 // branch every operand of every product would have to be moved there, 60 to 130 cycles for each).
 __device__ __forceinline__ void warp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -78,26 +60,6 @@ __device__ __forceinline__ void warp_commit(uint64_t *bar) {
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
       "}\n" ::"r"(smem_u32(bar))
       : "memory");
-}
-__device__ __forceinline__ void tile_sync(int t) { asm volatile("barrier.cta.sync %0, 256;" ::"r"(t + 1) : "memory"); }
-// 2^x for a pair of x <= 100 or so, on the FMA units (the special units are what the softmax waits for): x = n + f, |f| <= 1/2, 2^f by the
-// polynomial of degree 5 with the least relative error (fitted by weighted least squares, 2.3e-7 in 32 bits), times 2^n from its bits. Far
-// below it is 0 exactly; NaN stays NaN.
-__device__ __forceinline__ void exp2_fma(float &x, float &y) {
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x));  // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y));
-  const auto both = [](float c) { return pack2(c, c); };
-  const uint64_t v = pack2(x, y), t = add2(v, both(12582912.f)), f = sub2(v, sub2(t, both(12582912.f)));
-  uint64_t p = fma2(both(1.3276471e-3f), f, both(9.6755419e-3f));
-  p = fma2(p, f, both(5.5507131e-2f));
-  p = fma2(p, f, both(2.4022120e-1f));
-  p = fma2(p, f, both(6.9314694e-1f));
-  p = fma2(p, f, both(1.0000001f));
-  float a, b, n, m;
-  unpack2(p, a, b);
-  unpack2(t, n, m);
-  x = a * __uint_as_float((__float_as_uint(n) << 23) + 0x3f800000u);
-  y = b * __uint_as_float((__float_as_uint(m) << 23) + 0x3f800000u);
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -143,9 +105,8 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const __grid_constant__ CUtensorMap map_v, PackedArgs a, int most) {
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t q_full[2], q_empty[2], full[STAGES], empty[STAGES], s_full[2], p_full[2], o_full[2],
-      clean[STAGES], taken[2][2], turn[2], drained;
+      clean[STAGES], taken[2][2], drained;
   __shared__ uint32_t tmem_slot;
-  __shared__ float exch[2][2][PT_M];  // maxima, and in the end sums, of the two halves of a row
   __shared__ int2 table[PT_TABLE];    // sequence and item in it, by falling work
   __shared__ int odd[2][2][2];  // by the item's parity: what each of the two warps found in each of the two value tiles
   constexpr uint32_t TILE = KB * PT_N * 128;
@@ -157,11 +118,10 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 2 * PT_M);
+      mbar_init(&p_full[t], PT_M);
       mbar_init(&o_full[t], 1);
-      mbar_init(&turn[t], 8);
-      mbar_init(&taken[0][t], 8);
-      mbar_init(&taken[1][t], 8);
+      mbar_init(&taken[0][t], 4);
+      mbar_init(&taken[1][t], 4);
     }
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full[s], 1);
@@ -210,11 +170,11 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   bool dead = false;  // a wait ran out: wait no more, finish and report
 
   if (warp < PT_SOFT) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    const int t = warp / 8, half = warp / 4 % 2, r = tid % PT_M;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp / 4, r = tid % PT_M;
     const uint32_t lane_base = (uint32_t)(warp % 4 * 32) << 16;
-    // the thread's scores, over which it puts its weights, and its half of the columns of O
-    const uint32_t tm_s = tm + t * PT_N + half * 64 + lane_base, tm_o = tm + 2 * PT_N + t * (KB * 64) + lane_base;
+    // the row's scores, over which it puts its weights, and its sums
+    const uint32_t tm_s = tm + t * PT_N + lane_base, tm_o = tm + 2 * PT_N + t * (KB * 64) + lane_base;
     const float c = a.scale * 1.4426950408889634f, ca = c == 0.f ? 1e-30f : fabsf(c);  // scores in units of log 2
     const uint64_t ca2 = pack2(ca, ca);
     if (!a.keep_rest) {  // rows of no sequence
@@ -224,7 +184,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int d = tid; d < pieces; d += PT_SOFT * WARP) row[d] = make_uint4(0, 0, 0, 0);
       }
     }
-    int steps = 0, done = 0, turns = 0;  // phases of s_full, o_full and turn
+    int steps = 0, done = 0;  // phases of s_full and o_full
     int parity = 0;
     for (int round = 0; round < rounds; ++round) {
       const int item = item_of(round);
@@ -239,42 +199,41 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (!dead) dead = !mbar_wait(&s_full[t], steps & 1);
         __syncwarp();
         tmem_fence_after();
-        uint32_t s[2][32];
+        uint32_t s[4][32];
         tmem_ld32(s[0], tm_s);
         tmem_ld32(s[1], tm_s + 32);
+        tmem_ld32(s[2], tm_s + 64);
+        tmem_ld32(s[3], tm_s + 96);
         tmem_wait_ld();
         if (c < 0.f) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
+          for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[q][e] ^= 0x80000000u;
         }
         if (j == last) {  // keys behind the row's own
 #pragma unroll
-          for (int q = 0; q < 2; ++q)
+          for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (half * 64 + q * 32 + e > r) s[q][e] = 0xff800000u;
+              if (q * 32 + e > r) s[q][e] = 0xff800000u;
         }
         float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) mm[e / 2 % 4] = max3(mm[e / 2 % 4], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
-        float mx = fmaxf(max3(mm[0], mm[1], mm[2]), mm[3]) * ca;
-        if (any_of_tile(t, j == 0 || mx > m + 8.f)) {
-          exch[t][half][r] = mx;
-          tile_sync(t);
-          mx = fmaxf(mx, exch[t][half ^ 1][r]);
-          if (j == 0) {
-            m = mx == -INFINITY ? 0.f : mx;
-          } else {
-            const bool grow = mx > m + 8.f;
+        const float mx = fmaxf(max3(mm[0], mm[1], mm[2]), mm[3]) * ca;
+        if (j == 0) {
+          m = mx == -INFINITY ? 0.f : mx;
+        } else {
+          const bool grow = mx > m + 8.f;
+          if (__any_sync(0xffffffffu, grow)) {
             const float corr = grow ? exp2_approx(m - mx) : 1.f;
             if (grow) m = mx;
             l *= corr;
 #pragma unroll 1
-            for (int q = half * 16; q < KB * 64; q += 32) {
+            for (int q = 0; q < KB * 64; q += 16) {
               uint32_t o[16];
               tmem_ld16(o, tm_o + q);
               tmem_wait_ld();
@@ -283,37 +242,23 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               tmem_st16(tm_o + q, o);
             }
           }
-          tile_sync(t);  // (before the next maxima are written)
-        }
-        // The two tiles take turns with their exponentials, 0, 1, 0, 1, ... while both have keys left: at the same time they would both be
-        // slow and then both wait for the products.
-        const bool turned = w.rows > PT_M && j <= w.q0 / PT_N;
-        if (turned) {
-          if ((t == 1 || turns > 0) && !dead) dead = !mbar_wait(&turn[t ^ 1], (t == 1 ? turns : turns - 1) & 1);
-          ++turns;
-          __syncwarp();
         }
         const uint64_t nm2 = pack2(-m, -m);
         uint64_t l2[2] = {0, 0};
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < 4; ++q) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x, y;
             unpack2(fma2(pack2(__uint_as_float(s[q][2 * e]), __uint_as_float(s[q][2 * e + 1])), ca2, nm2), x, y);
-            if (e % PT_EVERY == PT_EVERY - 1) {
-              exp2_fma(x, y);
-            } else {
-              x = exp2_approx(x);
-              y = exp2_approx(y);
-            }
+            x = exp2_approx(x);
+            y = exp2_approx(y);
             l2[e % 2] = add2(l2[e % 2], pack2(x, y));
             p[e] = pack_pair<T>(x, y);
           }
           tmem_st16(tm_s + q * 16, p);
         }
-        if (turned && lane == 0) mbar_arrive(&turn[t]);
         float x, y;
         unpack2(add2(l2[0], l2[1]), x, y);
         l += x + y;
@@ -321,10 +266,6 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         tmem_fence_before();
         mbar_arrive(&p_full[t]);
       }
-      exch[t][half][r] = l;
-      tile_sync(t);
-      l += exch[t][half ^ 1][r];
-      tile_sync(t);
       if (!dead) dead = !mbar_wait(&o_full[t], done & 1);
       ++done;
       __syncwarp();
@@ -335,7 +276,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (lane == 0) mbar_arrive(&taken[parity][t]);
       T *out = static_cast<T *>(a.out) + ((long long)(w.first + w.q0 + t * PT_M + r) * a.H + h) * a.D;
 #pragma unroll 1
-      for (int q = half * 16; q < a.D; q += 32) {
+      for (int q = 0; q < a.D; q += 16) {
         uint32_t o[16];
         tmem_ld16(o, tm_o + q);
         tmem_wait_ld();
@@ -375,7 +316,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_fence_before();  // (the next item's first product into O waits for this thread's next weights)
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     int slot = 0;              // ring slots passed so far; slot n is stage n % STAGES in its n / STAGES-th use
     int used[2] = {0, 0};      // items that used query tile 0, 1
     unsigned looked = 0;       // phases of clean, a bit each
@@ -437,7 +378,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const uint64_t v = v0 + at % STAGES * (TILE / 16);
 #pragma unroll
           for (int x = 0; x < PT_N / 16; ++x)
-            warp_mma_ts(tm + 2 * PT_N + t * (KB * 64), tm + t * PT_N + x / 4 * 64 + x % 4 * 8, v + (uint64_t)(x * 128), idesc_o,
+            warp_mma_ts(tm + 2 * PT_N + t * (KB * 64), tm + t * PT_N + x * 8, v + (uint64_t)(x * 128), idesc_o,
                         x > 0 ? 1u : (uint32_t)begun);
         };
         // slots of this item: K0, V0, K1, V1, ... Those of the next step are waited for behind this step's products.
