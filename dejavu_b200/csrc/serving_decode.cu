@@ -327,12 +327,13 @@ struct DecodeSums<float, DP> {
   __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c, int D) {
     const int lane = threadIdx.x % WARP, token = lane % TOKENS, part = lane / TOKENS;
     float s[4] = {};
-    for (int ch = part; ch * 4 < D; ch += PARTS) {
+#pragma unroll 4
+    for (int i = 0; i < DP / 4 / PARTS; ++i) {
+      const int ch = i * PARTS + part;
       const float4 k = at(k_sm + tile_offset<TOKENS>(token, ch));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        if (r >= rows) break;
-        const float4 q = __ldg(reinterpret_cast<const float4 *>(query + r * hq + ch * 4));
+        const float4 q = r < rows && ch * 4 < D ? __ldg(reinterpret_cast<const float4 *>(query + r * hq + ch * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
         s[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[r]))));
       }
     }
