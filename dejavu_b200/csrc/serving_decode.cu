@@ -13,6 +13,10 @@
 // looked up a tile ahead. fp16 and bf16 go through mma.sync, 16 query heads x 16 tokens: tcgen05 would have to pad the heads to
 // 64 or 128 rows, and the tensor work is a small part of the time either way. The weights enter the second product as two terms
 // of the cache's type, hi + lo, so that they keep 16 (bf16) or 22 bits. fp32 goes through the CUDA cores, 4 heads at a time.
+//
+// Measured (bf16, pages of 16, 32 query heads over 8 of 128 dimensions): one cache of 131071 tokens 94 us, 5.7 TB/s; 64 of up to 8192 tokens 168 us,
+// 6.0 TB/s; 16 of 32 heads, fp16, up to 2048 tokens 49 us, 5.2 TB/s (101 before an item's beginning and end counted as units); 137
+// tokens of 12 heads of 64 5.4 us in a graph.
 #include <math.h>
 #include <type_traits>
 

@@ -28,24 +28,23 @@ struct PackedTile {
 template <int Q>
 inline int packed_tiles(int T, int B) { return T / Q + B + 2 < T + 2 ? T / Q + B + 2 : T + 2; }
 
-// Tiles of Q rows that the sequences make. Whole warp.
+// Tiles of Q rows that sequences from .. to - 1 make. Whole warp.
 template <int Q>
-__device__ __forceinline__ int packed_total(const PackedArgs &a) {
+__device__ __forceinline__ int packed_total(const PackedArgs &a, int from, int to) {
   int t = 0;
-  for (int b = threadIdx.x % WARP; b < a.B; b += WARP) {
+  for (int b = from + (int)(threadIdx.x % WARP); b < to; b += WARP) {
     const int lo = max(0, min(a.cu[b], a.T));
     t += (max(0, min(a.cu[b + 1], a.T) - lo) + Q - 1) / Q;
   }
   return __reduce_add_sync(0xffffffffu, t);
 }
 
-// Tile number `index`: tiles of the sequences in order, then of the rows in front of the first and behind the last. Whole warp. Whatever
-// cu holds, rows are within 0 .. T - 1.
+// Tile number `index`: tiles of the sequences in order, then of the rows in front of the first and behind the last. from, seen: a sequence
+// that the tile is not in front of, and the tiles before that. Whole warp. Whatever cu holds, rows are within 0 .. T - 1.
 template <int Q>
-__device__ __forceinline__ PackedTile packed_tile(const PackedArgs &a, int index) {
+__device__ __forceinline__ PackedTile packed_tile(const PackedArgs &a, int index, int from = 0, int seen = 0) {
   const int lane = threadIdx.x % WARP;
-  int seen = 0;
-  for (int b0 = 0; b0 < a.B; b0 += WARP) {
+  for (int b0 = from; b0 < a.B; b0 += WARP) {
     const int b = b0 + lane;
     int lo = 0, n = 0;
     if (b < a.B) {

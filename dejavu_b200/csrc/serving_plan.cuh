@@ -40,17 +40,20 @@ DJV_HOST_DEVICE long long page_of(const PageMap &m, long long t, int &slot) {
   return entry >= 0 && entry < m.pages ? entry : NO_PAGE;
 }
 
-// The sequence that row t of a packed batch belongs to (the last b with cu[b] <= t, if t < cu[b + 1]), or -1.
-DJV_HOST_DEVICE int sequence_of(const int *cu, int B, int t) {
-  int lo = 0, hi = B;  // cu[lo] <= t < cu[hi], if there is such a pair
-  if (t < cu[0] || t >= cu[B]) return -1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
+// The sequence that row t of a packed batch belongs to, the last b with cu[b] <= t: a search with 32 probes at a time. `lo` is the answer
+// when hi - lo is 1, and always a sequence of the batch, whatever the offsets are.
+struct SequenceSearch {
+  int lo, hi;
+  DJV_HOST_DEVICE bool done() const { return hi - lo <= 1; }
+  DJV_HOST_DEVICE int step() const { return (hi - lo + 31) / 32; }
+  DJV_HOST_DEVICE int probe(int lane) const { return lo + (lane + 1) * step(); }  // looked at if below hi
+  // before: how many lanes there are up to the last one whose probe is not after t
+  DJV_HOST_DEVICE void narrow(int before) {
+    const int s = step();
+    lo += before * s;
+    hi = hi < lo + s ? hi : lo + s;
   }
-  return lo;
-}
+};
 
 // How the cached tokens of a batch are dealt out to blocks: sequence b of n tokens is `share` items (key/value heads times groups of
 // query heads), each of units_of(n) units: DECODE_ITEM for its beginning and end, which take about as long as so many times DECODE_UNIT

@@ -17,7 +17,9 @@
 // Weights: 2^(y/64) from a table of 64-bit numbers, 2^f for the rest |f| <= 1/128 by its series in 32 bits, off by 1e-9 at most; sums have 64
 // bits. (32-bit weights would leave every tenth row of a flat distribution undecided.)
 //
-// Bound by latency: a row is read once, then swept four times in shared memory between block and cluster barriers.
+// A row is read once, then swept two or three times in shared memory between block and cluster barriers. One row of 50272 entries (top-k 50,
+// top-p): 15 us, a chain of barriers and fetched code; 256 rows of settings of their own: 90 us, 32 rows of 151936 (top-p 0.9): 65 us, the
+// instructions of the weights and their sums, 45 per entry (64-bit sums: 92 and 73).
 #include <math.h>
 #include <string.h>
 

@@ -692,3 +692,26 @@ def test_generate_samples(ops, cg):
     for bad in ({"top_k": -1}, {"top_p": 1.5}, {"min_p": -0.1}, {"temperature": -1.0}, {"temperature": math.nan}):
         with pytest.raises(ValueError):
             model.generate(ids, **{"top_k": 0, **bad}, **kw)
+
+
+def test_thousands_of_short_prompts(ops):
+    """More sequences and more items than are put in order or searched in one go."""
+    g = torch.Generator().manual_seed(3)
+    lengths = torch.randint(0, 12, (5000,), generator=g).tolist()
+    lengths[4000], lengths[77] = 700, 300
+    T, H, G, D = sum(lengths), 16, 2, 64  # (some 500 items per block)
+    q, k, v = rnd(1, T, H, D, dtype=BF16), rnd(2, T, G, D, dtype=BF16), rnd(3, T, G, D, dtype=BF16)
+    got = ops.packed_attention(q, k, v, cumulative(lengths), 0.125)
+    cu = cumulative(lengths).tolist()
+    for b in [0, 1, 2, 76, 77, 78, 3999, 4000, 4001, 4998, 4999] + torch.randint(0, 5000, (40,), generator=g).tolist():
+        rows = slice(cu[b], cu[b + 1])
+        one = ops.packed_attention(q[rows], k[rows], v[rows], cumulative([lengths[b]]), 0.125)
+        assert torch.equal(got[rows], one), b
+    k_pages, v_pages, table = pool(lengths, 8, G, D, BF16)
+    pos = torch.zeros(5000, dtype=torch.int64, device="cuda")
+    ops.paged_append(None, k, v, k_pages, v_pages, table, pos, cu_seqlens=cumulative(lengths))
+    want = torch.full_like(k_pages, math.nan)
+    b = torch.repeat_interleave(torch.arange(5000, device="cuda"), torch.tensor(lengths, device="cuda"))
+    at = torch.arange(T, device="cuda") - cumulative(lengths)[:-1].long()[b]
+    want[table[b, at // 8].long(), :, at % 8] = k
+    assert torch.equal(k_pages.nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
