@@ -80,7 +80,8 @@ struct SampleShared {
   float2 table[64];           // 2^(j / 64), as the sum of two floats
   double part[SA_WARPS], part2[SA_WARPS], part3[SA_WARPS];
   u64 wide[SA_WARPS];
-  float narrow[SA_WARPS];
+  float narrow[SA_WARPS], narrow2[SA_WARPS];
+  unsigned counts[SA_WARPS];
   // written by the blocks of the cluster
   u64 best[SA_CLUSTER];
   float least[SA_CLUSTER];
@@ -197,26 +198,27 @@ __device__ __noinline__ void sort_list(u64 *list, int n) {
 }
 
 // Sum of v over the threads in front of this one; total receives the block's.
-__device__ __noinline__ double block_before(double v, double *slots, double &total) {
+template <typename V>
+__device__ __noinline__ V block_before(V v, V *slots, V &total) {
   const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
-  double sum = v;
+  V sum = v;
 #pragma unroll
   for (int o = 1; o < WARP; o <<= 1) {
-    const double up = __shfl_up_sync(0xffffffffu, sum, o);
+    const V up = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += up;
   }
   __syncthreads();
   if (lane == WARP - 1) slots[warp] = sum;
   __syncthreads();
-  double run = slots[lane % SA_WARPS];
+  V run = slots[lane % SA_WARPS];
 #pragma unroll
   for (int o = 1; o < SA_WARPS; o <<= 1) {
-    const double up = __shfl_up_sync(0xffffffffu, run, o, SA_WARPS);
+    const V up = __shfl_up_sync(0xffffffffu, run, o, SA_WARPS);
     if (lane % SA_WARPS >= o) run += up;
   }
   total = __shfl_sync(0xffffffffu, run, SA_WARPS - 1);
-  const double front = __shfl_sync(0xffffffffu, run, warp ? warp - 1 : 0);
-  return (warp ? front : 0.0) + (sum - v);
+  const V front = __shfl_sync(0xffffffffu, run, warp ? warp - 1 : 0);
+  return (warp ? front : V(0)) + (sum - v);
 }
 
 // The largest entry of a row and what follows from it.
@@ -805,9 +807,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     static_assert(SA_EACH == 4, "16-byte loads of counts");
     const uint4 n4 = *reinterpret_cast<const uint4 *>(&s.upto[at]);
     const unsigned n[SA_EACH] = {n4.x, n4.y, n4.z, n4.w};
-    double total;
-    const unsigned run = (unsigned)block_before(n[0] + n[1] + n[2] + n[3], s.part, total);
-    by_rank = by_rank && total > k;
+    unsigned total;
+    const unsigned run = block_before(n[0] + n[1] + n[2] + n[3], s.counts, total);
+    by_rank = by_rank && total > (unsigned)k;
     {
       unsigned upto = run;
 #pragma unroll
@@ -842,38 +844,38 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     if (by_mass) {
       // top-p: bounds of the running sums at the steps' borders. A step's n entries at f_i of it (0 .. 1) weigh E 2^(-c f_i) each, E at its
       // beginning: together at least E n 2^(-c F), with F the average, and at most E n (1 - F (1 - 2^-c)). For the half a
-      // part that places are rounded by, and 32-bit arithmetic, the bounds are widened.
-      const double width = z.inv > 0.f ? 1.0 / z.inv : 0.0, per = log2_unit * width, full = power_of_2(-per);
-      const double wider = 1 + 1e-5 + per / z.fine, less = fmax(0.0, 2 - wider);
-      double begin = power_of_2(-per * at);
-      double low[SA_EACH], high[SA_EACH], low_total, high_total;
+      // part that places are rounded by, and 32-bit arithmetic here (sums of 2048 numbers, 2^-18 at most), the bounds are widened.
+      const double per_step = z.inv > 0.f ? log2_unit / z.inv : 0.0;
+      const float per = (float)per_step, full = exp2f(-per), wider = 1.f + 1e-5f + per / z.fine, less = fmaxf(0.f, 2.f - wider);
+      float low[SA_EACH], high[SA_EACH], low_total, high_total;
 #pragma unroll
       for (int e = 0; e < SA_EACH; ++e) {
         const int bin = at + e;
+        const float begin = exp2f((float)(-per_step * bin));
         low[e] = high[e] = 0;
         if (n[e] && bin <= rank_bin) {
           if (bin < rank_bin) {
-            const double f = __fdividef((float)s.all_into[bin], (float)n[e] * z.fine);
-            high[e] = begin * n[e] * (1 - f * (1 - full)) * wider;
-            low[e] = begin * n[e] * exp2f((float)(-per * (f + 1.0 / z.fine))) * less;
+            const float f = __fdividef((float)s.all_into[bin], (float)n[e] * z.fine);
+            high[e] = begin * n[e] * (1.f - f * (1.f - full)) * wider;
+            low[e] = begin * n[e] * exp2f(-per * (f + 1.f / z.fine)) * less;
           } else {  // only the first ones of the step
             high[e] = begin * (k - rank_before) * wider;
             low[e] = begin * (k - rank_before) * full * less;
           }
           if (z.inv == 0.f) low[e] = 0;  // (no steps: equal entries, or a range that floats do not hold)
         }
-        begin *= full;
       }
-      double high_run = block_before(high[0] + high[1] + high[2] + high[3], s.part, high_total);
-      double low_run = block_before(low[0] + low[1] + low[2] + low[3], s.part2, low_total);
+      float high_run = block_before(high[0] + high[1] + high[2] + high[3], s.narrow, high_total);
+      float low_run = block_before(low[0] + low[1] + low[2] + low[3], s.narrow2, low_total);
+      const float reach_high = (float)p * high_total * 1.00001f, reach_low = (float)p * low_total * 0.99999f;
       // can: the first step at whose end the sum can have reached p of the total; must: the first at whose end it has to have
       unsigned can = SA_BINS - 1, must = SA_BINS - 1;
 #pragma unroll
       for (int e = 0; e < SA_EACH; ++e) {
         high_run += high[e];
         low_run += low[e];
-        if (can == SA_BINS - 1 && high_run >= p * low_total) can = at + e;
-        if (must == SA_BINS - 1 && low_run >= p * high_total) must = at + e;
+        if (can == SA_BINS - 1 && high_run >= reach_low) can = at + e;
+        if (must == SA_BINS - 1 && low_run >= reach_high) must = at + e;
       }
       can = (unsigned)block_least(can, s.wide);
       must = (unsigned)block_least(must, s.wide);
@@ -986,27 +988,29 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   else if (tid == 0) a.token[b] = token;
 }
 
-// Blocks of a row: as many as are resident at once with B rows, two to a multiprocessor; slices that are small enough stay in shared memory,
-// others are read from L2 in every sweep. (256 rows of 50272 entries: 91 us with four blocks per row, in four waves.)
+// Blocks of a row: as many as are resident at once with B rows, two to a multiprocessor (clusters stay inside a group of multiprocessors, so
+// fewer of the larger ones fit), but not so few that a slice finds no room beside another one. Slices that find none are read from L2
+// in every sweep. (256 rows of 50272 entries: 88 us with four blocks per row in four waves, 134 with one block per row and L2.)
 template <typename T>
 static cudaError_t launch_sample(const SampleArgs &a, int B, bool vec, cudaStream_t st) {
-  constexpr int N = Chunk<T>::N, fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16, most = 200 * 1024;
-  int C = SA_CLUSTER;
-  // (not so few that a slice finds no room beside another one)
-  while (C > 1 && (a.V / C < 512 || ((long long)B * C > 2 * sm_count() && (long long)(a.V / C) * 2 * sizeof(T) <= 112 * 1024 - fixed))) C /= 2;
-  const int slice = ceil_div(ceil_div(a.V, C), N) * N;
-  const int room = (B * C <= sm_count() ? most : 112 * 1024) - fixed;
-  const bool stored = (long long)slice * sizeof(T) <= room;
-  const int smem = fixed + (stored ? slice * (int)sizeof(T) : 0);
+  constexpr int N = Chunk<T>::N, fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16, most = 200 * 1024, beside = 112 * 1024;
   static DevicePrep prep;
-  const int(*unused)[4];
+  const int(*resident)[4];
   cudaError_t e = prep.get(
-      [&](int(&)[4]) {
-        cudaError_t f = cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      [&](int(&clusters)[4]) {
+        cudaError_t f = cluster_residency(sample_kernel<T, true>, SA_THREADS, beside, 2, clusters);
+        if (f == cudaSuccess) f = cudaFuncSetAttribute(sample_kernel<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         return f != cudaSuccess ? f : cudaFuncSetAttribute(sample_kernel<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       },
-      unused);
+      resident);
   if (e != cudaSuccess) return e;
+  int log = 3;
+  static_assert(SA_CLUSTER == 8, "clusters of up to 2^3 blocks");
+  while (log > 0 && (a.V >> log < 512 || (B > (*resident)[log] && (long long)(a.V >> log) * 2 * (int)sizeof(T) <= beside - fixed))) --log;
+  const int C = 1 << log, slice = ceil_div(ceil_div(a.V, C), N) * N;
+  const int room = ((long long)B * C <= sm_count() ? most : beside) - fixed;
+  const bool stored = (long long)slice * (int)sizeof(T) <= room;
+  const int smem = fixed + (stored ? slice * (int)sizeof(T) : 0);
   return djv::launch_kernel_cluster(vec ? sample_kernel<T, true> : sample_kernel<T, false>, dim3(B * C), dim3(SA_THREADS), smem, st, dim3(C, 1, 1),
                                     a, slice, (int)stored);
 }
