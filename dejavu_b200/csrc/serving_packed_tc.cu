@@ -29,7 +29,7 @@
 
 namespace djv {
 
-constexpr int PT_THREADS = 384, PT_M = 128, PT_N = 128, PT_Q = 2 * PT_M;  // rows of a query tile, of a key tile, of an item
+constexpr int PT_THREADS = 384, PT_M = 128;  // rows of a query tile
 constexpr int PT_SOFT = 8, PT_LOADER = 8, PT_ISSUER = 9, PT_SCAN = 10;  // softmax warps, and the others
 constexpr int PT_TABLE = 1024;  // items per head that are put in order
 constexpr int PT_ROUNDS = 256;  // items of a block that are looked up at a time
@@ -75,7 +75,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 __device__ unsigned g_packed_timeouts;  // bounded waits that ran out (never, in a healthy run)
 
-// a box of 64 elements x 1 head x 128 rows
+// a box of 64 elements x 1 head x the map's rows
 __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap *map, int d, int head, int row, uint64_t *bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
@@ -105,7 +105,8 @@ struct Exponent<__half> {
   static constexpr uint32_t MASK = 0x7c007c00u, ONE = 0x04000400u;
 };
 
-template <typename T, int KB, int STAGES, bool FULL>  // KB: blocks of 64 elements in a row; FULL: all of them are in use
+// KB: blocks of 64 elements in a row; FULL: all of them are in use; NT: query tiles of an item; KN: keys of a tile
+template <typename T, int KB, bool FULL, int NT, int KN, int STAGES>
 __global__ void __launch_bounds__(PT_THREADS, 1)
 packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, PackedArgs a, int most) {
@@ -116,10 +117,11 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __shared__ int2 table[PT_TABLE];    // sequence and item in it, by falling work
   __shared__ int4 mine[PT_ROUNDS];    // the block's items: the sequence's first row, first query in it, queries, head
   __shared__ int odd[2][2][2];  // by the item's parity: what each of the two warps found in each of the two value tiles
-  constexpr uint32_t TILE = KB * PT_N * 128;
+  constexpr uint32_t Q_TILE = KB * PT_M * 128, TILE = KB * KN * 128, O_AT = NT * KN;  // bytes; columns of TMEM in front of O
+  constexpr int PT_Q = NT * PT_M;
   const int tid = threadIdx.x, warp = tid / WARP, lane = tid % WARP;
   unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  const uint32_t q_sm = smem_u32(base), ring = q_sm + 2 * TILE;
+  const uint32_t q_sm = smem_u32(base), ring = q_sm + NT * Q_TILE;
   if (tid == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
@@ -225,7 +227,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const int t = warp / 4, r = tid % PT_M;
     const uint32_t lane_base = (uint32_t)(warp % 4 * 32) << 16;
     // the row's scores, over which it puts its weights, and its sums
-    const uint32_t tm_s = tm + t * PT_N + lane_base, tm_o = tm + 2 * PT_N + t * (KB * 64) + lane_base;
+    const uint32_t tm_s = tm + t * KN + lane_base, tm_o = tm + O_AT + t * (KB * 64) + lane_base;
     const float c = a.scale * 1.4426950408889634f, ca = c == 0.f ? 1e-30f : fabsf(c);  // scores in units of log 2
     const uint64_t ca2 = pack2(ca, ca);
     if (!a.keep_rest) {  // rows of no sequence
@@ -247,34 +249,33 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (w.z <= 0) continue;
       parity ^= 1;
       if (rows <= 0) continue;
-      const int last = q0 / PT_N + t;  // the key tile of the row's own key
+      const int last = (q0 + min(w.z, (t + 1) * PT_M) - 1) / KN;  // the key tile of the tile's last key
       float m = 0.f, l = 0.f;
       for (int j = 0; j <= last; ++j, ++steps) {
         if (!dead) dead = !mbar_wait(&s_full[t], steps & 1);
         __syncwarp();
         tmem_fence_after();
-        uint32_t s[4][32];
-        tmem_ld32(s[0], tm_s);
-        tmem_ld32(s[1], tm_s + 32);
-        tmem_ld32(s[2], tm_s + 64);
-        tmem_ld32(s[3], tm_s + 96);
+        uint32_t s[KN / 32][32];
+#pragma unroll
+        for (int q = 0; q < KN / 32; ++q) tmem_ld32(s[q], tm_s + q * 32);
         tmem_wait_ld();
         if (c < 0.f) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < KN / 32; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e) s[q][e] ^= 0x80000000u;
         }
-        if (j == last) {  // keys behind the row's own
+        if ((j + 1) * KN > q0 + t * PT_M) {  // keys behind the row's own
+          const int own = q0 + t * PT_M + r - j * KN;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q < KN / 32; ++q)
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (q * 32 + e > r) s[q][e] = 0xff800000u;
+              if (q * 32 + e > own) s[q][e] = 0xff800000u;
         }
         float mm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int q = 0; q < KN / 32; ++q)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) mm[e / 2 % 4] = max3(mm[e / 2 % 4], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
         const float mx = fmaxf(max3(mm[0], mm[1], mm[2]), mm[3]) * ca;
@@ -300,7 +301,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const uint64_t nm2 = pack2(-m, -m);
         uint64_t l2[2] = {0, 0};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < KN / 32; ++q) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -341,8 +342,8 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const int i = q0 + t * PT_M + r, g = h / (a.H / a.G);
           for (int d2 = 0; d2 < 2; ++d2) {
             if (!(d2 ? odd1 : odd0)) continue;
-            const int j0 = q0 + d2 * PT_N;
-            for (int j = j0; j <= min(i, j0 + PT_N - 1); ++j) {
+            const int j0 = (q0 / KN + d2) * KN;
+            for (int j = j0; j <= min(i, j0 + KN - 1); ++j) {
               const T *v = static_cast<const T *>(a.v) + (long long)(first + j) * a.ldv + g * a.hv;
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
@@ -384,9 +385,10 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       const int4 w = mine[round % PT_ROUNDS];
       if (w.z <= 0 || dead) continue;
-      const int row0 = w.x, q0 = w.y, h = w.w, g = h / (a.H / a.G), d0 = q0 / PT_N;
+      const int row0 = w.x, q0 = w.y, h = w.w, g = h / (a.H / a.G), d0 = q0 / KN;
       const bool both = w.z > PT_M;
-      const int n = d0 + (both ? 2 : 1);  // key tiles
+      // the last key tiles of the query tiles, and how many there are; from d0 on not every row sees all of a tile
+      const int last0 = (q0 + min(w.z, PT_M) - 1) / KN, n = (q0 + w.z - 1) / KN + 1;
       parity ^= 1;
       if (warp == PT_LOADER) {
         if (lane == 0) {
@@ -395,48 +397,49 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (slot >= STAGES && !dead) dead = !mbar_wait(&empty[s], (slot / STAGES - 1) & 1);
             if (dead) return;
             mbar_arrive_expect_tx(&full[s], TILE);
-            for (int b = 0; b < KB; ++b) tma_load_rows(ring + s * TILE + b * PT_N * 128, map, b * 64, head, row, &full[s]);
+            for (int b = 0; b < KB; ++b) tma_load_rows(ring + s * TILE + b * KN * 128, map, b * 64, head, row, &full[s]);
             ++slot;
           };
           for (int t = 0; t < (both ? 2 : 1); ++t) {
             if (used[t] && !dead) dead = !mbar_wait(&q_empty[t], (used[t] - 1) & 1);
             if (dead) break;
             ++used[t];
-            mbar_arrive_expect_tx(&q_full[t], TILE);
+            mbar_arrive_expect_tx(&q_full[t], Q_TILE);
             for (int b = 0; b < KB; ++b)
-              tma_load_rows(q_sm + t * TILE + b * PT_M * 128, &map_q, b * 64, h, row0 + q0 + t * PT_M, &q_full[t]);
+              tma_load_rows(q_sm + t * Q_TILE + b * PT_M * 128, &map_q, b * 64, h, row0 + q0 + t * PT_M, &q_full[t]);
             if (t == 0) load(&map_k, g, row0);
           }
           for (int j = 0; j < n && !dead; ++j) {
-            if (j) load(&map_k, g, row0 + j * PT_N);
-            load(&map_v, g, row0 + j * PT_N);
+            if (j) load(&map_k, g, row0 + j * KN);
+            load(&map_v, g, row0 + j * KN);
           }
         }
         dead = __shfl_sync(0xffffffffu, (int)dead, 0) != 0;
       } else if (warp == PT_ISSUER) {
         constexpr bool FP16 = !__is_same(T, bf16);
-        const uint32_t idesc_s = mma_idesc(PT_M, PT_N, false, false, FP16), idesc_o = mma_idesc(PT_M, FULL ? KB * 64 : (a.D + 15) / 16 * 16, false, true, FP16);
+        const uint32_t idesc_s = mma_idesc(PT_M, KN, false, false, FP16), idesc_o = mma_idesc(PT_M, FULL ? KB * 64 : (a.D + 15) / 16 * 16, false, true, FP16);
         const int k_steps = FULL ? KB * 4 : (a.D + 15) / 16;
-        const uint64_t qd = desc_k_major(q_sm, PT_M, 0), k0 = desc_k_major(ring, PT_N, 0), v0 = desc_mn_major(ring, PT_N, 0);
+        const uint64_t qd = desc_k_major(q_sm, PT_M, 0), k0 = desc_k_major(ring, KN, 0), v0 = desc_mn_major(ring, KN, 0);
         auto wait = [&](uint64_t *bar, int phase) {
           if (!dead && !mbar_try_wait(bar, phase & 1)) dead = !mbar_wait(bar, phase & 1);
           __syncwarp();
           tmem_fence_after();
         };
         auto scores = [&](int t, int at) {
-          const uint64_t q = qd + t * (TILE / 16), k = k0 + at % STAGES * (TILE / 16);
+          const uint64_t q = qd + t * (Q_TILE / 16), k = k0 + at % STAGES * (TILE / 16);
 #pragma unroll
           for (int x = 0; x < KB * 4; ++x) {
-            const uint32_t step = (x / 4) * (PT_N * 128 / 16) + (x % 4) * 2;  // descriptor units of 16 bytes
-            if (FULL || x < k_steps) warp_mma_ss(tm + t * PT_N, q + step, k + step, idesc_s, x > 0);
+            // (descriptor units of 16 bytes)
+            if (FULL || x < k_steps)
+              warp_mma_ss(tm + t * KN, q + (x / 4) * (PT_M * 128 / 16) + (x % 4) * 2, k + (x / 4) * (KN * 128 / 16) + (x % 4) * 2, idesc_s, x > 0);
           }
           warp_commit(&s_full[t]);
         };
         auto values = [&](int t, int at, bool begun) {
           const uint64_t v = v0 + at % STAGES * (TILE / 16);
 #pragma unroll
-          for (int x = 0; x < PT_N / 16; ++x)
-            warp_mma_ts(tm + 2 * PT_N + t * (KB * 64), tm + t * PT_N + x * 8, v + (uint64_t)(x * 128), idesc_o,
+          for (int x = 0; x < KN / 16; ++x)
+            warp_mma_ts(tm + O_AT + t * (KB * 64), tm + t * KN + x * 8, v + (uint64_t)(x * 128), idesc_o,
                         x > 0 ? 1u : (uint32_t)begun);
         };
         // slots of this item: K0, V0, K1, V1, ... Those of the next step are waited for behind this step's products.
@@ -460,13 +463,13 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         arrive(0);
         for (int j = 0; j < n; ++j) {
           const int vs = first + 2 * j + 1;
-          if (j <= d0) {
+          if (j <= last0) {
             wait(&p_full[0], stepped[0]);
             ++stepped[0];
             values(0, vs, j > 0);
-            if (j < d0) {
+            if (j < last0) {
               scores(0, vs + 1);
-              if (j + 1 == d0) warp_commit(&q_empty[0]);
+              if (j + 1 == last0) warp_commit(&q_empty[0]);
             } else {
               warp_commit(&o_full[0]);
               if (j == 0) warp_commit(&q_empty[0]);  // (a tile with one key tile)
@@ -481,7 +484,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           if (j + 1 < n) {
             if (both) {
               scores(1, vs + 1);
-              if (j == d0) warp_commit(&q_empty[1]);
+              if (j + 2 == n) warp_commit(&q_empty[1]);
             }
             warp_commit(&empty[(vs + 1) % STAGES]);
             arrive(j + 1);
@@ -507,7 +510,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (lane == 0) mbar_arrive(&empty[vs % STAGES]);
             continue;
           }
-          uint4 *v = reinterpret_cast<uint4 *>(base + 2 * TILE + vs % STAGES * TILE);
+          uint4 *v = reinterpret_cast<uint4 *>(base + NT * Q_TILE + vs % STAGES * TILE);
           // the largest magnitude, two 16-bit numbers at a time: infinities and NaN are above all others
           uint32_t large[4] = {0, 0, 0, 0};
 #pragma unroll 4
@@ -562,11 +565,11 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   }
 }
 
-// rows of heads of D elements: boxes of 64 elements x 1 head x 128 rows with the 128-byte swizzle, zeros outside
-static bool rows_map(CUtensorMap *map, bool fp16, const void *p, long long ld, long long hs, int T, int heads, int D) {
+// rows of heads of D elements: boxes of 64 elements x 1 head x `rows` rows with the 128-byte swizzle, zeros outside
+static bool rows_map(CUtensorMap *map, bool fp16, const void *p, long long ld, long long hs, int T, int heads, int D, int rows) {
   const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)T},
                    strides[2] = {(cuuint64_t)(heads > 1 ? hs : ld) * 2, (cuuint64_t)ld * 2};
-  const cuuint32_t box[3] = {64, 1, PT_M}, unit[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)rows}, unit[3] = {1, 1, 1};
   return encode_tiled()(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(p), dims,
                         strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -577,28 +580,29 @@ static bool rows_fit(const void *p, long long ld, long long hs, int heads) {
   return aligned16(p) && ld > 0 && ld % 8 == 0 && ld < (1ll << 36) && (heads == 1 || (hs > 0 && hs % 8 == 0 && hs < (1ll << 36)));
 }
 bool packed_tc_supported(int dtype, const PackedArgs &a) {
-  return dtype != DJV_DTYPE_F32 && a.D % 8 == 0 && a.D <= 128 && rows_fit(a.q, a.ldq, a.hq, a.H) && rows_fit(a.k, a.ldk, a.hk, a.G) &&
-         rows_fit(a.v, a.ldv, a.hv, a.G) && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (long long)packed_tiles<PT_Q>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
+  return dtype != DJV_DTYPE_F32 && a.D % 8 == 0 && a.D <= 256 && rows_fit(a.q, a.ldq, a.hq, a.H) && rows_fit(a.k, a.ldk, a.hk, a.G) &&
+         rows_fit(a.v, a.ldv, a.hv, a.G) && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (long long)packed_tiles<PT_M>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
 }
 
 template <typename T, int KB, bool FULL>
 static int launch_packed_tc(const PackedArgs &a, cudaStream_t st) {
-  constexpr int STAGES = KB == 1 ? 8 : 4, smem = 1024 + (2 + STAGES) * KB * PT_N * 128;
+  // Heads of more than 128: O takes 256 columns of TMEM, so that there is room for one query tile, and tiles of 64 keys for four stages.
+  constexpr int NT = KB > 2 ? 1 : 2, KN = KB > 2 ? 64 : 128, STAGES = KB == 1 ? 8 : 4;
+  constexpr int smem = 1024 + NT * KB * PT_M * 128 + STAGES * KB * KN * 128;
   constexpr bool FP16 = !__is_same(T, bf16);
+  const auto kernel = packed_tc_kernel<T, KB, FULL, NT, KN, STAGES>;
   CUtensorMap q, k, v;
-  if (!rows_map(&q, FP16, a.q, a.ldq, a.hq, a.T, a.H, a.D) || !rows_map(&k, FP16, a.k, a.ldk, a.hk, a.T, a.G, a.D) ||
-      !rows_map(&v, FP16, a.v, a.ldv, a.hv, a.T, a.G, a.D)) {
+  if (!rows_map(&q, FP16, a.q, a.ldq, a.hq, a.T, a.H, a.D, PT_M) || !rows_map(&k, FP16, a.k, a.ldk, a.hk, a.T, a.G, a.D, KN) ||
+      !rows_map(&v, FP16, a.v, a.ldv, a.hv, a.T, a.G, a.D, KN)) {
     set_error("packed_attention: a tensor map was refused");
     return DJV_ERR_CUDA;
   }
   static DevicePrep prep;
   const int(*unused)[4];
-  cudaError_t e = prep.get(
-      [&](int(&)[4]) { return cudaFuncSetAttribute(packed_tc_kernel<T, KB, STAGES, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); },
-      unused);
-  const int tiles = packed_tiles<PT_Q>(a.T, a.B), grid = tiles * a.H < sm_count() ? tiles * a.H : sm_count();  // (no fewer than there can be)
-  if (e == cudaSuccess)
-    e = djv::launch_kernel(packed_tc_kernel<T, KB, STAGES, FULL>, dim3(grid), dim3(PT_THREADS), smem, st, q, k, v, a, tiles);
+  cudaError_t e = prep.get([&](int(&)[4]) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); }, unused);
+  // (no fewer than there can be)
+  const int tiles = packed_tiles<NT * PT_M>(a.T, a.B), grid = tiles * a.H < sm_count() ? tiles * a.H : sm_count();
+  if (e == cudaSuccess) e = djv::launch_kernel(kernel, dim3(grid), dim3(PT_THREADS), smem, st, q, k, v, a, tiles);
   if (e != cudaSuccess) {
     cudaGetLastError();
     set_error("packed_attention: CUDA error %d (%s)", (int)e, cudaGetErrorString(e));
@@ -612,7 +616,8 @@ int packed_tc(int dtype, const PackedArgs &a, cudaStream_t st) {
   const auto of = [&](auto t) {
     using T = decltype(t);
     if (a.D <= 64) return a.D == 64 ? launch_packed_tc<T, 1, true>(a, st) : launch_packed_tc<T, 1, false>(a, st);
-    return a.D == 128 ? launch_packed_tc<T, 2, true>(a, st) : launch_packed_tc<T, 2, false>(a, st);
+    if (a.D <= 128) return a.D == 128 ? launch_packed_tc<T, 2, true>(a, st) : launch_packed_tc<T, 2, false>(a, st);
+    return a.D == 256 ? launch_packed_tc<T, 4, true>(a, st) : launch_packed_tc<T, 4, false>(a, st);
   };
   return dtype == DJV_DTYPE_F16 ? of(__half()) : of(bf16());
 }

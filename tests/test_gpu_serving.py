@@ -373,6 +373,32 @@ def test_packed_attention_values_that_are_not_finite_reach_those_who_see_them(op
         assert torch.equal(got, want), r
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [136, 192, 256])
+def test_packed_attention_of_wide_heads(ops, dtype, D):
+    """Tiles of 64 keys, of which a sequence's last query tile sees one or two that not all its rows see."""
+    lengths, H, G = [64, 65, 191, 192, 193, 1, 900, 63], 3, 1
+    T = sum(lengths)
+    check_packed(ops, rnd(51, T, H, D, dtype=dtype), rnd(52, T, G, D, dtype=dtype), rnd(53, T, G, D, dtype=dtype), lengths, D ** -0.5)
+    up = torch.linspace(0, 300, 900, device="cuda")[:, None, None] / D  # scores that grow along the keys
+    ones = torch.ones(900, 1, D, dtype=dtype, device="cuda")
+    check_packed(ops, ones, (up * ones).to(dtype), rnd(54, 900, 1, D, dtype=dtype), [900], 1.0)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_packed_attention_of_wide_heads_with_values_that_are_not_finite(ops, dtype):
+    n, H, D = 330, 2, 160
+    q, k, v = rnd(34, n, H, D, dtype=dtype), rnd(35, n, H, D, dtype=dtype), rnd(36, n, H, D, dtype=dtype)
+    want = ops.packed_attention(q, k, v, cumulative([n]), 0.1)
+    for r in (0, 63, 64, 127, 128, 191, 192, 255, 256, 329):
+        w = v.clone()
+        w[r, 1, 150] = math.inf
+        got = ops.packed_attention(q, k, w, cumulative([n]), 0.1)
+        assert bool((got[r:, 1, 150] == math.inf).all())
+        got[r:, 1, 150] = want[r:, 1, 150]
+        assert torch.equal(got, want), r
+
+
 @pytest.mark.parametrize("form", ["odd_rows", "odd_address", "heads_first", "every_second"])
 def test_packed_attention_takes_any_layout(ops, form):
     lengths, H, G, D = [130, 7], 4, 2, 64
