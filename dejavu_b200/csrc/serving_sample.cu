@@ -26,13 +26,17 @@
 #include <cooperative_groups.h>
 #include <utility>
 
+#include "pairs.cuh"
 #include "serving.cuh"
 
 namespace djv {
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / WARP, SA_BINS = 2048, SA_LIST = 2048, SA_CLUSTER = 8;
 constexpr int SA_EACH = SA_BINS / SA_THREADS;  // steps, or entries of the list, of a thread
-constexpr double SA_CLOSE = 3e-9;   // what counts as close, of a sum: three times the weights' relative error
+constexpr double SA_CLOSE = 3e-9;   // what counts as close, of a sum: more than twice the weights' relative error
+constexpr int SA_TABLE = 256;
+constexpr float SA_MAGIC = 12582912.f;  // added to a number below 2^22 rounds it: the lowest bits are then the number's
+constexpr uint32_t SA_ROUND = 0x4b400000u;  // (its bits)
 constexpr float SA_FAR = 45.f;      // temperatures below the largest entry from where on nothing counts (e^-45 = 3e-20)
 
 struct SampleArgs {
@@ -61,7 +65,6 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
-constexpr uint32_t SA_NONE = 0x007fffffu;  // order_of(-inf)
 __device__ __forceinline__ u64 place_of(uint32_t key, int i) { return (u64)key << 32 | (uint32_t)~i; }
 
 struct SampleShared {
@@ -77,7 +80,7 @@ struct SampleShared {
     double mass[SA_BINS];       // (of a block that works alone)
   };
   unsigned into[SA_BINS], all_into[SA_BINS];  // sum of how far into the step entries are, in parts; of the slice, of the row
-  float2 table[64];           // 2^(j / 64), as the sum of two floats
+  uint2 table[SA_TABLE];      // 2^(30 + j / 256), rounded, less SA_ROUND; and as a float
   double part[SA_WARPS], part2[SA_WARPS], part3[SA_WARPS];
   u64 wide[SA_WARPS];
   float narrow[SA_WARPS], narrow2[SA_WARPS];
@@ -236,44 +239,42 @@ struct SampleScale {
   __device__ __forceinline__ float part_of(float x) const { return x == top ? 8388608.f : fmaf(top - x, inv_fine, 8388608.f); }
   __device__ __forceinline__ float parts(float step) const { return fmaf(step, fine, 8388608.f); }
   __device__ __forceinline__ double exact(float x) const { return x == top ? 1.0 : exp(((double)x - (double)top) / temperature); }
-  // For x that counts (for others a number that means nothing): y = (x - top) log2(e) / temperature >= -65 as the sum of two floats,
-  // y = k / 64 + f
-  __device__ __forceinline__ int reduced(float x, float &q) const {  // k, and 2^f - 1
-    const float t = x - top, v = t - x, e = (x - (t - v)) - (top + v);  // x - top = t + e
-    const float y = fmaxf(t * c_hi, -100.f), rest = fmaf(t, c_hi, -y) + fmaf(t, c_lo, e * c_hi);
-    const float k = rintf(y * 64.f);
-    const float f = (fmaf(k, -0.015625f, y) + rest) * 0.69314718f;  // (the difference is exact)
-    q = fmaf(f * f, fmaf(f, fmaf(f, 0.041666668f, 0.16666667f), 0.5f), f);
-    return (int)k;
+  // For x that counts (for others a number that means nothing): 2^((x - top) c) = 2^(n / 256) (1 + q), in two at a time; bits receives n as
+  // the lowest bits of SA_MAGIC + n. |q| <= 0.00136, so that two terms of its series are left to 3e-13.
+  __device__ __forceinline__ uint64_t reduced(uint64_t t, uint64_t x, uint64_t &bits) const {  // t: x - top, rounded
+    const uint64_t ch = pack2(c_hi, c_hi), zero = pack2(0.f, 0.f);
+    const uint64_t v = sub2(t, x), e = sub2(sub2(x, sub2(t, v)), add2(pack2(top, top), v));  // x - top = t + e
+    const uint64_t ny = fma2(t, pack2(-c_hi, -c_hi), zero);                                   // -y, and what it lacks:
+    const uint64_t rest = add2(fma2(t, ch, ny), fma2(t, pack2(c_lo, c_lo), fma2(e, ch, zero)));
+    bits = fma2(ny, pack2(-256.f, -256.f), pack2(SA_MAGIC, SA_MAGIC));
+    const uint64_t n = sub2(bits, pack2(SA_MAGIC, SA_MAGIC)), nf = fma2(n, pack2(0.00390625f, 0.00390625f), ny);  // (exact)
+    const uint64_t f = fma2(sub2(rest, nf), pack2(0.69314718f, 0.69314718f), zero);
+    return fma2(fma2(f, f, zero), fma2(f, pack2(0.16666667f, 0.16666667f), pack2(0.5f, 0.5f)), f);
   }
-  __device__ __forceinline__ double weight(float x, const float2 *table) const {
-    float q;
-    const int n = reduced(x, q);
-    const double w = (double)table[n & 63].x + (double)table[n & 63].y;
-    const double scaled = __longlong_as_double(__double_as_longlong(fma(w, (double)q, w)) + ((long long)(n >> 6) << 52));
-    return x == top ? 1.0 : scaled;  // (+inf among them)
+  // 2^(n / 256) (1 + q) as an integer times 2^(-30 - down): off by 1.2e-9 of it at most (the table by 2^-31, the rounding by as much)
+  __device__ __forceinline__ static uint32_t mantissa(float bits, float q, const uint2 *table, unsigned &down) {
+    const uint32_t n = __float_as_uint(bits);
+    const uint2 w = table[n % SA_TABLE];
+    down = SA_ROUND / SA_TABLE - n / SA_TABLE;
+    return w.x + __float_as_uint(fmaf(__uint_as_float(w.y), q, SA_MAGIC));
   }
-  // the same as the sum of two floats
-  __device__ __forceinline__ float2 weight_pair(float x, const float2 *table) const {
-    float q;
-    const int n = reduced(x, q);
-    const float2 w = table[n & 63];
-    const float scale = __uint_as_float((uint32_t)((n >> 6) + 127) << 23), rest = fmaf(w.x, q, w.y), hi = w.x + rest;
-    return x == top ? make_float2(1.f, 0.f) : make_float2(hi * scale, (rest - (hi - w.x)) * scale);
+  __device__ __forceinline__ double weight(float x, const uint2 *table) const {
+    uint64_t bits;
+    float b0, b1, q0, q1;
+    const uint64_t x2 = pack2(x, x);
+    unpack2(reduced(sub2(x2, pack2(top, top)), x2, bits), q0, q1);
+    unpack2(bits, b0, b1);
+    unsigned down;
+    const uint32_t m = mantissa(b0, q0, table, down);
+    return (double)m * __longlong_as_double((long long)(1023 - 30 - down) << 52);
   }
 };
-
-// A sum of such pairs, with 40 bits and more: what the larger part loses joins the smaller one. (Additions of 64-bit numbers take
-// ten times as long as one of 32 bits.)
-struct PairSum {
-  float hi = 0.f, lo = 0.f;
-  __device__ __forceinline__ void add(float2 w) {
-    const float s = hi + w.x, back = s - hi;
-    lo += ((hi - (s - back)) + (w.x - back)) + w.y;
-    hi = s;
-  }
-  __device__ __forceinline__ double value() const { return (double)hi + (double)lo; }
-};
+constexpr int SA_UNITS = 52;  // sums are integers, 2^52 to the largest weight: 4096 of those fit
+__device__ __forceinline__ u64 shifted(u64 v, unsigned down) {  // (0 from 64 on)
+  u64 r;
+  asm("shr.u64 %0, %1, %2;" : "=l"(r) : "l"(v), "r"(down));
+  return r;
+}
 
 // One row by one block, in 64 bits, from global memory: nothing is too close and nothing too much.
 template <typename T, bool VEC>
@@ -414,35 +415,63 @@ struct SampleAlone {
     __syncthreads();
     double total = 0;
     for (int w = 0; w < SA_WARPS; ++w) total += s.part[w];
-    return locate(entries, lo, hi, 0.0, u * total, total, kept);
+    return locate(entries, from, to, share, 0.0, u * total, total, kept);
   }
 
-  // s.part has the warps' sums, `before` is in front of the first: where the running sum passes target. found[1]: too close to tell.
-  template <typename K>
-  __device__ int locate(const T *entries, int lo, int hi, double before, double target, double total, K kept) {
-    const int warp = threadIdx.x / WARP, lane = threadIdx.x % WARP;
-    int mine = SA_WARPS;  // the warp whose part the target falls into: the first whose running sum exceeds it
-    int last = 0;         // the last warp that keeps anything
+  // The first of SA_WARPS sums at which the running sum exceeds target (before: in front of the first, then of that one); SA_WARPS: none, and
+  // last has the last that is not 0.
+  __device__ __forceinline__ static int passed(const double *sums, double &before, double target, int &last) {
+    last = 0;
+    double run = before;
     for (int w = 0; w < SA_WARPS; ++w) {
-      if (s.part[w] > 0) last = w;
-      if (mine == SA_WARPS && before + s.part[w] > target) mine = w;
-      if (mine == SA_WARPS) before += s.part[w];
+      if (sums[w] > 0) last = w;
+      if (run + sums[w] > target) {
+        before = run;
+        return w;
+      }
+      run += sums[w];
     }
-    if (mine == SA_WARPS) {  // (rounding: the last entry that is kept)
-      mine = last;
+    return SA_WARPS;
+  }
+  // s.part has the sums of shares of the entries from .. to - 1, `before` is in front of the first: where the running sum passes target.
+  // found[1]: too close to tell.
+  template <typename K>
+  __device__ int locate(const T *entries, int from, int to, int share, double before, double target, double total, K kept) {
+    const int warp = threadIdx.x / WARP, lane = threadIdx.x % WARP;
+    int last;
+    int at = passed(s.part, before, target, last);
+    if (at == SA_WARPS) {  // (rounding: the last entry that is kept)
+      at = last;
       target = INFINITY;
       before = 0;
     }
-    if (warp == mine) {
+    // that share by all warps
+    from = min(to, from + at * share);
+    to = min(to, from + share);
+    share = (share + SA_THREADS - 1) / SA_THREADS * WARP;
+    const int lo = min(to, from + warp * share), hi = min(to, lo + share);
+    double sum = 0;
+    for (int i = lo + lane; i < hi; i += WARP) sum += kept(to_f(entries[i]), i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s.part2[warp] = sum;
+    __syncthreads();
+    at = passed(s.part2, before, target, last);
+    bool near = false;
+    if (at == SA_WARPS) {
+      near = target < INFINITY;  // (the two sums differ in their rounding)
+      at = last;
+    }
+    if (warp == at) {
       double run = before;
       int token = -1, latest = -1;
-      bool near = fabs(before - target) <= SA_CLOSE * total;
+      near |= fabs(before - target) <= SA_CLOSE * total;
       for (int i0 = lo; i0 < hi && token < 0; i0 += WARP) {
         const int i = i0 + lane;
         const double w = i < hi ? kept(to_f(entries[i]), i) : 0.0;
         const unsigned any = __ballot_sync(0xffffffffu, w > 0);
         if (any == 0) continue;
-        double sum = w;
+        sum = w;
 #pragma unroll
         for (int o = 1; o < WARP; o <<= 1) {
           const double up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -543,7 +572,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   SampleAlone<T, VEC> r{row, a.V, s, {}};
   SampleScale &z = r.z;
   // four entries at a time, whatever their type: short code
-  constexpr int FOUR = VEC ? 4 : 1;
+  constexpr int FOUR = VEC ? 4 : 2;
   auto four = [&](int i, float (&x)[FOUR]) {
     if (VEC && i + FOUR <= hi) {
       if (sizeof(T) == 4) {
@@ -613,10 +642,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
       }
     }
   }
-  if (tid < 64) {
-    const double w = power_of_2(tid * 0.015625);
-    const float high = (float)w;
-    s.table[tid] = make_float2(high, (float)(w - (double)high));
+  if (tid < SA_TABLE) {
+    const double w = power_of_2(30.0 + tid * (1.0 / SA_TABLE));
+    s.table[tid] = make_uint2(__double2uint_rn(w) - SA_ROUND, __float_as_uint((float)w));
   }
   for (int i = tid; i < SA_BINS; i += SA_THREADS) s.count[i] = s.into[i] = 0;
   if (tid == 0) s.listed = s.own = 0;
@@ -663,6 +691,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     const int token = r.token(k, p, min_p, u);
     if (tid == 0) a.token[b] = token;
   };
+  if (z.top == INFINITY || !(log2_unit > 1e-25 && log2_unit < 1e30)) {  // (not for sums of two floats)
+    if (rank == 0) alone();
+    return;
+  }
   // The block's own list (indices; fewer than SA_LIST, as the counts say): begun, an entry, and sent to the first block's list.
   auto begin_list = [&]() {
     if (tid == 0) s.own = 0;
@@ -693,38 +725,65 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     cluster.sync();
   };
   const bool by_min = min_p > 0;
+  const float min_high = (float)min_p * 1.000001f, min_low = (float)min_p * 0.999999f;  // (of weights in 32 bits)
   auto enough = [&](float x, double w) { return w >= min_p * (1 + 1e-8) || (w >= min_p * (1 - 1e-8) && z.exact(x) >= min_p); };
   // Weights of the entries that top-k keeps: in front of step `from` and from step `to` on (to the first block's sums), and, in s.part, of the
   // first ones that min-p keeps too, warp by warp. Those between go to the lists. (No branches around the weights, so that those
-  // of a chunk overlap.)
+  // of a chunk overlap. Sums are integers: exact whatever their order, and a third of what pairs of floats take.)
   auto weigh = [&](float from, float to) {
     begin_list();
     from = z.parts(from);  // (infinite ones stay so)
     to = z.parts(to);
     const float rank_from = z.parts((float)rank_bin), rank_to = z.parts((float)rank_bin + 1);
-    PairSum front, behind, enough_too;
-    for (int i = lo + lane * FOUR; i < hi; i += WARP * FOUR) {
-      float x[FOUR];
-      four(i, x);
-      unsigned between = 0;
+    double x0 = 0, x1 = 0, x2 = 0;
+    const uint64_t top2 = pack2(z.top, z.top), down2 = pack2(-z.inv_fine, -z.inv_fine), zero_part = pack2(8388608.f, 8388608.f);
+    constexpr int RUN = ((1 << (64 - SA_UNITS)) - FOUR) / FOUR * WARP * FOUR;  // so many of a warp's entries leave room in its lanes' sums
+    for (int begin = lo; begin < hi; begin += RUN) {
+      u64 front = 0, behind = 0, enough_too = 0;
+      const int end = min(hi, begin + RUN);
+      for (int i = begin + lane * FOUR; i < end; i += WARP * FOUR) {
+        float x[FOUR];
+        four(i, x);
+        unsigned between = 0;
 #pragma unroll
-      for (int e = 0; e < FOUR; ++e) {
-        const float at = z.part_of(x[e]);
-        bool keep = z.counts(x[e]);
-        if (rank_bin < SA_BINS) keep = keep && (at < rank_from || (at < rank_to && place_of(order_of(x[e]), i + e) >= cut));
-        const float2 w = z.weight_pair(x[e], s.table);
-        const bool first_ones = keep && at < from, last_ones = keep && at >= to;
-        front.add(first_ones ? w : make_float2(0.f, 0.f));
-        behind.add(last_ones ? w : make_float2(0.f, 0.f));
-        if (by_min && first_ones && enough(x[e], (double)w.x + (double)w.y)) enough_too.add(w);
-        between |= (unsigned)(keep && !first_ones && !last_ones) << e;
+        for (int e = 0; e < FOUR; e += 2) {
+          const uint64_t xx = pack2(x[e], x[e + 1]), t2 = sub2(xx, top2);
+          uint64_t bits2;
+          float t[2], at[2], bits[2], q[2];
+          unpack2(z.reduced(t2, xx, bits2), q[0], q[1]);
+          unpack2(t2, t[0], t[1]);
+          unpack2(fma2(t2, down2, zero_part), at[0], at[1]);
+          unpack2(bits2, bits[0], bits[1]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            bool keep = -t[h] <= z.reach;
+            if (rank_bin < SA_BINS) keep = keep && (at[h] < rank_from || (at[h] < rank_to && place_of(order_of(x[e + h]), i + e + h) >= cut));
+            unsigned down;
+            const uint32_t m = z.mantissa(bits[h], q[h], s.table, down);
+            const u64 w = shifted((u64)m << (SA_UNITS - 30), down);
+            const bool first_ones = keep && at[h] < from, last_ones = keep && at[h] >= to;
+            if (first_ones) front += w;
+            if (last_ones) behind += w;
+            if (by_min && first_ones) {
+              const float about = (float)m * __uint_as_float((127 - 30 - down) << 23);
+              if (about >= min_high || (about >= min_low && z.exact(x[e + h]) >= min_p)) enough_too += w;
+            }
+            between |= (unsigned)(keep && !first_ones && !last_ones) << (e + h);
+          }
+        }
+        while (between) {
+          own(i + __ffs(between) - 1);
+          between &= between - 1;
+        }
       }
-      while (between) {
-        own(i + __ffs(between) - 1);
-        between &= between - 1;
-      }
+      x0 += (double)front;
+      x1 += (double)behind;
+      x2 += (double)(by_min ? enough_too : front);
     }
-    double x0 = front.value(), x1 = behind.value(), x2 = by_min ? enough_too.value() : x0;
+    constexpr double UNIT = 1.0 / (1ll << SA_UNITS);
+    x0 *= UNIT;
+    x1 *= UNIT;
+    x2 *= UNIT;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       x0 += __shfl_xor_sync(0xffffffffu, x0, o);
@@ -977,7 +1036,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     in_front = before;
   }
   if (rank != owner) return;
-  const int token = r.locate(entries, lo, hi, in_front, target, total, [&](float x, int i) -> double {
+  const int token = r.locate(entries, from, to, share, in_front, target, total, [&](float x, int i) -> double {
     if (!z.counts(x) || place_of(order_of(x), i) < cut) return 0.0;
     const double w = z.weight(x, s.table);
     return !by_min || enough(x, w) ? w : 0.0;

@@ -515,6 +515,16 @@ def test_sample_tokens_odd_entries(ops):
             check_sample(ops, logits[ordinary], u[ordinary], **settings)
 
 
+@pytest.mark.parametrize("settings", [{}, {"top_k": 30}, {"top_p": 0.7}, {"min_p": 0.5}], ids=str)
+def test_sample_tokens_at_temperatures_far_from_one(ops, settings):
+    """Next to none, of which one entry or its equals are left, and so large that all entries weigh the same."""
+    t = [1e-45, 1e-40, 1e-35, 1e-28, 1e-10, 1e4, 1e15, 1e24, 1e28, 1e38]
+    logits, u = rnd(57, len(t), 1500), torch.rand(len(t), device="cuda", generator=torch.Generator("cuda").manual_seed(9))
+    logits[::2, 700] = logits[::2, 3] = 9.0
+    check_sample(ops, logits, u, temperature=torch.tensor(t, device="cuda"), **settings)
+    check_sample(ops, logits * 1e30, u, temperature=torch.tensor(t, device="cuda"), **settings)
+
+
 def test_sample_tokens_takes_any_layout(ops):
     logits, u = rnd(54, 6, 1003), torch.rand(6, device="cuda")
     want = ops.sample_tokens(logits, u, top_p=0.9)
