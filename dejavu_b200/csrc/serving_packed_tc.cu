@@ -7,7 +7,8 @@
 //   warp 9          issues the products: S = Q K^T, O (TMEM) += P V
 //   warps 10, 11    look through the value tiles that hold keys some row does not see (the last one or two of an item)
 // With one score tile per query tile in TMEM (S 2 x 128 + O 2 x 128 columns are all there is) a tile's steps are a chain: QK, softmax, PV;
-// the two tiles' chains interleave.
+// the two tiles' chains interleave. Heads of more than 128 have one query tile (O takes 256 columns, Q 64 KB) and tiles of 64 keys, four of
+// which fit beside it: nothing runs behind the chain.
 //
 // O is only rescaled when a row's maximum grows by more than 2^8 (the division by the sum makes up for the rest), by the softmax
 // threads themselves: the barrier that says S is there also says that the product before it is complete.
@@ -18,6 +19,7 @@
 // 1.64 GHz; 24 prompts of 16384 tokens in all 0.31 ms, 0.72 PFLOP/s. A step of an item takes about 3000 cycles, the exponentials of its two
 // tiles 2048 of the special units and its products 2048 of the tensor cores. What did not pay: two threads per row, exponentials by
 // polynomials, turns between the tiles, values' products that begin with half the weights, waits that spin.
+// 16 heads over 8 of 256 dimensions: 4096 tokens 0.19 ms, 0.72 PFLOP/s (27.7 ms on the CUDA cores), 16384 tokens 2.5 ms, 0.87 PFLOP/s.
 //
 // What a row does not see must not reach it: scores are masked by comparison, but a weight of 0 times an infinity would be NaN. So
 // entries of those value tiles that are not finite are set to 0 before the products, and joined again at the end for the rows that
@@ -581,7 +583,8 @@ static bool rows_fit(const void *p, long long ld, long long hs, int heads) {
 }
 bool packed_tc_supported(int dtype, const PackedArgs &a) {
   return dtype != DJV_DTYPE_F32 && a.D % 8 == 0 && a.D <= 256 && rows_fit(a.q, a.ldq, a.hq, a.H) && rows_fit(a.k, a.ldk, a.hk, a.G) &&
-         rows_fit(a.v, a.ldv, a.hv, a.G) && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 && (long long)packed_tiles<PT_M>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
+         rows_fit(a.v, a.ldv, a.hv, a.G) && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 &&
+         (long long)packed_tiles<PT_M>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
 }
 
 template <typename T, int KB, bool FULL>

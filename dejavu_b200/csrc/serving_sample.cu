@@ -14,12 +14,14 @@
 // thousands), go to one block, which reads the row from L2 as often as it needs, narrows the range by 2048 steps of the 64-bit number at
 // a time, and has weights from exp in 64 bits: the token is that of the 64-bit definition.
 //
-// Weights: 2^(y/64) from a table of 64-bit numbers, 2^f for the rest |f| <= 1/128 by its series in 32 bits, off by 1e-9 at most; sums have 64
-// bits. (32-bit weights would leave every tenth row of a flat distribution undecided.)
+// Weights: 2^(n/256) from a table, 2^f for the rest |f| <= 1/512 by its series in 32 bits, off by 1.2e-9 at most; sums have 64 bits. (32-bit
+// weights would leave every tenth row of a flat distribution undecided.) Rows whose differences two floats do not hold (a largest entry of
+// +inf, temperatures below 1e-30 or above 1e25) are left to one block too.
 //
 // A row is read once, then swept two or three times in shared memory between block and cluster barriers. One row of 50272 entries (top-k 50,
-// top-p): 15 us, a chain of barriers and fetched code; 256 rows of settings of their own: 90 us, 32 rows of 151936 (top-p 0.9): 65 us, the
-// instructions of the weights and their sums, 45 per entry (64-bit sums: 92 and 73).
+// top-p): 14 us, a chain of barriers and fetched code; 256 rows of settings of their own: 79 us, four waves of such chains and sweeps;
+// 32 rows of 151936 (top-p 0.9): 49 us, a third of it the weights and their sums. (With pairs of floats as sums, and a warp alone
+// with the share that the token is in: 88 and 65.)
 #include <math.h>
 #include <string.h>
 
@@ -258,7 +260,7 @@ struct SampleScale {
     down = SA_ROUND / SA_TABLE - n / SA_TABLE;
     return w.x + __float_as_uint(fmaf(__uint_as_float(w.y), q, SA_MAGIC));
   }
-  __device__ __forceinline__ double weight(float x, const uint2 *table) const {
+  __device__ __forceinline__ double weight(float x, const uint2 *table) const {  // the same in 64 bits
     uint64_t bits;
     float b0, b1, q0, q1;
     const uint64_t x2 = pack2(x, x);
@@ -269,6 +271,8 @@ struct SampleScale {
     return (double)m * __longlong_as_double((long long)(1023 - 30 - down) << 52);
   }
 };
+// (where a few are made in cold code)
+__device__ __noinline__ double weight_of(const SampleScale &z, float x, const uint2 *table) { return z.weight(x, table); }
 constexpr int SA_UNITS = 52;  // sums are integers, 2^52 to the largest weight: 4096 of those fit
 __device__ __forceinline__ u64 shifted(u64 v, unsigned down) {  // (0 from 64 on)
   u64 r;
@@ -501,7 +505,7 @@ __device__ __noinline__ int sample_list(SampleShared &s, const SampleScale &z, i
   if (threadIdx.x == 0) s.found[1] = 0;
 #pragma unroll
   for (int e = 0; e < SA_EACH; ++e) {
-    w[e] = at + e < n ? z.weight(logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
+    w[e] = at + e < n ? weight_of(z, logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
     mine += w[e];
   }
   double run = block_before(mine, s.part, total);
@@ -527,7 +531,7 @@ __device__ __noinline__ int sample_list(SampleShared &s, const SampleScale &z, i
   mine = 0;
 #pragma unroll
   for (int e = 0; e < SA_EACH; ++e) {
-    w[e] = at + e < n ? z.weight(logit_of((uint32_t)s.list[at + e]), s.table) : 0.0;
+    w[e] = at + e < n ? weight_of(z, logit_of((uint32_t)s.list[at + e]), s.table) : 0.0;
     mine += w[e];
   }
   run = block_before(mine, s.part, total);
@@ -545,6 +549,67 @@ __device__ __noinline__ int sample_list(SampleShared &s, const SampleScale &z, i
   if (near) s.found[1] = 1;
   __syncthreads();
   return (int)~(uint32_t)(s.list[over] >> 32);
+}
+
+// The same for a list of up to 64 entries that is not sorted, of which the first `most` can be kept: by one warp, two entries to a lane, without
+// a barrier. -1: too close to tell.
+__device__ __noinline__ int sample_short(const SampleShared &s, const SampleScale &z, int n, int most, double behind, double p, double min_p, double u) {
+  const int lane = threadIdx.x % WARP;
+  u64 v[2];
+  for (int h = 0; h < 2; ++h) v[h] = lane + 32 * h < n ? s.list[lane + 32 * h] : 0;
+  bool near = false;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {  // the first ones first: what is kept; by index: the token
+#pragma unroll 1
+    for (int k = 2; k <= 64; k *= 2) merge_in_warp(v[0], v[1], 0, k, k / 2);
+    double w[2], upto[2], total = 0;
+    bool in[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      in[h] = v[h] != 0 && (pass || lane + 32 * h < most);
+      w[h] = in[h] ? weight_of(z, logit_of((uint32_t)(pass ? v[h] : v[h] >> 32)), s.table) : 0.0;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      double sum = w[h];
+#pragma unroll
+      for (int o = 1; o < WARP; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      upto[h] = total + sum;
+      total += __shfl_sync(0xffffffffu, sum, WARP - 1);
+    }
+    if (pass == 0) {
+      const double all = total + behind, mass = p * all;
+      double last = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const double up = __shfl_up_sync(0xffffffffu, upto[h], 1), before = lane ? up : last;
+        last = __shfl_sync(0xffffffffu, upto[h], WARP - 1);
+        if (in[h] && p < 1 && lane + h > 0) {
+          in[h] = before < mass;
+          near |= fabs(before - mass) <= SA_CLOSE * all;
+        }
+        if (in[h] && min_p > 0 && w[h] < min_p * (1 + 1e-8))
+          in[h] = w[h] >= min_p * (1 - 1e-8) && z.exact(logit_of((uint32_t)(v[h] >> 32))) >= min_p;
+        v[h] = in[h] ? v[h] << 32 | v[h] >> 32 : 0;
+      }
+    } else {
+      const double target = u * total;
+      unsigned over[2], some[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        near |= in[h] && fabs(upto[h] - target) <= SA_CLOSE * total;
+        over[h] = __ballot_sync(0xffffffffu, in[h] && upto[h] > target);
+        some[h] = __ballot_sync(0xffffffffu, in[h]);
+      }
+      const int at = over[0] ? __ffs(over[0]) - 1 : over[1] ? 31 + __ffs(over[1]) : __popc(some[0]) + __popc(some[1]) - 1;  // (rounding: the last one)
+      const u64 found = __shfl_sync(0xffffffffu, at < 32 ? v[0] : v[1], at % WARP);
+      n = (int)~(uint32_t)(found >> 32);
+    }
+  }
+  return __any_sync(0xffffffffu, near) ? -1 : n;
 }
 
 template <typename T, bool VEC>
@@ -820,6 +885,18 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   // The first block makes the rest of what it has in the list, `behind` is the weight of the others that top-p counts.
   auto finish = [&](int most, double behind) {
     const int n = s.listed;
+    if (n <= 64) {
+      if (warp == 0) {
+        const int token = sample_short(s, z, n, most, behind, p, min_p, u);
+        if (lane == 0) s.found[0] = token;
+      }
+      __syncthreads();
+      const int token = s.found[0];
+      __syncthreads();
+      if (token < 0) alone();
+      else if (tid == 0) a.token[b] = token;
+      return;
+    }
     sort_list(s.list, n);
     const int token = sample_list(s, z, min(n, most), behind, p, min_p, u);
     const bool close = s.found[1] != 0;
@@ -936,8 +1013,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
         if (can == SA_BINS - 1 && high_run >= reach_low) can = at + e;
         if (must == SA_BINS - 1 && low_run >= reach_high) must = at + e;
       }
-      can = (unsigned)block_least(can, s.wide);
-      must = (unsigned)block_least(must, s.wide);
+      const u64 both = block_all((u64)can << 32 | must, s.wide, [](u64 x, u64 y) { return min(x >> 32, y >> 32) << 32 | min((unsigned)x, (unsigned)y); });
+      can = (unsigned)(both >> 32);
+      must = (unsigned)both;
       int most = (int)s.upto[must], least = can ? (int)s.upto[can - 1] : 0;
       if (by_rank) {
         most = min(most, k);
@@ -1049,7 +1127,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
 
 // Blocks of a row: as many as are resident at once with B rows, two to a multiprocessor (clusters stay inside a group of multiprocessors, so
 // fewer of the larger ones fit), but not so few that a slice finds no room beside another one. Slices that find none are read from L2
-// in every sweep. (256 rows of 50272 entries: 88 us with four blocks per row in four waves, 134 with one block per row and L2.)
+// in every sweep. (256 rows of 50272 entries: 88 us with four blocks per row in four waves, 134 with one block per row and L2; 79 by now.)
 template <typename T>
 static cudaError_t launch_sample(const SampleArgs &a, int B, bool vec, cudaStream_t st) {
   constexpr int N = Chunk<T>::N, fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16, most = 200 * 1024, beside = 112 * 1024;
