@@ -226,7 +226,7 @@ class GenerationMixin:
         one; ranks of a tensor-parallel group have theirs seeded alike). Returns an object with
         .sequences (B, max_length) and, when asked, .scores (list of (B, vocab) logits per new token).
         prompt_chunk: the prompt runs in portions of at most that many tokens (models that take portions)."""
-        if top_k < 0 or not 0 <= top_p <= 1 or not 0 <= min_p <= 1 or not temperature >= 0:
+        if top_k != 1 and (top_k < 0 or not 0 <= top_p <= 1 or not 0 <= min_p <= 1 or not temperature >= 0):
             raise ValueError(f"top_k {top_k}, top_p {top_p}, min_p {min_p}, temperature {temperature}")
         assert prompt_chunk is None or getattr(self, "takes_portions", False), "this model takes a prompt in one piece"
         from . import ops
@@ -261,7 +261,7 @@ class GenerationMixin:
                 token = logits.argmax(dim=-1, keepdim=True)
             else:
                 token = ops.sample_tokens(logits, torch.rand(B, device=device, generator=generator), temperature, top_k, top_p or 1.0,
-                                          min_p)[:, None]
+                                          min_p).clamp_(min=0)[:, None]  # (a row of NaN goes on with token 0)
             sequences.append(token)
             if ip.sequence_len_offset >= max_length - 1:
                 break

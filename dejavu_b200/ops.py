@@ -986,7 +986,7 @@ def paged_faults() -> int:
 def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     """Causal attention over whole prompts, packed row after row (djv_packed_attention): rows cu[b] .. cu[b + 1] - 1 of q (T, H, D), k
     and v (T, G, D) are sequence b, cu_seqlens (B + 1,) int32. H a multiple of G, D at most 256; any row and head strides. Returns
-    (T, H, D). Rows of no sequence are zeros or, with `out` given (T, H, D, contiguous), left as they are."""
+    (T, H, D). Rows of no sequence are zeros or, with `out` given (T, H, D, contiguous, apart from q, k and v), left as they are."""
     device = _place(q, k, v, cu_seqlens, out)
     if device != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
@@ -1003,6 +1003,10 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     keep = out is not None
     if keep:
         assert out.shape == (T, H, D) and out.is_contiguous() and out.dtype is dtype, f"out: ({T}, {H}, {D}) {dtype}, contiguous"
+        begin, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+        for t in (q, k, v):
+            last = sum((n - 1) * step for n, step in zip(t.shape, t.stride())) + 1
+            assert T == 0 or end <= t.data_ptr() or t.data_ptr() + last * t.element_size() <= begin, "out: apart from q, k and v"
     else:
         out = q.new_empty(T, H, D)
     if T:

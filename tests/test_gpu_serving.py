@@ -655,7 +655,7 @@ def test_tensors_of_another_stream(ops):
 def test_serving_operators_refuse_what_does_not_fit(ops):
     k_pages, v_pages, table = pool([20, 20], 16, 2, 64, BF16)
     q, k, v, pos = rnd(1, 2, 4, 64, dtype=BF16), rnd(2, 2, 2, 64, dtype=BF16), rnd(3, 2, 2, 64, dtype=BF16), torch.zeros(2, dtype=torch.int64, device="cuda")
-    cu = cumulative([1, 1])
+    cu, wide = cumulative([1, 1]), rnd(4, 3, 4, 64, dtype=BF16)
     good = ops.paged_attention(q, k_pages, v_pages, table, pos - 1, 0.1)
     assert not bool(good.any())
     refused = [
@@ -683,6 +683,8 @@ def test_serving_operators_refuse_what_does_not_fit(ops):
         lambda: ops.packed_attention(q, k, v, cu, math.nan),
         lambda: ops.packed_attention(q, k, v, cu, 0.1, out=torch.empty(2, 4, 64, device="cuda")),
         lambda: ops.packed_attention(q.double(), k.double(), v.double(), cu, 0.1),
+        lambda: ops.packed_attention(q, k, v, cu, 0.1, out=q),
+        lambda: ops.packed_attention(wide[:2], k, v, cu, 0.1, out=wide[1:]),
         lambda: ops.sample_tokens(q[:, 0], torch.rand(3, device="cuda")),
         lambda: ops.sample_tokens(q[:, 0], torch.rand(2, device="cuda").double()),
         lambda: ops.sample_tokens(q[:, 0], torch.rand(2, device="cuda"), temperature=-1.0),
@@ -728,6 +730,10 @@ def test_generate_samples(ops, cg):
     for bad in ({"top_k": -1}, {"top_p": 1.5}, {"min_p": -0.1}, {"temperature": -1.0}, {"temperature": math.nan}):
         with pytest.raises(ValueError):
             model.generate(ids, **{"top_k": 0, **bad}, **kw)
+    for p in model.transformer.ln_f.parameters():
+        p.data.fill_(math.nan)
+    none = model.generate(ids, top_k=0, **kw)  # no entry to choose from
+    assert bool(none.scores[0].isnan().all()) and not bool(none.sequences[:, 7:].any())
 
 
 def test_thousands_of_short_prompts(ops):
