@@ -68,10 +68,12 @@ __device__ __forceinline__ PackedTile packed_tile(const PackedArgs &a, int index
     seen += __shfl_sync(0xffffffffu, s, WARP - 1);
   }
   const int head = max(0, min(a.cu[0], a.T)), tail = max(0, min(a.cu[a.B], a.T));
-  const int at = (index - seen) * Q;
+  const long long at = (long long)(index - seen) * Q;
   const int in_head = (head + Q - 1) / Q * Q;
-  if (at < in_head) return {0, at, min(Q, head - at), 1, -1};
-  return {tail, at - in_head, min(Q, a.T - tail - (at - in_head)), 1, -1};
+  if (at < in_head) return {0, (int)at, min(Q, head - (int)at), 1, -1};
+  const long long left = a.T - tail - (at - in_head);
+  if (left <= 0) return {0, 0, 0, 1, -1};
+  return {tail, (int)(at - in_head), left < Q ? (int)left : Q, 1, -1};
 }
 
 }  // namespace djv

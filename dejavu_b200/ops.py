@@ -879,6 +879,15 @@ def _rows(t):
     return t, (t.data_ptr(), ld, head)
 
 
+def _even(t, args):
+    """What _rows gave, or a copy: rows and heads on multiples of 16 bytes (of 16-bit elements)."""
+    at, ld, head = args
+    if at & 15 or (ld | head) & 7 or not ld or not head:
+        t = t.clone(memory_format=torch.contiguous_format)
+        return _rows(t)
+    return t, args
+
+
 def _pages(k_pages, v_pages, table, pos, dtype, G: int, D: int):
     """Checks a paged cache against what is stored in it; its arguments of the C ABI."""
     P, heads, page, dim = shape = k_pages.shape
@@ -1000,6 +1009,8 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     assert 1 <= D <= 256, f"heads of {D}"
     B = _cumulative(cu_seqlens)
     (q, q_args), (k, k_args), (v, v_args) = _rows(q), _rows(k), _rows(v)
+    if dtype is not torch.float32 and not D & 7:  # rows that TMA can read: a copy costs a tenth or less of what the CUDA cores would take more
+        (q, q_args), (k, k_args), (v, v_args) = _even(q, q_args), _even(k, k_args), _even(v, v_args)
     keep = out is not None
     if keep:
         assert out.shape == (T, H, D) and out.is_contiguous() and out.dtype is dtype, f"out: ({T}, {H}, {D}) {dtype}, contiguous"
