@@ -1,19 +1,23 @@
 // Causal attention over packed prompts on the CUDA cores, whatever the element type, strides and alignment.
 //
-// A block takes 64 queries of one head and walks the key tiles of 32 up to its last query; a thread keeps 4 rows x 4 keys of the scores
-// and 4 rows x D / 8 columns of the sums in registers, everything in fp32.
+// A block takes 128 queries of one head and walks the key tiles of 64 up to its last query; a thread keeps 8 rows x 4 keys of the scores
+// and 8 rows x D / 16 columns of the sums in registers, everything in fp32. What bounds it are the loads of operands from shared memory,
+// 12 of 16 bytes for 64 instructions of two products each in the scores. fp32, one prompt of 4096 tokens, 16 heads over 8: heads of
+// 64 1.26 ms, of 128 2.6 ms (27 TFLOP/s), of 256 5.5 ms (25; library products of whole score matrices take 5.0). With 64 queries, 4 rows and a key
+// tile of 32: 2.6, 4.8 and 22.6 ms.
 #include "pairs.cuh"
 #include "serving_packed.cuh"
 
 namespace djv {
 
-constexpr int PS_Q = 128, PS_THREADS = 256, PS_ROWS = 8;  // queries of a block; rows of a thread
+constexpr int PS_Q = 128, PS_KEYS = 64, PS_THREADS = 256, PS_ROWS = 8;  // queries of a block, keys of a tile; rows of a thread
 
 template <typename T, int DP>  // DP: D rounded up
 __global__ void __launch_bounds__(PS_THREADS) packed_simple_kernel(PackedArgs a) {
   extern __shared__ __align__(16) float smem[];
-  constexpr int KEYS = DP > 128 ? 32 : 64, LD = DP + 4, LP = KEYS + 4, J = KEYS / 16, N = DP / 64;
-  float *sq = smem, *sk = sq + PS_Q * LD, *sv = sk + KEYS * LD, *sp = sv + KEYS * LD;  // sp (128, LP)
+  // Key and value tiles are staged by up to 128 columns at a time; where that is all there are, both at once.
+  constexpr int KEYS = PS_KEYS, COLS = DP < 128 ? DP : 128, PARTS = DP / COLS, LD = DP + 4, LK = COLS + 4, LP = KEYS + 4, J = KEYS / 16, N = DP / 64;
+  float *sq = smem, *sk = sq + PS_Q * LD, *sv = PARTS > 1 ? sk : sk + KEYS * LK, *sp = sv + KEYS * LK;  // sp (128, LP)
   __shared__ PackedTile tile;
   pdl_prologue();
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16, h = blockIdx.y, g = h / (a.H / a.G);
@@ -49,27 +53,37 @@ __global__ void __launch_bounds__(PS_THREADS) packed_simple_kernel(PackedArgs a)
     for (int n = 0; n < 2 * N; ++n) o[i][n] = 0;
   }
   const int end = w.q0 + w.rows, depth = (a.D + 3) / 4 * 4;  // keys that the last query sees
+  auto stage = [&](float *to, const T *from, long long ld, int j0, int part) {
+    constexpr int EACH = KEYS * COLS / PS_THREADS, STEP = PS_THREADS / COLS;  // a thread's column, and rows; all of its loads are on their way at once
+    const int r0 = tid / COLS, c = tid % COLS, d = c + part * COLS;
+    const T *at = from + (j0 + r0) * ld + d;
+    T x[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) x[i] = j0 + r0 + i * STEP < end && d < a.D ? at[i * STEP * ld] : from_f<T>(0.f);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) to[(r0 + i * STEP) * LK + c] = to_f(x[i]);
+  };
   for (int j0 = 0; j0 < end; j0 += KEYS) {
-    __syncthreads();
-#pragma unroll 8
-    for (int i = tid; i < KEYS * DP; i += PS_THREADS) {
-      const int r = i / DP, d = i % DP;
-      const bool ok = j0 + r < end && d < a.D;
-      sk[r * LD + d] = ok ? to_f(k[(j0 + r) * a.ldk + d]) : 0.f;
-      sv[r * LD + d] = ok ? to_f(v[(j0 + r) * a.ldv + d]) : 0.f;
-    }
-    __syncthreads();
     uint64_t s2[PS_ROWS][J] = {};
+#pragma unroll 1
+    for (int part = 0; part < PARTS; ++part) {
+      __syncthreads();
+      stage(sk, k, a.ldk, j0, part);
+      if (PARTS == 1) stage(sv, v, a.ldv, j0, 0);
+      __syncthreads();
+      const float *x0 = sq + ty * PS_ROWS * LD + part * COLS;
+      const int limit = min(COLS, depth - part * COLS);
 #pragma unroll 2
-    for (int d = 0; d < depth; d += 4) {
-      ulonglong2 y[J];
+      for (int d = 0; d < limit; d += 4) {
+        ulonglong2 y[J];
 #pragma unroll
-      for (int j = 0; j < J; ++j) y[j] = *reinterpret_cast<const ulonglong2 *>(sk + (tx + j * 16) * LD + d);
+        for (int j = 0; j < J; ++j) y[j] = *reinterpret_cast<const ulonglong2 *>(sk + (tx + j * 16) * LK + d);
 #pragma unroll
-      for (int i = 0; i < PS_ROWS; ++i) {
-        const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(sq + (ty * PS_ROWS + i) * LD + d);
+        for (int i = 0; i < PS_ROWS; ++i) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(x0 + i * LD + d);
 #pragma unroll
-        for (int j = 0; j < J; ++j) s2[i][j] = fma2(x.y, y[j].y, fma2(x.x, y[j].x, s2[i][j]));
+          for (int j = 0; j < J; ++j) s2[i][j] = fma2(x.y, y[j].y, fma2(x.x, y[j].x, s2[i][j]));
+        }
       }
     }
 #pragma unroll
@@ -99,32 +113,51 @@ __global__ void __launch_bounds__(PS_THREADS) packed_simple_kernel(PackedArgs a)
       for (int n = 0; n < 2 * N; ++n) o[i][n] = fma2(o[i][n], corr2, 0);
     }
     __syncwarp();  // (a row's weights are made and read by one warp)
-    auto add = [&](int i, int c, float p) {
-      const uint64_t p2 = pack2(p, p);
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(sv + c * LD + n * 64 + tx * 4);
-        o[i][2 * n] = fma2(p2, y.x, o[i][2 * n]);
-        o[i][2 * n + 1] = fma2(p2, y.y, o[i][2 * n + 1]);
+    for (int part = 0; part < PARTS; ++part) {
+      if (PARTS > 1) {
+        if (part * COLS >= a.D) break;
+        __syncthreads();
+        stage(sv, v, a.ldv, j0, part);
+        __syncthreads();
       }
-    };
-    if (j0 + KEYS - 1 <= w.q0 + ty * PS_ROWS) {
+      auto row = [&](int c, ulonglong2(&y)[COLS / 64]) {
+#pragma unroll
+        for (int n = 0; n < COLS / 64; ++n) y[n] = *reinterpret_cast<const ulonglong2 *>(sv + c * LK + n * 64 + tx * 4);
+      };
+      auto add = [&](int i, float p, const ulonglong2(&y)[COLS / 64]) {
+        const uint64_t p2 = pack2(p, p);
+#pragma unroll
+        for (int n = 0; n < COLS / 64; ++n) {
+          uint64_t *to = o[i] + 2 * (part * (COLS / 64) + n);
+          to[0] = fma2(p2, y[n].x, to[0]);
+          to[1] = fma2(p2, y[n].y, to[1]);
+        }
+      };
+      const int own = w.q0 + ty * PS_ROWS - j0;  // the key that the thread's first row sees last
+      ulonglong2 y[COLS / 64];
+      if (own >= KEYS - 1) {
 #pragma unroll 1
-      for (int c = 0; c < KEYS; c += 4) {
-        float p[PS_ROWS][4];
+        for (int c = 0; c < KEYS; c += 4) {
+          float p[PS_ROWS][4];
 #pragma unroll
-        for (int i = 0; i < PS_ROWS; ++i) *reinterpret_cast<float4 *>(p[i]) = *reinterpret_cast<const float4 *>(sp + (ty * PS_ROWS + i) * LP + c);
+          for (int i = 0; i < PS_ROWS; ++i) *reinterpret_cast<float4 *>(p[i]) = *reinterpret_cast<const float4 *>(sp + (ty * PS_ROWS + i) * LP + c);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+          for (int e = 0; e < 4; ++e) {
+            row(c + e, y);
 #pragma unroll
-          for (int i = 0; i < PS_ROWS; ++i) add(i, c + e, p[i][e]);
+            for (int i = 0; i < PS_ROWS; ++i) add(i, p[i][e], y);
+          }
+        }
+      } else {  // a key that a row does not see weighs nothing, whatever its value is
+#pragma unroll 1
+        for (int c = 0; c < min(KEYS, own + PS_ROWS); ++c) {
+          row(c, y);
+#pragma unroll
+          for (int i = 0; i < PS_ROWS; ++i)
+            if (c <= own + i) add(i, sp[(ty * PS_ROWS + i) * LP + c], y);
+        }
       }
-    } else {  // a key that a row does not see weighs nothing, whatever its value is
-#pragma unroll 1
-      for (int c = 0; c < KEYS; ++c)
-#pragma unroll
-        for (int i = 0; i < PS_ROWS; ++i)
-          if (j0 + c <= w.q0 + ty * PS_ROWS + i) add(i, c, sp[(ty * PS_ROWS + i) * LP + c]);
     }
   }
 #pragma unroll
@@ -147,7 +180,7 @@ __global__ void __launch_bounds__(PS_THREADS) packed_simple_kernel(PackedArgs a)
 
 template <typename T, int DP>
 static cudaError_t launch_packed_simple(const PackedArgs &a, cudaStream_t st) {
-  constexpr int keys = DP > 128 ? 32 : 64, smem = ((PS_Q + 2 * keys) * (DP + 4) + PS_Q * (keys + 4)) * 4;
+  constexpr int smem = (PS_Q * (DP + 4) + (DP > 128 ? 1 : 2) * PS_KEYS * ((DP < 128 ? DP : 128) + 4) + PS_Q * (PS_KEYS + 4)) * 4;
   static DevicePrep prep;
   const int(*unused)[4];
   cudaError_t e = prep.get(
