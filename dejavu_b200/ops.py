@@ -879,13 +879,9 @@ def _rows(t):
     return t, (t.data_ptr(), ld, head)
 
 
-def _even(t, args):
-    """What _rows gave, or a copy: rows and heads on multiples of 16 bytes (of 16-bit elements)."""
-    at, ld, head = args
-    if at & 15 or (ld | head) & 7 or not ld or not head:
-        t = t.clone(memory_format=torch.contiguous_format)
-        return _rows(t)
-    return t, args
+def _even(at: int, ld: int, head: int) -> bool:
+    """Whether rows and heads of 16-bit elements are apart and start on multiples of 16 bytes."""
+    return not (at & 15 or (ld | head) & 7) and ld > 0 and head > 0
 
 
 def _pages(k_pages, v_pages, table, pos, dtype, G: int, D: int):
@@ -1010,7 +1006,8 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     B = _cumulative(cu_seqlens)
     (q, q_args), (k, k_args), (v, v_args) = _rows(q), _rows(k), _rows(v)
     if dtype is not torch.float32 and not D & 7:  # rows that TMA can read: a copy costs a tenth or less of what the CUDA cores would take more
-        (q, q_args), (k, k_args), (v, v_args) = _even(q, q_args), _even(k, k_args), _even(v, v_args)
+        (q, q_args), (k, k_args), (v, v_args) = (x if _even(*x[1]) else _rows(x[0].clone(memory_format=torch.contiguous_format))
+                                                 for x in ((q, q_args), (k, k_args), (v, v_args)))
     keep = out is not None
     if keep:
         assert out.shape == (T, H, D) and out.is_contiguous() and out.dtype is dtype, f"out: ({T}, {H}, {D}) {dtype}, contiguous"

@@ -539,6 +539,19 @@ def test_sample_tokens_takes_any_layout(ops):
     assert ops.sample_tokens(logits[:0], u[:0]).shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_sample_tokens_of_millions(ops, dtype):
+    """Rows too long for the blocks' memory, and for one sum of a thread: equal entries, so that the token is known."""
+    V, first = 2 ** 25, 2 ** 22
+    logits = torch.full((1, V), 1.5, dtype=dtype, device="cuda")
+    for x in (0.0, 0.3, 0.77, 1 - 2.0 ** -24):
+        u = torch.full((1,), x, device="cuda")
+        assert int(ops.sample_tokens(logits, u)) == int(float(u) * V)
+        logits[:, :first] = -math.inf
+        assert int(ops.sample_tokens(logits, u, min_p=0.5)) == first + int(float(u) * (V - first))
+        logits[:, :first] = 1.5
+
+
 def test_sample_tokens_next_to_borders(ops):
     """Numbers next to the borders between tokens, where 32-bit weights cannot tell: the token of the 64-bit sums."""
     V, B = 4000, 256
