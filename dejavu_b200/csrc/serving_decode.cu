@@ -12,11 +12,12 @@
 // item to item, so that the next one's rows are on their way while one ends, and the page of a tile is
 // looked up a tile ahead. fp16 and bf16 go through mma.sync, 16 query heads x 16 tokens: tcgen05 would have to pad the heads to
 // 64 or 128 rows, and the tensor work is a small part of the time either way. The weights enter the second product as two terms
-// of the cache's type, hi + lo, so that they keep 16 (bf16) or 22 bits. fp32 goes through the CUDA cores, 4 heads at a time.
+// of the cache's type, hi + lo, so that they keep 16 (bf16) or 22 bits. fp32 goes through the CUDA cores, 4 heads and 8 or 16 tokens at a time.
 //
 // Measured (bf16, pages of 16, 32 query heads over 8 of 128 dimensions): one cache of 131071 tokens 94 us, 5.7 TB/s; 64 of up to 8192 tokens 168 us,
 // 6.0 TB/s; 16 of 32 heads, fp16, up to 2048 tokens 49 us, 5.2 TB/s (101 before an item's beginning and end counted as units); 137
-// tokens of 12 heads of 64 5.4 us in a graph.
+// tokens of 12 heads of 64 5.4 us in a graph. fp32, 16 caches of up to 4000 tokens, 32 heads over 8 of 128: 67 us where HBM alone would take 50 (96
+// with queries from L1, branches for the rows and 16 tokens).
 #include <math.h>
 #include <type_traits>
 
@@ -302,74 +303,126 @@ struct DecodeSums<bf16, DP> : MmaSums<bf16, DP> {};
 template <int DP>
 struct DecodeSums<__half, DP> : MmaSums<__half, DP> {};
 
-// fp32: for the scores a lane has a token and every PARTS-th chunk of it, for the values DP / 32 dimensions
+// fp32: for the scores a lane has a token and every PARTS-th chunk of it (of wide heads two tokens, one after the other), so that its share of
+// the queries takes 128 registers; for the values it has DP / 32 adjacent dimensions (or two times four). Products go two to an instruction.
 template <int DP>
 struct DecodeSums<float, DP> {
-  static constexpr int TOKENS = DP > 128 ? 8 : 16, PARTS = WARP / TOKENS, W = DP / 32;
-  const float *query;
-  long long hq;
+  static constexpr int TOKENS = DP > 64 ? 8 : 16, TURNS = DP > 128 ? 2 : 1, AT_ONCE = TOKENS / TURNS, PARTS = WARP / AT_ONCE, W = DP / 32,
+                       EACH = DP / 4 / PARTS;  // EACH: chunks of a lane
   int rows;
-  float o[4][W], m[4], l[4];
+  ulonglong2 q[EACH][4];
+  float m[4], l[4];
+  union {
+    uint64_t o2[4][W / 2];
+    float o[4][W];
+  };
 
-  __device__ __forceinline__ void start(const float *q, long long h, int n, int) {
-    query = q;
-    hq = h;
+  // the dimension of a lane's i-th sum
+  __device__ __forceinline__ static int dim(int i) {
+    const int lane = threadIdx.x % WARP;
+    return W <= 4 ? lane * W + i : i / 4 * 128 + lane * 4 + i % 4;
+  }
+  // a lane's i-th chunk (eight lanes that read at once have eight different columns of the swizzle)
+  __device__ __forceinline__ static int chunk(int i) {
+    const int part = threadIdx.x % WARP / AT_ONCE;
+    return TURNS == 1 ? i * PARTS + part : i * PARTS + part / 2 + part % 2 * 4;
+  }
+  __device__ __forceinline__ void start(const float *first, long long h, int n, int D) {
     rows = n;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       m[r] = -INFINITY;
       l[r] = 0.f;
 #pragma unroll
-      for (int i = 0; i < W; ++i) o[r][i] = 0.f;
+      for (int i = 0; i < W / 2; ++i) o2[r][i] = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+        q[i][r] = r < rows && chunk(i) * 4 < D ? __ldg(reinterpret_cast<const ulonglong2 *>(first + r * h + chunk(i) * 4)) : make_ulonglong2(0, 0);
     }
   }
-  __device__ __forceinline__ static float4 at(uint32_t sm) {
-    float4 v;
-    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(sm) : "memory");
+  __device__ __forceinline__ static ulonglong2 at(uint32_t sm) {
+    ulonglong2 v;
+    asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(sm) : "memory");
     return v;
   }
-  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c, int D) {
-    const int lane = threadIdx.x % WARP, token = lane % TOKENS, part = lane / TOKENS;
-    float s[4] = {};
-#pragma unroll 4
-    for (int i = 0; i < DP / 4 / PARTS; ++i) {
-      const int ch = i * PARTS + part;
-      const float4 k = at(k_sm + tile_offset<TOKENS>(token, ch));
+  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c, int) {
+    if (rows == 1) tile_of<1>(k_sm, v_sm, seen, c);
+    else if (rows == 2) tile_of<2>(k_sm, v_sm, seen, c);
+    else tile_of<4>(k_sm, v_sm, seen, c);
+  }
+  template <int R>  // rows (of four the last may be zeros): no branches, so that their chains overlap
+  __device__ __forceinline__ void tile_of(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c) {
+    const int lane = threadIdx.x % WARP, mine = lane % AT_ONCE;
+    float s[TURNS][R];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float4 q = r < rows && ch * 4 < D ? __ldg(reinterpret_cast<const float4 *>(query + r * hq + ch * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        s[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[r]))));
+    for (int n = 0; n < TURNS; ++n) {
+      uint64_t s2[R] = {};
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const ulonglong2 k = at(k_sm + tile_offset<TOKENS>(n * AT_ONCE + mine, chunk(i)));
+#pragma unroll
+        for (int r = 0; r < R; ++r) s2[r] = fma2(q[i][r].y, k.y, fma2(q[i][r].x, k.x, s2[r]));
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float x, y;
+        unpack2(s2[r], x, y);
+        s[n][r] = x + y;
+      }
+    }
+    float top[R];
+#pragma unroll
+    for (int x = AT_ONCE; x < WARP; x <<= 1)
+#pragma unroll
+      for (int n = 0; n < TURNS; ++n)
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[n][r] += __shfl_xor_sync(0xffffffffu, s[n][r], x);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      top[r] = m[r];
+#pragma unroll
+      for (int n = 0; n < TURNS; ++n) {
+        s[n][r] = (seen >> (n * AT_ONCE + mine)) & 1 ? s[n][r] * c : -INFINITY;
+        top[r] = fmaxf(top[r], s[n][r]);
       }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (r >= rows) break;
+    for (int x = AT_ONCE / 2; x > 0; x >>= 1)
 #pragma unroll
-      for (int x = TOKENS; x < WARP; x <<= 1) s[r] += __shfl_xor_sync(0xffffffffu, s[r], x);
-      s[r] = (seen >> token) & 1 ? s[r] * c : -INFINITY;
-      float top = s[r];
+      for (int r = 0; r < R; ++r) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], x));
 #pragma unroll
-      for (int x = TOKENS / 2; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      top = fmaxf(top, m[r]);
-      const float base = top == -INFINITY ? 0.f : top, corr = exp2f(m[r] - base);
-      m[r] = top;
-      s[r] = exp2f(s[r] - base);
-      l[r] = l[r] * corr + (part == 0 ? s[r] : 0.f);
+    for (int r = 0; r < R; ++r) {
+      const float base = top[r] == -INFINITY ? 0.f : top[r], corr = exp2f(m[r] - base);
+      m[r] = top[r];
+      l[r] *= corr;
 #pragma unroll
-      for (int i = 0; i < W; ++i) o[r][i] *= corr;
+      for (int n = 0; n < TURNS; ++n) {
+        s[n][r] = exp2f(s[n][r] - base);
+        if (lane < AT_ONCE) l[r] += s[n][r];
+      }
+      const uint64_t corr2 = pack2(corr, corr);
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) o2[r][i] = fma2(o2[r][i], corr2, 0);
     }
 #pragma unroll
     for (int t = 0; t < TOKENS; ++t) {
-      float p[4];
+      uint64_t v[W / 2];
+      if (W == 2) {
+        asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v[0]) : "r"(v_sm + tile_offset<TOKENS>(t, lane / 2) + lane % 2 * 8) : "memory");
+      } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) p[r] = __shfl_sync(0xffffffffu, s[r], t);
+        for (int i = 0; i < W / 4; ++i) {
+          const ulonglong2 x = at(v_sm + tile_offset<TOKENS>(t, i * WARP + lane));
+          v[2 * i % (W / 2)] = x.x;
+          v[(2 * i + 1) % (W / 2)] = x.y;
+        }
+      }
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        float v;
-        const int d = i * WARP + lane;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(v_sm + tile_offset<TOKENS>(t, d / 4) + (d % 4) * 4) : "memory");
+      for (int r = 0; r < R; ++r) {
+        const float p = __shfl_sync(0xffffffffu, s[t / AT_ONCE][r], t % AT_ONCE);
+        const uint64_t p2 = pack2(p, p);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[r][i] = fmaf(p[r], v, o[r][i]);
+        for (int i = 0; i < W / 2; ++i) o2[r][i] = fma2(p2, v[i], o2[r][i]);
       }
     }
   }
@@ -384,7 +437,7 @@ struct DecodeSums<float, DP> {
       m[r] = top;
       l[r] = l[r] * mine + sl[r] * its;
 #pragma unroll
-      for (int i = 0; i < W; ++i) o[r][i] = o[r][i] * mine + sums[r * DP + i * WARP + threadIdx.x % WARP] * its;
+      for (int i = 0; i < W; ++i) o[r][i] = o[r][i] * mine + sums[r * DP + i * WARP + threadIdx.x % WARP] * its;  // (any order, as store has it)
     }
   }
   __device__ __forceinline__ void emit(float *out, float *slot, int n, int D) const {
@@ -395,7 +448,7 @@ struct DecodeSums<float, DP> {
       const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        const int d = i * WARP + lane;
+        const int d = dim(i);
         if (d >= D) continue;
         if (slot == nullptr) out[r * D + d] = o[r][i] * inv;
         else slot[r * DP + d] = o[r][i];
