@@ -722,7 +722,7 @@ __global__ void __launch_bounds__(DE_THREADS) decode_join_kernel(DecodeArgs a, i
   const int lane = threadIdx.x % WARP, warp = threadIdx.x / WARP;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   long long per;
-  const int share = a.G * a.groups, R = a.H / a.G;
+  const int R = a.H / a.G;
   // (positions and their like are those the first kernel worked with: it let this one start when they were complete)
   const DecodePlace w = decode_locate(a, [&](long long total) {
     per = units_per_block(total, blocks, least);
