@@ -1006,8 +1006,12 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     B = _cumulative(cu_seqlens)
     (q, q_args), (k, k_args), (v, v_args) = _rows(q), _rows(k), _rows(v)
     if dtype is not torch.float32 and not D & 7:  # rows that TMA can read: a copy costs a tenth or less of what the CUDA cores would take more
-        (q, q_args), (k, k_args), (v, v_args) = (x if _even(*x[1]) else _rows(x[0].clone(memory_format=torch.contiguous_format))
-                                                 for x in ((q, q_args), (k, k_args), (v, v_args)))
+        if not _even(*q_args):
+            q, q_args = _rows(q.clone(memory_format=torch.contiguous_format))
+        if not _even(*k_args):
+            k, k_args = _rows(k.clone(memory_format=torch.contiguous_format))
+        if not _even(*v_args):
+            v, v_args = _rows(v.clone(memory_format=torch.contiguous_format))
     keep = out is not None
     if keep:
         assert out.shape == (T, H, D) and out.is_contiguous() and out.dtype is dtype, f"out: ({T}, {H}, {D}) {dtype}, contiguous"
