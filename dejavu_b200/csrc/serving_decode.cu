@@ -12,7 +12,9 @@
 // item to item, so that the next one's rows are on their way while one ends, and the page of a tile is
 // looked up a tile ahead. fp16 and bf16 go through mma.sync, 16 query heads x 16 tokens: tcgen05 would have to pad the heads to
 // 64 or 128 rows, and the tensor work is a small part of the time either way. The weights enter the second product as two terms
-// of the cache's type, hi + lo, so that they keep 16 (bf16) or 22 bits. fp32 goes through the CUDA cores, 4 heads and 8 or 16 tokens at a time.
+// of the cache's type, hi + lo, so that they keep 16 bits (bf16), or 22 (fp16) down to 2^-18 of the largest and 2^-40 of that below: fp16
+// ends at 2^-24, so its weights are 2^15 times as large, and so are their sums. fp32 goes through the CUDA cores, 4 heads and 8 or 16
+// tokens at a time.
 //
 // Measured (bf16, pages of 16, 32 query heads over 8 of 128 dimensions): one cache of 131071 tokens 94 us, 5.7 TB/s; 64 of up to 8192 tokens 168 us,
 // 6.0 TB/s; 16 of 32 heads, fp16, up to 2048 tokens 49 us, 5.2 TB/s (101 before an item's beginning and end counted as units); 137
@@ -152,6 +154,7 @@ __device__ __forceinline__ float2 floats_of<__half>(uint32_t u) { return h2f(u);
 template <typename T, int DP>
 struct MmaSums {
   static constexpr int TOKENS = 16;
+  static constexpr float LIFT = std::is_same<T, __half>::value ? 15.f : 0.f;  // weights and sums are 2^LIFT times what they stand for
   uint32_t q[DP / 16][4];
   float o[DP / 8][4], m[2], l[2];
   uint32_t k_at[4], v_at[4];  // where the lane's rows and chunks of the operands are, in a 128-byte block of a tile
@@ -206,13 +209,13 @@ struct MmaSums {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       top = fmaxf(top, m[r]);
-      const float base = top == -INFINITY ? 0.f : top;
+      const float base = top == -INFINITY ? 0.f : top, low = base - LIFT;
       corr[r] = exp2_approx(m[r] - base);
       m[r] = top;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 2 * r; e < 2 * r + 2; ++e) s[n][e] = exp2_approx(s[n][e] - base);
+        for (int e = 2 * r; e < 2 * r + 2; ++e) s[n][e] = exp2_approx(s[n][e] - low);
       l[r] = l[r] * corr[r] + ((s[0][2 * r] + s[0][2 * r + 1]) + (s[1][2 * r] + s[1][2 * r + 1]));
     }
     if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
