@@ -11,7 +11,9 @@
 // which fit beside it: nothing runs behind the chain.
 //
 // O is only rescaled when a row's maximum grows by more than 2^8 (the division by the sum makes up for the rest), by the softmax
-// threads themselves: the barrier that says S is there also says that the product before it is complete.
+// threads themselves: the barrier that says S is there also says that the product before it is complete. fp16 ends at 2^-24 and goes up to
+// 2^16, so its weights, up to 2^8, are made 2^7 times as large, and so are their sums: from 2^-21 of the largest on they have all their
+// bits, below that they are off by 2^-32 of the largest at most.
 //
 // Items go out in the order of falling work, back and forth over the blocks; sequences may have any lengths.
 //
@@ -120,6 +122,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __shared__ int4 mine[PT_ROUNDS];    // the block's items: the sequence's first row, first query in it, queries, head
   __shared__ int odd[2][2][2];  // by the item's parity: what each of the two warps found in each of the two value tiles
   constexpr uint32_t Q_TILE = KB * PT_M * 128, TILE = KB * KN * 128, O_AT = NT * KN;  // bytes; columns of TMEM in front of O
+  constexpr float LIFT = __is_same(T, bf16) ? 0.f : 7.f;  // weights and sums are 2^LIFT times what they stand for
   constexpr int PT_Q = NT * PT_M;
   const int tid = threadIdx.x, warp = tid / WARP, lane = tid % WARP;
   unsigned char *base = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -300,7 +303,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
           }
         }
-        const uint64_t nm2 = pack2(-m, -m);
+        const uint64_t nm2 = pack2(LIFT - m, LIFT - m);
         uint64_t l2[2] = {0, 0};
 #pragma unroll
         for (int q = 0; q < KN / 32; ++q) {

@@ -39,3 +39,18 @@ def test_paged_attention_of_weak_keys(ops, dtype, n, batch, gap):
         tiny = 2.0 ** -40 * v[:, 0].double().sum(0) if dtype is F16 else 0.0
         ok, why = S.within(got, want.expand(batch, 1, 64), slack + tiny, dtype)
         assert ok, (at, why)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("gap", [12.0, 14.0, 16.0, 18.0])
+def test_packed_attention_of_weak_keys(ops, dtype, gap):
+    n = 16001
+    for at in (0, 700):
+        q, k, v = one_ahead(n, at, gap, dtype)
+        got = ops.packed_attention(q, k, v, cumulative([n]), 1.0)
+        for r in (129, 699, 700, 2500, 8191, n - 1):
+            want, slack = S.attend(q[r], k[:r + 1, 0], v[:r + 1, 0], 1.0, weight_step=S.half_step(dtype))
+            # fp16 weights of less than 2^-21 of the largest: half of the smallest step, 2^-24, of numbers that go up to 2^7
+            tiny = 2.0 ** -32 * v[:r + 1, 0].double().sum(0) if dtype is F16 else 0.0
+            ok, why = S.within(got[r], want, slack + tiny, dtype)
+            assert ok, (at, r, why)
