@@ -16,6 +16,11 @@
 // ends at 2^-24, so its weights are 2^15 times as large, and so are their sums. fp32 goes through the CUDA cores, 4 heads and 8 or 16
 // tokens at a time.
 //
+// A value that is not finite and is seen makes its dimension so: hi is rounded towards 0, so that lo is not negative, and neither is 0
+// where it stands for something (0 times an infinity is NaN). In fp16 that holds however small the weight is, in bf16 and fp32 for weights
+// of 2^-126 of the largest and more, which is what 32 bits hold. (A look at the sums at the end of an item costs 2 us of 49 with short
+// items: code that is fetched once.)
+//
 // Measured (bf16, pages of 16, 32 query heads over 8 of 128 dimensions): one cache of 131071 tokens 94 us, 5.7 TB/s; 64 of up to 8192 tokens 168 us,
 // 6.0 TB/s; 16 of 32 heads, fp16, up to 2048 tokens 49 us, 5.2 TB/s (101 before an item's beginning and end counted as units); 137
 // tokens of 12 heads of 64 5.4 us in a graph. fp32, 16 caches of up to 4000 tokens, 32 heads over 8 of 128: 67 us where HBM alone would take 50 (96
@@ -143,6 +148,34 @@ __device__ __forceinline__ uint32_t pair_of<__half>(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t *>(&h);
 }
+// rounded towards 0
+template <typename T>
+__device__ __forceinline__ uint32_t pair_below(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pair_below<bf16>(float lo, float hi) {
+  uint32_t v;
+  asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
+}
+template <>
+__device__ __forceinline__ uint32_t pair_below<__half>(float lo, float hi) {
+  uint32_t v;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+  return v;
+}
+// the smallest number above 0 where it is less
+template <typename T>
+__device__ __forceinline__ uint32_t above_zero(uint32_t v);
+template <>
+__device__ __forceinline__ uint32_t above_zero<bf16>(uint32_t v) {
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(0x00010001u));
+  return v;
+}
+template <>
+__device__ __forceinline__ uint32_t above_zero<__half>(uint32_t v) {
+  asm("max.f16x2 %0, %0, %1;" : "+r"(v) : "r"(0x00010001u));
+  return v;
+}
 template <typename T>
 __device__ __forceinline__ float2 floats_of(uint32_t u);
 template <>
@@ -155,6 +188,8 @@ template <typename T, int DP>
 struct MmaSums {
   static constexpr int TOKENS = 16;
   static constexpr float LIFT = std::is_same<T, __half>::value ? 15.f : 0.f;  // weights and sums are 2^LIFT times what they stand for
+  // what sums of lower maxima are scaled by: not 0 in fp16, whose sums stay below 2^80
+  __device__ __forceinline__ static float factor(float f) { return LIFT > 0 ? fmaxf(f, 1.17549435e-38f) : f; }
   uint32_t q[DP / 16][4];
   float o[DP / 8][4], m[2], l[2];
   uint32_t k_at[4], v_at[4];  // where the lane's rows and chunks of the operands are, in a 128-byte block of a tile
@@ -210,7 +245,7 @@ struct MmaSums {
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       top = fmaxf(top, m[r]);
       const float base = top == -INFINITY ? 0.f : top, low = base - LIFT;
-      corr[r] = exp2_approx(m[r] - base);
+      corr[r] = factor(exp2_approx(m[r] - base));
       m[r] = top;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -228,9 +263,10 @@ struct MmaSums {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float x = s[e >> 1][(e & 1) * 2], y = s[e >> 1][(e & 1) * 2 + 1];
-      hi[e] = pair_of<T>(x, y);
+      hi[e] = pair_below<T>(x, y);
+      if (LIFT > 0) hi[e] = above_zero<T>(hi[e]);  // (values behind the last token are zeros)
       const float2 h = floats_of<T>(hi[e]);
-      lo[e] = pair_of<T>(x - h.x, y - h.y);
+      lo[e] = above_zero<T>(pair_of<T>(x - h.x, y - h.y));
     }
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
@@ -255,7 +291,7 @@ struct MmaSums {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const float other = sm[g + r * 8], top = fmaxf(m[r], other), base = top == -INFINITY ? 0.f : top;
-      const float mine = exp2_approx(m[r] - base), its = exp2_approx(other - base);
+      const float mine = factor(exp2_approx(m[r] - base)), its = factor(exp2_approx(other - base));
       m[r] = top;
       l[r] = l[r] * mine + sl[g + r * 8] * its;
 #pragma unroll
@@ -713,6 +749,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   }
 }
 
+// A sum times a factor from 0 to 1; an infinite one stays, whatever the factor has been rounded to.
+__device__ __forceinline__ float scaled(float y, float f) { return fabsf(y) == INFINITY ? y : y * f; }
+
 // Joins the parts of the item that begins in block blockIdx.x of `blocks` and ends in a later one, if there is one: row blockIdx.y, the
 // parts dealt out to the warps, four dimensions to a lane.
 template <typename T, int DP>
@@ -770,14 +809,14 @@ __global__ void __launch_bounds__(DE_THREADS) decode_join_kernel(DecodeArgs a, i
     m = top;
     l *= corr;
 #pragma unroll
-    for (int z = 0; z < WIDE; ++z) o[z] = make_float4(o[z].x * corr, o[z].y * corr, o[z].z * corr, o[z].w * corr);
+    for (int z = 0; z < WIDE; ++z) o[z] = make_float4(scaled(o[z].x, corr), scaled(o[z].y, corr), scaled(o[z].z, corr), scaled(o[z].w, corr));
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const float f = exp2f(pm[x] - base);
       l = fmaf(pl[x], f, l);
 #pragma unroll
       for (int z = 0; z < WIDE; ++z)
-        o[z] = make_float4(fmaf(y[x][z].x, f, o[z].x), fmaf(y[x][z].y, f, o[z].y), fmaf(y[x][z].z, f, o[z].z), fmaf(y[x][z].w, f, o[z].w));
+        o[z] = make_float4(o[z].x + scaled(y[x][z].x, f), o[z].y + scaled(y[x][z].y, f), o[z].z + scaled(y[x][z].z, f), o[z].w + scaled(y[x][z].w, f));
     }
   }
 #pragma unroll
@@ -798,7 +837,7 @@ __global__ void __launch_bounds__(DE_THREADS) decode_join_kernel(DecodeArgs a, i
     for (int x = 0; x < DE_WARPS; ++x) {
       const float f = exp2f(sm[x] - base);
       sum = fmaf(sl[x], f, sum);
-      y = fmaf(reinterpret_cast<const float *>(so[x])[d], f, y);
+      y += scaled(reinterpret_cast<const float *>(so[x])[d], f);
     }
     static_cast<T *>(a.out)[((long long)w.b * a.H + g * R + h0 + r) * a.D + d] = from_f<T>(sum == 0.f ? 0.f : y / sum);
   }

@@ -54,3 +54,49 @@ def test_packed_attention_of_weak_keys(ops, dtype, gap):
             tiny = 2.0 ** -32 * v[:r + 1, 0].double().sum(0) if dtype is F16 else 0.0
             ok, why = S.within(got[r], want, slack + tiny, dtype)
             assert ok, (at, r, why)
+
+
+# ---- values that are not finite ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("n,D,page", [(150, 64, 16), (150, 128, 7), (4000, 64, 16), (4000, 128, 16), (1500, 256, 24)])
+def test_paged_attention_of_values_that_are_not_finite(ops, dtype, n, D, page):
+    """A value that is not finite makes its dimension so, of the heads that see it, and no other; infinities of both signs make NaN."""
+    H, G = 6, 2
+    k_pages, v_pages, table = pool([n, 40], page, G, D, dtype)
+    k, v, q = rnd(1, n, G, D, dtype=dtype), rnd(2, n, G, D, dtype=dtype), rnd(3, 2, H, D, dtype=dtype)
+    put(k_pages, table, 0, 0, k), put(v_pages, table, 0, 0, v)
+    put(k_pages, table, 1, 0, k[:40]), put(v_pages, table, 1, 0, v[:40])
+    pos = torch.tensor([n - 1, 39], device="cuda")
+    want = ops.paged_attention(q, k_pages, v_pages, table, pos, 0.3)
+    for t in (0, 17, n // 2, n - 1):
+        w = v[t].clone()
+        w[1, 5], w[1, 6], w[1, 7] = math.inf, -math.inf, math.nan
+        put(v_pages, table, 0, t, w[None])
+        got = ops.paged_attention(q, k_pages, v_pages, table, pos, 0.3)
+        assert bool((got[0, 3:, 5] == math.inf).all()) and bool((got[0, 3:, 6] == -math.inf).all()) and bool(got[0, 3:, 7].isnan().all()), t
+        got[0, 3:, 5:8] = want[0, 3:, 5:8]
+        assert torch.equal(got, want), t
+        put(v_pages, table, 0, t, v[t][None])
+    w = v[10:12].clone()
+    w[0, 0, 9], w[1, 0, 9] = math.inf, -math.inf
+    put(v_pages, table, 0, 10, w)
+    got = ops.paged_attention(q, k_pages, v_pages, table, pos, 0.3)
+    assert bool(got[0, :3, 9].isnan().all())
+    got[0, :3, 9] = want[0, :3, 9]
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,gap", [(F16, 14.0), (F16, 30.0), (F16, 150.0), (BF16, 14.0), (BF16, 80.0), (F32, 14.0), (F32, 80.0)])
+@pytest.mark.parametrize("n", [150, 4000])
+def test_paged_attention_of_an_infinite_value_with_a_small_weight(ops, dtype, gap, n):
+    """An infinite value that is seen is not lost and does not turn into NaN, as long as 32 bits hold its weight, in fp16 however small that is."""
+    for at in (0, n // 2, n - 1):
+        q, k, v = one_ahead(n, at, gap, dtype)
+        for t in (1, n // 3, n - 2):
+            w = v.clone()
+            w[t, 0, 5] = -math.inf
+            k_pages, v_pages, table = pool([n], 16, 1, 64, dtype)
+            put(k_pages, table, 0, 0, k), put(v_pages, table, 0, 0, w)
+            got = ops.paged_attention(q[:1], k_pages, v_pages, table, torch.tensor([n - 1], device="cuda"), 1.0)[0, 0]
+            assert float(got[5]) == -math.inf and int(got.isfinite().sum()) == 63, (at, t)
