@@ -25,7 +25,9 @@
 //
 // What a row does not see must not reach it: scores are masked by comparison, but a weight of 0 times an infinity would be NaN. So
 // entries of those value tiles that are not finite are set to 0 before the products, and joined again at the end for the rows that
-// see them.
+// see them. In the tiles that all rows see the products take them as they are; where a weight (or what O is rescaled by) has been rounded
+// to 0 that is NaN too, and a warp whose results are not finite, though the sum of the weights is, goes through the values once more (looking at
+// each 16 columns as they are stored took 2 % more; at the end of them it takes nothing).
 #include "pairs.cuh"
 #include "serving_packed.cuh"
 #include "tcgen05.cuh"
@@ -335,14 +337,38 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(&taken[parity][t]);
       T *out = static_cast<T *>(a.out) + ((long long)(first + q0 + t * PT_M + r) * a.H + h) * a.D;
-#pragma unroll 1
-      for (int q = 0; q < a.D; q += 16) {
+      float z = 0.f;  // or NaN: a result is not finite
+      auto results = [&](int q, bool again) {
         uint32_t o[16];
         tmem_ld16(o, tm_o + q);
         tmem_wait_ld();
         float f[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * inv;
+        if (!again) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) z = fmaf(f[e], 0.f, z);
+        } else {  // values of whole tiles that are not finite
+          float x[16] = {};
+          const T *v = static_cast<const T *>(a.v) + (long long)first * a.ldv + h / (a.H / a.G) * a.hv + q;
+#pragma unroll 4
+          for (int j = lane; j < q0; j += WARP)
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+              if (q + e >= a.D) continue;
+              float y[8];
+              unpack_chunk<T>(*reinterpret_cast<const uint4 *>(v + j * a.ldv + e), y);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (!(fabsf(y[i]) < INFINITY)) x[e + i] += y[i];
+            }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) x[e] += __shfl_xor_sync(0xffffffffu, x[e], d);
+            if (f[e] != f[e] && x[e] != 0.f) f[e] = x[e];
+          }
+        }
         if ((odd0 || odd1) && r < rows) {  // values that are not finite, for who sees them
           const int i = q0 + t * PT_M + r, g = h / (a.H / a.G);
           for (int d2 = 0; d2 < 2; ++d2) {
@@ -372,6 +398,12 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           }
         }
         __syncwarp();
+      };
+#pragma unroll 1
+      for (int q = 0; q < a.D; q += 16) results(q, false);
+      if (__any_sync(0xffffffffu, z != 0.f && l == l && r < rows)) {
+#pragma unroll 1
+        for (int q = 0; q < a.D; q += 16) results(q, true);
       }
       tmem_fence_before();  // (the next item's first product into O waits for this thread's next weights)
     }

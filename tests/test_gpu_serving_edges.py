@@ -100,3 +100,20 @@ def test_paged_attention_of_an_infinite_value_with_a_small_weight(ops, dtype, ga
             put(k_pages, table, 0, 0, k), put(v_pages, table, 0, 0, w)
             got = ops.paged_attention(q[:1], k_pages, v_pages, table, torch.tensor([n - 1], device="cuda"), 1.0)[0, 0]
             assert float(got[5]) == -math.inf and int(got.isfinite().sum()) == 63, (at, t)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128, 160])
+@pytest.mark.parametrize("gap", [14.0, 30.0, 100.0])
+def test_packed_attention_of_an_infinite_value_with_a_small_weight(ops, dtype, D, gap):
+    n = 900
+    for at in (0, 400):  # the key that has the weight, in front of the value and behind it
+        q, k, v = one_ahead(n, at, gap, dtype, D)
+        clean = ops.packed_attention(q, k, v, cumulative([n]), 1.0)
+        for t in (3, 130, 300, 520):
+            w = v.clone()
+            w[t, 0, 5], w[t, 0, D - 1] = math.inf, math.nan
+            got = ops.packed_attention(q, k, w, cumulative([n]), 1.0)
+            assert bool((got[t:, 0, 5] == math.inf).all()) and bool(got[t:, 0, D - 1].isnan().all()), (at, t)
+            got[t:, 0, 5], got[t:, 0, D - 1] = clean[t:, 0, 5], clean[t:, 0, D - 1]
+            assert torch.equal(got, clean), (at, t)
