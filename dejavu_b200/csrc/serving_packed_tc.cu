@@ -287,7 +287,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           for (int e = 0; e < 32; e += 2) mm[e / 2 % 4] = max3(mm[e / 2 % 4], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
         const float mx = fmaxf(max3(mm[0], mm[1], mm[2]), mm[3]) * ca;
         if (j == 0) {
-          m = mx == -INFINITY ? 0.f : mx;
+          m = mx == -INFINITY ? -3e38f : mx;  // (a tile that weighs nothing: any later maximum is more)
         } else {
           const bool grow = mx > m + 8.f;
           if (__any_sync(0xffffffffu, grow)) {

@@ -117,3 +117,19 @@ def test_packed_attention_of_an_infinite_value_with_a_small_weight(ops, dtype, D
             assert bool((got[t:, 0, 5] == math.inf).all()) and bool(got[t:, 0, D - 1].isnan().all()), (at, t)
             got[t:, 0, 5], got[t:, 0, D - 1] = clean[t:, 0, 5], clean[t:, 0, D - 1]
             assert torch.equal(got, clean), (at, t)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 128, 160])
+def test_packed_attention_after_keys_that_weigh_nothing(ops, dtype, D):
+    """Scores of -inf in a whole tile of keys, the first one, and scores far below 0 behind it."""
+    n, H = 400, 2
+    q, k, v = rnd(1, n, H, D, dtype=dtype).abs() + 1, rnd(2, n, H, D, dtype=dtype), rnd(3, n, H, D, dtype=dtype)
+    k[:128, :, 0] = -math.inf
+    k[128:, :, 1] = -300
+    got = ops.packed_attention(q, k, v, cumulative([n]), 1.0)
+    for r in (128, 129, 255, 256, 399):
+        for h in range(H):
+            want, slack = S.attend(q[r, h:h + 1], k[128:r + 1, h], v[128:r + 1, h], 1.0, weight_step=S.half_step(dtype))
+            ok, why = S.within(got[r, h:h + 1], want, slack, dtype)
+            assert ok, (r, h, why)
