@@ -742,7 +742,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   z.c_lo = (float)(log2_unit - (double)z.c_hi);
   z.reach = (float)fmin(SA_FAR * temperature, 3e38);
   const float range = fminf(z.top - bottom, z.reach);
-  z.inv = range > 0.f && range < 3e38f ? SA_BINS / range * 0.99999f : 0.f;
+  // (one step for all where they would be too fine or too coarse for floats, their parts, 2^23 in all, among them)
+  z.inv = range > 1e-30f && range < 3e38f ? SA_BINS / range * 0.99999f : 0.f;
   z.fine_bits = min(12, __clz(a.V) - 1);  // (the sum of parts over the row stays below 2^31)
   z.fine = (float)(1 << z.fine_bits);
   z.inv_fine = z.inv * z.fine;

@@ -133,3 +133,20 @@ def test_packed_attention_after_keys_that_weigh_nothing(ops, dtype, D):
             want, slack = S.attend(q[r, h:h + 1], k[128:r + 1, h], v[128:r + 1, h], 1.0, weight_step=S.half_step(dtype))
             ok, why = S.within(got[r, h:h + 1], want, slack, dtype)
             assert ok, (r, h, why)
+
+
+# ---- sampling ------------------------------------------------------------------------------------------------------------------
+
+NARROW = [{}, {"top_k": 3}, {"top_k": 700}, {"top_p": 0.7}, {"min_p": 0.5}, {"top_k": 900, "top_p": 0.5, "min_p": 0.9}]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("settings", NARROW, ids=str)
+@pytest.mark.parametrize("unit", [1e-20, 1e-30, 1e-31, 3e-32, 1e-33, 1e-38])
+def test_sample_tokens_of_next_to_equal_logits(ops, dtype, settings, unit):
+    """Differences next to none: the entries weigh the same but keep their order."""
+    logits, u = rnd(58, 6, 1500) * unit, torch.rand(6, device="cuda", generator=torch.Generator("cuda").manual_seed(10))
+    check_sample(ops, logits.to(dtype), u, **settings)
+    one = torch.zeros(6, 5003, device="cuda")
+    one[:, 4000], one[3:, 17] = unit, -unit
+    check_sample(ops, one.to(dtype), u, **settings)
