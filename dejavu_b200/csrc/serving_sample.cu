@@ -35,7 +35,7 @@ namespace djv {
 
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / WARP, SA_BINS = 2048, SA_LIST = 2048, SA_CLUSTER = 8;
 constexpr int SA_EACH = SA_BINS / SA_THREADS;  // steps, or entries of the list, of a thread
-constexpr double SA_CLOSE = 3e-9;   // what counts as close, of a sum: more than twice the weights' relative error
+constexpr double SA_CLOSE = 3e-9;   // what counts as close, of a sum: more than twice the weights' relative error (and what they lose in sums)
 constexpr int SA_TABLE = 256;
 constexpr float SA_MAGIC = 12582912.f;  // added to a number below 2^22 rounds it: the lowest bits are then the number's
 constexpr uint32_t SA_ROUND = 0x4b400000u;  // (its bits)
@@ -234,6 +234,7 @@ struct SampleScale {
   double temperature;
   float c_hi, c_lo;     // log2(e) / temperature
   float reach;          // entries further below the largest are dropped
+  double close;         // see SA_CLOSE
 
   __device__ __forceinline__ bool counts(float x) const { return top - x <= reach || x == top; }
   // For x that counts: how many parts of a step, `fine` of them to one, are in front of it, rounded, plus 2^23: a number whose lowest bits
@@ -273,7 +274,7 @@ struct SampleScale {
 };
 // (where a few are made in cold code)
 __device__ __noinline__ double weight_of(const SampleScale &z, float x, const uint2 *table) { return z.weight(x, table); }
-constexpr int SA_UNITS = 52;  // sums are integers, 2^52 to the largest weight: 4096 of those fit
+constexpr int SA_UNITS = 52;  // sums are integers, 2^52 to the largest weight: 4096 of those fit. Entries 36 temperatures below it are 0 in them.
 __device__ __forceinline__ u64 shifted(u64 v, unsigned down) {  // (0 from 64 on)
   u64 r;
   asm("shr.u64 %0, %1, %2;" : "=l"(r) : "l"(v), "r"(down));
@@ -469,7 +470,7 @@ struct SampleAlone {
     if (warp == at) {
       double run = before;
       int token = -1, latest = -1;
-      near |= fabs(before - target) <= SA_CLOSE * total;
+      near |= fabs(before - target) <= z.close * total;
       for (int i0 = lo; i0 < hi && token < 0; i0 += WARP) {
         const int i = i0 + lane;
         const double w = i < hi ? kept(to_f(entries[i]), i) : 0.0;
@@ -482,7 +483,7 @@ struct SampleAlone {
           if (lane >= o) sum += up;
         }
         const unsigned over = __ballot_sync(0xffffffffu, w > 0 && run + sum > target);
-        near |= __any_sync(0xffffffffu, w > 0 && fabs(run + sum - target) <= SA_CLOSE * total) != 0;
+        near |= __any_sync(0xffffffffu, w > 0 && fabs(run + sum - target) <= z.close * total) != 0;
         latest = i0 + 31 - __clz(any);
         if (over) token = i0 + __ffs(over) - 1;
         run += __shfl_sync(0xffffffffu, sum, WARP - 1);
@@ -517,7 +518,7 @@ __device__ __noinline__ int sample_list(SampleShared &s, const SampleScale &z, i
     bool in = at + e < n;
     if (in && p < 1 && at + e > 0) {
       in = run < mass;
-      near |= fabs(run - mass) <= SA_CLOSE * (total + behind);
+      near |= fabs(run - mass) <= z.close * (total + behind);
     }
     if (in && min_p > 0 && w[e] < min_p * (1 + 1e-8)) in = w[e] >= min_p * (1 - 1e-8) && z.exact(logit_of((uint32_t)(s.list[at + e] >> 32))) >= min_p;
     left += in;
@@ -542,7 +543,7 @@ __device__ __noinline__ int sample_list(SampleShared &s, const SampleScale &z, i
     double upto = run;
     for (int x = 0; x <= e; ++x) upto += w[x];
     if (at + e >= n) continue;
-    near |= fabs(upto - target) <= SA_CLOSE * total;
+    near |= fabs(upto - target) <= z.close * total;
     if (upto > target) over = min(over, at + e);
   }
   over = (int)block_least((u64)over, s.wide);
@@ -589,7 +590,7 @@ __device__ __noinline__ int sample_short(const SampleShared &s, const SampleScal
         last = __shfl_sync(0xffffffffu, upto[h], WARP - 1);
         if (in[h] && p < 1 && lane + h > 0) {
           in[h] = before < mass;
-          near |= fabs(before - mass) <= SA_CLOSE * all;
+          near |= fabs(before - mass) <= z.close * all;
         }
         if (in[h] && min_p > 0 && w[h] < min_p * (1 + 1e-8))
           in[h] = w[h] >= min_p * (1 - 1e-8) && z.exact(logit_of((uint32_t)(v[h] >> 32))) >= min_p;
@@ -600,7 +601,7 @@ __device__ __noinline__ int sample_short(const SampleShared &s, const SampleScal
       unsigned over[2], some[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        near |= in[h] && fabs(upto[h] - target) <= SA_CLOSE * total;
+        near |= in[h] && fabs(upto[h] - target) <= z.close * total;
         over[h] = __ballot_sync(0xffffffffu, in[h] && upto[h] > target);
         some[h] = __ballot_sync(0xffffffffu, in[h]);
       }
@@ -737,6 +738,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
   }
   z.top = logit_of((uint32_t)(best >> 32));
   z.temperature = temperature;
+  z.close = SA_CLOSE + a.V * (1.0 / (1ll << SA_UNITS));  // (a sum is 1 or more, and each entry loses less than a unit of it)
   const double log2_unit = 1.4426950408889634 / temperature;
   z.c_hi = (float)log2_unit;
   z.c_lo = (float)(log2_unit - (double)z.c_hi);
@@ -1067,7 +1069,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
 #pragma unroll
         for (int e = 0; e < SA_EACH; ++e) {
           if (at + e < length && at + e > 0) {
-            near |= fabs(before - mass) <= SA_CLOSE * all;
+            near |= fabs(before - mass) <= z.close * all;
             if (before < mass) last = at + e;
           }
           before += w[e];

@@ -150,3 +150,18 @@ def test_sample_tokens_of_next_to_equal_logits(ops, dtype, settings, unit):
     one = torch.zeros(6, 5003, device="cuda")
     one[:, 4000], one[3:, 17] = unit, -unit
     check_sample(ops, one.to(dtype), u, **settings)
+
+
+def test_sample_tokens_of_many_small_weights(ops):
+    """Entries 34 temperatures below the last one, which together make up 10^-7: a number that falls among them."""
+    V = 2 ** 26
+    logits = torch.zeros(1, V, device="cuda")
+    logits[0, V - 1] = 34.0
+    w = math.exp(-34.0)
+    total = 1 + (V - 1) * w
+    for part in (0.2, 0.9, 0.953, 0.9999, 1.0001, 2.0):
+        u = torch.tensor([part * (V - 1) * w / total], device="cuda")
+        at = float(u.double()) * total / w  # so many of them
+        if not 1e-3 < at % 1 < 1 - 1e-3:
+            continue
+        assert int(ops.sample_tokens(logits, u)) == min(int(at), V - 1), part
