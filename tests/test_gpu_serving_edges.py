@@ -165,3 +165,15 @@ def test_sample_tokens_of_many_small_weights(ops):
         if not 1e-3 < at % 1 < 1 - 1e-3:
             continue
         assert int(ops.sample_tokens(logits, u)) == min(int(at), V - 1), part
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_sample_tokens_with_a_number_of_zero(ops, dtype):
+    """The lowest index that is kept, however little it weighs."""
+    V = 3001
+    logits, u = rnd(59, 7, V).mul(2).to(dtype), torch.zeros(7, device="cuda")
+    for b, below in enumerate((30, 44, 46, 60, 100, 700, 800)):
+        logits[b, 0] = float(logits[b].float().max()) - below
+    for settings in ({}, {"top_k": 50}, {"top_k": V - 1}, {"top_p": 0.9}, {"min_p": 0.1}, {"min_p": 1e-30}, {"top_k": V, "temperature": 2.0},
+                     {"temperature": 0.5}):
+        check_sample(ops, logits, u, **settings)
