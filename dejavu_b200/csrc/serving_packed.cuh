@@ -14,7 +14,7 @@ struct PackedArgs {
   int keep_rest;
 };
 
-// the tensor-core form: fp16 and bf16, rows that TMA can read
+// the tensor-core form: fp16 and bf16, rows that TMA can read, results that start on 16 bytes
 bool packed_tc_supported(int dtype, const PackedArgs &a);
 int packed_tc(int dtype, const PackedArgs &a, cudaStream_t st);
 

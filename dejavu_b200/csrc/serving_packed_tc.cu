@@ -111,7 +111,7 @@ struct Exponent<__half> {
   static constexpr uint32_t MASK = 0x7c007c00u, ONE = 0x04000400u;
 };
 
-// KB: blocks of 64 elements in a row; FULL: all of them are in use; NT: query tiles of an item; KN: keys of a tile
+// KB: blocks of 64 elements in a row; FULL: all of them are in use, and results start on 32 bytes; NT: query tiles of an item; KN: keys of a tile
 template <typename T, int KB, bool FULL, int NT, int KN, int STAGES>
 __global__ void __launch_bounds__(PT_THREADS, 1)
 packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -618,7 +618,7 @@ static bool rows_fit(const void *p, long long ld, long long hs, int heads) {
 }
 bool packed_tc_supported(int dtype, const PackedArgs &a) {
   return dtype != DJV_DTYPE_F32 && a.D % 8 == 0 && a.D <= 256 && rows_fit(a.q, a.ldq, a.hq, a.H) && rows_fit(a.k, a.ldk, a.hk, a.G) &&
-         rows_fit(a.v, a.ldv, a.hv, a.G) && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0 &&
+         rows_fit(a.v, a.ldv, a.hv, a.G) && aligned16(a.out) &&
          (long long)packed_tiles<PT_M>(a.T, a.B) * a.H < (1ll << 30) && encode_tiled();
 }
 
@@ -653,9 +653,10 @@ static int launch_packed_tc(const PackedArgs &a, cudaStream_t st) {
 int packed_tc(int dtype, const PackedArgs &a, cudaStream_t st) {
   const auto of = [&](auto t) {
     using T = decltype(t);
-    if (a.D <= 64) return a.D == 64 ? launch_packed_tc<T, 1, true>(a, st) : launch_packed_tc<T, 1, false>(a, st);
-    if (a.D <= 128) return a.D == 128 ? launch_packed_tc<T, 2, true>(a, st) : launch_packed_tc<T, 2, false>(a, st);
-    return a.D == 256 ? launch_packed_tc<T, 4, true>(a, st) : launch_packed_tc<T, 4, false>(a, st);
+    const bool sectors = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;  // whole heads are stored 32 bytes at a time
+    if (a.D <= 64) return a.D == 64 && sectors ? launch_packed_tc<T, 1, true>(a, st) : launch_packed_tc<T, 1, false>(a, st);
+    if (a.D <= 128) return a.D == 128 && sectors ? launch_packed_tc<T, 2, true>(a, st) : launch_packed_tc<T, 2, false>(a, st);
+    return a.D == 256 && sectors ? launch_packed_tc<T, 4, true>(a, st) : launch_packed_tc<T, 4, false>(a, st);
   };
   return dtype == DJV_DTYPE_F16 ? of(__half()) : of(bf16());
 }

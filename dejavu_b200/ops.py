@@ -1005,7 +1005,8 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     assert 1 <= D <= 256, f"heads of {D}"
     B = _cumulative(cu_seqlens)
     (q, q_args), (k, k_args), (v, v_args) = _rows(q), _rows(k), _rows(v)
-    if dtype is not torch.float32 and not D & 7:  # rows that TMA can read: a copy costs a tenth or less of what the CUDA cores would take more
+    tensor_cores = dtype is not torch.float32 and not D & 7
+    if tensor_cores:  # rows that TMA can read: a copy costs a tenth or less of what the CUDA cores would take more
         if not _even(*q_args):
             q, q_args = _rows(q.clone(memory_format=torch.contiguous_format))
         if not _even(*k_args):
@@ -1021,10 +1022,11 @@ def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
             assert T == 0 or end <= t.data_ptr() or t.data_ptr() + last * t.element_size() <= begin, "out: apart from q, k and v"
     else:
         out = q.new_empty(T, H, D)
+    to = out.clone() if tensor_cores and out.data_ptr() & 15 else out  # (and results that it stores 16 bytes at a time)
     if T:
-        call("djv_packed_attention", code, out.data_ptr(), *q_args, *k_args, *v_args, cu_seqlens.data_ptr(), B, T, H, G, D, float(scale),
+        call("djv_packed_attention", code, to.data_ptr(), *q_args, *k_args, *v_args, cu_seqlens.data_ptr(), B, T, H, G, D, float(scale),
              int(keep), _stream())
-    return out
+    return out if to is out else out.copy_(to)
 
 
 def _bits(x: float) -> int:

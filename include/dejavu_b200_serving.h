@@ -59,7 +59,8 @@ unsigned djv_serving_timeouts(void);
 /* Causal attention over whole prompts, packed: rows cu[b] .. cu[b + 1] - 1 (cu: B + 1 int32, ascending, within 0 .. T) of q (T, H, D), k
  * and v (T, G, D) are sequence b; row i sees rows j <= i of its sequence, whatever the others hold. Rows ldq, ldk, ldv elements
  * apart, heads hq, hk, hv apart, dimensions adjacent. H % G == 0, D <= 256. out (T, H, D), contiguous. Rows of no sequence:
- * zeros, or with keep_rest left as they are. */
+ * zeros, or with keep_rest left as they are. The tensor cores take fp16 and bf16 where D, strides and addresses, out's among them, are
+ * multiples of 16 bytes; all else goes to the CUDA cores, some 20 to 30 times slower. */
 int djv_packed_attention(int dtype, void *out, const void *q, long long ldq, long long hq, const void *k, long long ldk, long long hk,
                          const void *v, long long ldv, long long hv, const int32_t *cu, int B, int T, int H, int G, int D, float scale,
                          int keep_rest, void *stream);

@@ -135,6 +135,22 @@ def test_packed_attention_after_keys_that_weigh_nothing(ops, dtype, D):
             assert ok, (r, h, why)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [64, 72, 128, 200, 256])
+def test_packed_attention_into_any_address(ops, dtype, D):
+    """An output on any boundary holds the same bits, and rows of no sequence stay."""
+    T, H, G = 300, 3, 1
+    q, k, v = rnd(1, T, H, D, dtype=dtype), rnd(2, T, G, D, dtype=dtype), rnd(3, T, G, D, dtype=dtype)
+    cu = cumulative([200, 90], first=4)
+    want = ops.packed_attention(q, k, v, cu, 0.1)
+    for at in (0, 16, 8, 3):
+        room = torch.full((T * H * D + 16,), 7.0, dtype=dtype, device="cuda")
+        out = room[at:at + T * H * D].view(T, H, D)
+        assert ops.packed_attention(q, k, v, cu, 0.1, out=out) is out
+        assert torch.equal(out[4:294], want[4:294]), at
+        assert bool((out[:4] == 7).all()) and bool((out[294:] == 7).all()) and bool((room[:at] == 7).all()) and bool((room[at + T * H * D:] == 7).all())
+
+
 # ---- sampling ------------------------------------------------------------------------------------------------------------------
 
 NARROW = [{}, {"top_k": 3}, {"top_k": 700}, {"top_p": 0.7}, {"min_p": 0.5}, {"top_k": 900, "top_p": 0.5, "min_p": 0.9}]
