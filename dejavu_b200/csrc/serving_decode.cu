@@ -60,8 +60,8 @@ struct DecodeArgs {
 
 // Tokens of sequence b.
 __device__ __forceinline__ long long decode_tokens(const DecodeArgs &a, int b) {
-  const long long n = a.pos[b] + 1, room = (long long)a.width * a.page;
-  return n < 0 ? 0 : (n > room ? room : n);
+  const long long p = a.pos[b], room = (long long)a.width * a.page;
+  return p < 0 ? 0 : (p >= room ? room : p + 1);
 }
 
 struct DecodePlace {

@@ -135,6 +135,19 @@ def test_packed_attention_after_keys_that_weigh_nothing(ops, dtype, D):
             assert ok, (r, h, why)
 
 
+def test_paged_attention_behind_the_last_position(ops):
+    """The largest position that there is: all tokens of the table are seen, and it is counted."""
+    H, G, D, n = 2, 1, 64, 32
+    k_pages, v_pages, table = pool([n], 16, G, D, F16)
+    put(k_pages, table, 0, 0, rnd(1, n, G, D, dtype=F16)), put(v_pages, table, 0, 0, rnd(2, n, G, D, dtype=F16))
+    q, before = rnd(3, 1, H, D, dtype=F16), ops.paged_faults()
+    want = ops.paged_attention(q, k_pages, v_pages, table, torch.tensor([n - 1], device="cuda"), 0.125)
+    assert ops.paged_faults() == before
+    for p in (n, 2 ** 31, 2 ** 63 - 1):
+        assert torch.equal(ops.paged_attention(q, k_pages, v_pages, table, torch.tensor([p], device="cuda"), 0.125), want), p
+    assert ops.paged_faults() > before
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("D", [64, 72, 128, 200, 256])
 def test_packed_attention_into_any_address(ops, dtype, D):
