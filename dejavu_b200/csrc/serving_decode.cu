@@ -622,8 +622,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   // The first token of the warp's next tile; where its row is in the pools (BOXES: the page and, in the upper half, the slot), or -1.
   // Without BOXES the lane's own token's, lanes beyond the tile's tokens repeat them.
   auto row_ahead = [&]() -> long long {
-    const int t = ahead.t0 + (ahead.i * DE_WARPS + warp) * TOKENS + (BOXES ? 0 : lane % TOKENS);
-    if (!more || t >= ahead.t1) return -1;
+    const int at = (ahead.i * DE_WARPS + warp) * TOKENS + (BOXES ? 0 : lane % TOKENS);
+    if (!more || at >= ahead.t1 - ahead.t0) return -1;  // (the tile's tokens may pass 2^31)
+    const int t = ahead.t0 + at;
     int slot;
     PageMap map = no_map;
     map.table = a.table + ahead.b * a.ld_table;

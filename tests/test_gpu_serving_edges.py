@@ -135,6 +135,20 @@ def test_packed_attention_after_keys_that_weigh_nothing(ops, dtype, D):
             assert ok, (r, h, why)
 
 
+# ---- positions and addresses ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("page,width", [(8176, (2 ** 31 - 16) // 8176), (49981, (2 ** 31 - 2) // 49981)])
+def test_paged_attention_next_to_2_31_tokens(ops, page, width):
+    """As many tokens as a table can have, all of one page: no position passes 32 bits, and nothing counts as refused."""
+    k_pages, v_pages = torch.zeros(1, 1, page, 8, dtype=F16, device="cuda"), torch.ones(1, 1, page, 8, dtype=F16, device="cuda")
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    before = ops.paged_faults()
+    got = ops.paged_attention(torch.ones(1, 1, 8, dtype=F16, device="cuda"), k_pages, v_pages, table,
+                              torch.tensor([page * width - 1], device="cuda"), 1.0)
+    # sums of 2^31 equal weights: 2^31 * 2^-24 would be the bound of a single running sum; parts of a 2^10th and their sum are off by 2^-3 at most
+    assert ops.paged_faults() == before and float((got - 1).abs().max()) <= 2 ** -3
+
+
 def test_paged_attention_behind_the_last_position(ops):
     """The largest position that there is: all tokens of the table are seen, and it is counted."""
     H, G, D, n = 2, 1, 64, 32
