@@ -55,7 +55,8 @@ __device__ __forceinline__ AppendPlace append_place(const AppendArgs &a, int t) 
   const int b = a.cu == nullptr ? t : sequence_of(a.cu, a.B, t);
   AppendPlace w{-1, -1};
   if (b < 0) return w;
-  w.p = a.pos[b] + (a.cu == nullptr ? 0 : t - a.cu[b]);
+  const long long begin = a.pos[b], row = a.cu == nullptr ? 0 : t - a.cu[b], most = 0x7fffffffffffffffll;
+  w.p = begin > most - row ? most : begin + row;  // (behind every table all the same)
   if (w.p < 0) return w;
   int slot;
   const PageMap m{a.table + b * a.ld_table, a.width, a.page, a.pages, a.by_page};

@@ -162,6 +162,18 @@ def test_paged_attention_behind_the_last_position(ops):
     assert ops.paged_faults() > before
 
 
+def test_append_behind_the_last_position(ops):
+    """Positions as large as there are: counted, not stored, and not taken for negative ones."""
+    G, D = 2, 64
+    k, v = rnd(1, 5, G, D, dtype=BF16), rnd(2, 5, G, D, dtype=BF16)
+    k_pages, v_pages, table = pool([20, 20], 16, G, D, BF16)
+    before = ops.paged_faults()
+    _, k_out = ops.paged_append(None, k, v, k_pages, v_pages, table, torch.tensor([2 ** 63 - 1, 2 ** 63 - 2], device="cuda"),
+                                cu_seqlens=cumulative([3, 2]), keys=True)
+    assert torch.equal(k_out, k) and ops.paged_faults() - before == 5
+    assert bool(k_pages.isnan().all()) and bool(v_pages.isnan().all())
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("D", [64, 72, 128, 200, 256])
 def test_packed_attention_into_any_address(ops, dtype, D):
