@@ -15,7 +15,8 @@
 // 2^16, so its weights, up to 2^8, are made 2^7 times as large, and so are their sums: from 2^-21 of the largest on they have all their
 // bits, below that they are off by 2^-32 of the largest at most.
 //
-// Items go out in the order of falling work, back and forth over the blocks; sequences may have any lengths.
+// Few items go out in the order of falling work, many from the last sequence's last one on, back and forth over the blocks; sequences
+// may have any lengths.
 //
 // Measured (32 heads over 8, 128 dimensions, bf16): 16001 tokens 1.71 ms, 1.22 PFLOP/s, and 1.97 ms when the power cap has the clocks at
 // 1.64 GHz; 24 prompts of 16384 tokens in all 0.31 ms, 0.72 PFLOP/s. A step of an item takes about 3000 cycles, the exponentials of its two
@@ -152,7 +153,10 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   // How many items there are, and if they are few their order: by falling number in the sequence, which is what they take.
   // (Offsets that do not ascend can make more than `most`, which is all that offsets that do can make: the rest is left out.)
   const int total = packed_total<PT_Q>(a, 0, a.B), tiles = total < 0 || total > most ? most : total;
-  const bool ordered = tiles == total && tiles <= PT_TABLE && (long long)tiles * a.B <= 64 * 1024;
+  // Every block makes the order for itself, in tiles * B steps or so, and what it evens out grows less with more sequences. 32 heads of 128, in
+  // order and not, by tiles * B: 444 128 and 136 us, 1848 241 and 250, 2592 222 and 256, 4608 550 and 570, 6528 200 and 192, 7344 483 and 472,
+  // 18944 216 and 207.
+  const bool ordered = tiles == total && tiles <= PT_TABLE && a.B <= 5 * 1024 && tiles * a.B <= 5 * 1024;
   if (ordered) {
     for (int i = warp; i < tiles; i += PT_THREADS / WARP) {
       const PackedTile w = packed_tile<PT_Q>(a, i);
