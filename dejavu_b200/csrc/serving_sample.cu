@@ -39,7 +39,8 @@ constexpr double SA_CLOSE = 3e-9;   // what counts as close, of a sum: more than
 constexpr int SA_TABLE = 256;
 constexpr float SA_MAGIC = 12582912.f;  // added to a number below 2^22 rounds it: the lowest bits are then the number's
 constexpr uint32_t SA_ROUND = 0x4b400000u;  // (its bits)
-constexpr float SA_FAR = 45.f;      // temperatures below the largest entry from where on nothing counts (e^-45 = 3e-20), unless u is 0
+constexpr float SA_FAR = 45.f;      // temperatures below the largest entry from where on nothing counts (e^-45 = 3e-20)
+constexpr double SA_TINY = 1e-10;   // unless u is less than what 2^30 of them make up together (3e-11): 0, or no usual random number
 
 struct SampleArgs {
   long long *token;
@@ -759,7 +760,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
     const int token = r.token(k, p, min_p, u);
     if (tid == 0) a.token[b] = token;
   };
-  if (!(u > 0)) {  // the first entry that is kept, even if it weighs next to nothing: down to where 64 bits end (2^-1074, 744.5 temperatures)
+  if (!(u >= SA_TINY)) {  // falls among the first entries that are kept, even if they weigh next to nothing: down to where 64 bits end (2^-1074)
     z.reach = (float)fmin(746.0 * temperature, 3e38);
     if (rank == 0) alone();
     return;

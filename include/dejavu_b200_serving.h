@@ -69,8 +69,8 @@ int djv_packed_attention(int dtype, void *out, const void *q, long long ldq, lon
  *   the first top_k (0: all); of those the ones in front of which less than top_p of their sum lies, the first always (1 or more:
  *   all); of those the ones with w >= min_p.
  * token[b] (int64) is the lowest index at which the running sum of kept w, in index order, exceeds u[b] times their sum. A temperature
- * not above 0 takes the largest entry, equal ones the lowest index. A row without entries gets -1. Entries more than 45
- * temperatures below the largest are dropped; sums are as exact as 64 bits make them wherever 32 could choose another token.
+ * not above 0 takes the largest entry, equal ones the lowest index. A row without entries gets -1. Sums are as exact as 64 bits make them
+ * wherever 32 could choose another token; entries more than 45 temperatures below the largest only count where they could (u below 1e-10).
  * Each setting is an array of B values on the device (float, int32, float, float) or, where that is NULL, the number beside it: of the
  * three real ones the bits of a double. */
 int djv_sample(int dtype, long long *token, const void *logits, long long ld, const float *u, const float *temperature,

@@ -232,3 +232,15 @@ def test_sample_tokens_with_a_number_of_zero(ops, dtype):
     for settings in ({}, {"top_k": 50}, {"top_k": V - 1}, {"top_p": 0.9}, {"min_p": 0.1}, {"min_p": 1e-30}, {"top_k": V, "temperature": 2.0},
                      {"temperature": 0.5}):
         check_sample(ops, logits, u, **settings)
+
+
+@pytest.mark.parametrize("number", [1e-9, 1e-12, 1e-19, 1e-21, 1e-30, 1e-38, 1e-44])
+def test_sample_tokens_with_numbers_next_to_zero(ops, number):
+    """Numbers that fall among entries of weights far below 32 bits."""
+    V = 3001
+    logits, u = rnd(62, 9, V).mul(2), torch.full((9,), number, device="cuda")
+    for b in range(9):
+        for i, below in enumerate((101, 95, 80, 60, 50, 47, 44, 30, 20)[b:]):
+            logits[b, i] = float(logits[b].max()) - below
+    for settings in ({}, {"top_k": V - 1}, {"min_p": 1e-25}):
+        check_sample(ops, logits, u, **settings)
