@@ -244,3 +244,13 @@ def test_sample_tokens_with_numbers_next_to_zero(ops, number):
             logits[b, i] = float(logits[b].max()) - below
     for settings in ({}, {"top_k": V - 1}, {"min_p": 1e-25}):
         check_sample(ops, logits, u, **settings)
+
+
+@pytest.mark.parametrize("dtype,low", [(BF16, -1e4), (F16, -1e4), (F32, -1e4), (F32, torch.finfo(F32).min), (F16, torch.finfo(F16).min)])
+@pytest.mark.parametrize("spread", [0.5, 2.5])
+def test_sample_tokens_with_finite_masks(ops, dtype, low, spread):
+    """Ids that no token has, at a large negative number instead of -inf."""
+    logits, u = rnd(60, 2, 151936).mul(spread), torch.rand(2, device="cuda", generator=torch.Generator("cuda").manual_seed(11))
+    logits[:, 50000:50016] = low
+    for settings in ({}, {"top_p": 0.5}, {"top_p": 0.9, "temperature": 0.8}, {"top_k": 50}, {"top_k": 3000, "min_p": 0.01}):
+        check_sample(ops, logits.to(dtype), u, **settings)
