@@ -220,7 +220,7 @@ struct MmaSums {
     l[0] = l[1] = 0.f;
   }
   // c: scale in units of log 2; seen: a bit for each of the 16 tokens
-  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c, int) {
+  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c) {
     const int t = threadIdx.x % 4;
     float s[2][4] = {};
 #pragma unroll
@@ -384,7 +384,7 @@ struct DecodeSums<float, DP> {
     asm volatile("ld.shared.v2.u64 {%0,%1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(sm) : "memory");
     return v;
   }
-  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c, int) {
+  __device__ __forceinline__ void tile(uint32_t k_sm, uint32_t v_sm, unsigned seen, float c) {
     if (rows == 1) tile_of<1>(k_sm, v_sm, seen, c);
     else if (rows == 2) tile_of<2>(k_sm, v_sm, seen, c);
     else tile_of<4>(k_sm, v_sm, seen, c);
@@ -720,7 +720,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
     for (int i = 0; i < at.tiles; ++i) {
       load(stage == 0 ? STAGES - 1 : stage - 1);
       const unsigned bits = arrived(stage, i);
-      if (bits) sums.tile(warp_ring + stage * 2 * TILE, warp_ring + stage * 2 * TILE + TILE, bits, c, a.D);
+      if (bits) sums.tile(warp_ring + stage * 2 * TILE, warp_ring + stage * 2 * TILE + TILE, bits, c);
       __syncwarp();
       stage = stage == STAGES - 1 ? 0 : stage + 1;
     }

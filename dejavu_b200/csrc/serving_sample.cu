@@ -1051,53 +1051,51 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
       }
       return;
     }
-    {
-        const int at = tid * SA_EACH;
-      u64 place = cut;
-      bool close = false;
-      if (rank == 0 && s.listed > 0) {
-        const int length = s.listed;
-        double in_front = 0, behind = 0, w[SA_EACH], sum = 0, between;
-        for (int c = 0; c < C; ++c) {
-          in_front += s.sums[c][0];
-          behind += s.sums[c][1];
-        }
-        sort_list(s.list, length);
+    const int at = tid * SA_EACH;
+    u64 place = cut;
+    bool close = false;
+    if (rank == 0 && s.listed > 0) {
+      const int length = s.listed;
+      double in_front = 0, behind = 0, w[SA_EACH], sum = 0, between;
+      for (int c = 0; c < C; ++c) {
+        in_front += s.sums[c][0];
+        behind += s.sums[c][1];
+      }
+      sort_list(s.list, length);
 #pragma unroll
-        for (int e = 0; e < SA_EACH; ++e) {
-          w[e] = at + e < length ? z.weight(logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
-          sum += w[e];
-        }
-        double before = in_front + block_before(sum, s.part2, between);
-        const double all = in_front + between + behind, mass = p * all;
-        bool near = false;
-        unsigned last = 0;
+      for (int e = 0; e < SA_EACH; ++e) {
+        w[e] = at + e < length ? z.weight(logit_of((uint32_t)(s.list[at + e] >> 32)), s.table) : 0.0;
+        sum += w[e];
+      }
+      double before = in_front + block_before(sum, s.part2, between);
+      const double all = in_front + between + behind, mass = p * all;
+      bool near = false;
+      unsigned last = 0;
 #pragma unroll
-        for (int e = 0; e < SA_EACH; ++e) {
-          if (at + e < length && at + e > 0) {
-            near |= fabs(before - mass) <= z.close * all;
-            if (before < mass) last = at + e;
-          }
-          before += w[e];
+      for (int e = 0; e < SA_EACH; ++e) {
+        if (at + e < length && at + e > 0) {
+          near |= fabs(before - mass) <= z.close * all;
+          if (before < mass) last = at + e;
         }
-        const u64 found = block_all((u64)near << 32 | last, s.wide, [](u64 x, u64 y) { return max(x >> 32, y >> 32) << 32 | max((unsigned)x, (unsigned)y); });
-        close = (found >> 32) != 0;
-        place = s.list[(unsigned)found];
+        before += w[e];
       }
-      if (tell(place, close)) {
-        if (rank == 0) alone();
-        return;
-      }
-      // the block's own entries between the bounds, as far as they are kept, join their warps' sums
-      for (int i = tid; i < s.own; i += SA_THREADS) {
-        const int j = s.owned[i];
-        const float x = to_f(entries[j]);
-        if (place_of(order_of(x), j) < cut) continue;
-        const double w = z.weight(x, s.table);
-        if (!by_min || enough(x, w)) atomicAdd(&s.part[(j - from) / share], w);
-      }
-      __syncthreads();
+      const u64 found = block_all((u64)near << 32 | last, s.wide, [](u64 x, u64 y) { return max(x >> 32, y >> 32) << 32 | max((unsigned)x, (unsigned)y); });
+      close = (found >> 32) != 0;
+      place = s.list[(unsigned)found];
     }
+    if (tell(place, close)) {
+      if (rank == 0) alone();
+      return;
+    }
+    // the block's own entries between the bounds, as far as they are kept, join their warps' sums
+    for (int i = tid; i < s.own; i += SA_THREADS) {
+      const int j = s.owned[i];
+      const float x = to_f(entries[j]);
+      if (place_of(order_of(x), j) < cut) continue;
+      const double w = z.weight(x, s.table);
+      if (!by_min || enough(x, w)) atomicAdd(&s.part[(j - from) / share], w);
+    }
+    __syncthreads();
   }
 
   // 4. the sums of what is kept, in index order
