@@ -23,7 +23,7 @@ def generate(argv) -> int:
     ap.add_argument("--prompt-chunk", type=int, default=None, help="run the prompt in portions of at most this many tokens")
     ap.add_argument("--temperature", type=float, default=None, help="sample at this temperature (1 if only other limits are given)")
     ap.add_argument("--top-k", type=int, default=None, help="sample among that many largest logits (0: all)")
-    ap.add_argument("--top-p", type=float, default=None, help="sample among the tokens that make up this share of the probability")
+    ap.add_argument("--top-p", type=float, default=None, help="sample among the tokens that make up this share of the probability (0 or 1: all)")
     ap.add_argument("--min-p", type=float, default=None, help="sample among the tokens with this share of the largest probability")
     ap.add_argument("--seed", type=int, default=None, help="of the random numbers")
     args = ap.parse_args(argv)

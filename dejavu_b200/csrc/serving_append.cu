@@ -3,8 +3,8 @@
 // A block of 128 threads takes one row: its angles are shared by all heads. What it reads of q, k and v, 16 bytes at a time, depends on
 // nothing and is asked for first; beside it runs the chain offsets -> position -> angles, page, which every warp goes through for
 // itself, so that the block meets once, over the angles. Small blocks, many of them on a multiprocessor, hide that chain.
-// Bound by HBM for prompts (8191 rows of 32 + 2 x 8 heads of 128, bf16: 41 us for 218 MB, 0.81 of the copy rate; element by element 180), by
-// the chain for a few rows (one row: 3.4 us in a graph). Layouts that 16-byte accesses cannot read go element by element.
+// Bound by HBM for prompts (8191 rows of 32 + 2 x 8 heads of 128, bf16: 41 us for 218 MB, 0.81 of the copy rate; element by element 180;
+// fp32 82 us), by the chain for a few rows (one row: 3.4 us in a graph, fp32 5.1). Layouts that 16-byte accesses cannot read go element by element.
 //
 // Angles: position * frequency is exact in 64 bits up to positions of 2^29; what is left of it after whole turns are taken off in 64
 // bits is rounded to 32 and goes through sincosf, so that far positions are as exact as near ones (in 32 bits the angle of position

@@ -12,8 +12,8 @@
 // item to item, so that the next one's rows are on their way while one ends, and the page of a tile is
 // looked up a tile ahead. fp16 and bf16 go through mma.sync, 16 query heads x 16 tokens: tcgen05 would have to pad the heads to
 // 64 or 128 rows, and the tensor work is a small part of the time either way. The weights enter the second product as two terms
-// of the cache's type, hi + lo, so that they keep 16 bits (bf16), or 22 (fp16) down to 2^-18 of the largest and 2^-40 of that below: fp16
-// ends at 2^-24, so its weights are 2^15 times as large, and so are their sums. fp32 goes through the CUDA cores, 4 heads and 8 or 16
+// of the cache's type, hi + lo, so that they keep 16 bits (bf16), or 22 (fp16) down to 2^-18 of the largest, below which they are off by 2^-38
+// of the largest at most: fp16 ends at 2^-24, so its weights are 2^15 times as large, and so are their sums. fp32 goes through the CUDA cores, 4 heads and 8 or 16
 // tokens at a time.
 //
 // A value that is not finite and is seen makes its dimension so: hi is rounded towards 0, so that lo is not negative, and neither is 0
@@ -21,10 +21,11 @@
 // of 2^-126 of the largest and more, which is what 32 bits hold. (A look at the sums at the end of an item costs 2 us of 49 with short
 // items: code that is fetched once.)
 //
-// Measured (bf16, pages of 16, 32 query heads over 8 of 128 dimensions): one cache of 131071 tokens 94 us, 5.7 TB/s; 64 of up to 8192 tokens 168 us,
-// 6.0 TB/s; 16 of 32 heads, fp16, up to 2048 tokens 49 us, 5.2 TB/s (101 before an item's beginning and end counted as units); 137
-// tokens of 12 heads of 64 5.4 us in a graph. fp32, 16 caches of up to 4000 tokens, 32 heads over 8 of 128: 67 us where HBM alone would take 50 (96
-// with queries from L1, branches for the rows and 16 tokens).
+// Measured (bf16, pages of 16, 32 query heads over 8 of 128 dimensions): one cache of 131071 tokens 95 us, 5.7 TB/s; 64 of up to 8192 tokens 173 us,
+// 5.9 TB/s; 16 of 32 heads, fp16, up to 2048 tokens 51 us, 5.0 TB/s (101 before an item's beginning and end counted as units); 137
+// tokens of 12 heads of 64 5.2 us in a graph. fp32, 16 caches of up to 4000 tokens, 32 heads over 8 of 128: 72 us, 4.0 TB/s (96 with queries from L1,
+// branches for the rows and 16 tokens): exponentials and shuffles of tiles of 8 tokens. Heads of 256, bf16, over the same lengths: 78 us,
+// 3.7 TB/s, as shared memory has room for one block.
 #include <math.h>
 #include <type_traits>
 
@@ -850,8 +851,9 @@ struct DecodePlan {
   size_t scratch;
   bool split;
 };
-// Units of an item up to which it is not split (256 tokens that one block reads take no longer than a second kernel does: 137 tokens of 12
-// heads 10 us whole, 14 split), and units that a block gets at least where items are split (2000 tokens of 8 heads, cold: 16 us
+// Units of an item up to which it is not split, by what the table has room for, as the lengths are on the device: three of tokens, 192 (that
+// one block reads them takes no longer than a second kernel does: 137 tokens of 12 heads, in a graph, 5.2 us whole and 9.4 split, which a table
+// with room for 193 and more makes them), and units that a block gets at least where items are split (2000 tokens of 8 heads, cold: 16 us
 // with two of them tokens, 18 with three, 21 with five).
 constexpr int DE_WHOLE = DECODE_ITEM + 3, DE_LEAST = DECODE_ITEM + 2;
 template <typename T, int DP>

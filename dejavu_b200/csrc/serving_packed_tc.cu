@@ -18,11 +18,15 @@
 // Few items go out in the order of falling work, many from the last sequence's last one on, back and forth over the blocks; sequences
 // may have any lengths.
 //
-// Measured (32 heads over 8, 128 dimensions, bf16): 16001 tokens 1.71 ms, 1.22 PFLOP/s, and 1.97 ms when the power cap has the clocks at
-// 1.64 GHz; 24 prompts of 16384 tokens in all 0.31 ms, 0.72 PFLOP/s. A step of an item takes about 3000 cycles, the exponentials of its two
+// The weights enter the second product as one term, rounded by half a step at most (2^-8 of a bf16 weight, 2^-11 of an fp16 one),
+// as the results are: off from 64 bits by 2.0e-3 (bf16) and 2.5e-4 (fp16) in all, where rounding the results alone makes 1.6e-3 and 2.0e-4.
+// A second term for what they lack would make the products with V twice as many: 16001 tokens 1.93 -> 3.31 ms, 24 prompts 0.33 -> 0.53.
+//
+// Measured (32 heads over 8, 128 dimensions, bf16): 16001 tokens 1.71 ms, 1.23 PFLOP/s, and 1.93 ms when the power cap has the clocks at
+// 1.61 GHz; 24 prompts of 16384 tokens in all 0.32 ms, 0.69 PFLOP/s. A step of an item takes about 3000 cycles, the exponentials of its two
 // tiles 2048 of the special units and its products 2048 of the tensor cores. What did not pay: two threads per row, exponentials by
 // polynomials, turns between the tiles, values' products that begin with half the weights, waits that spin.
-// 16 heads over 8 of 256 dimensions: 4096 tokens 0.19 ms, 0.72 PFLOP/s (27.7 ms on the CUDA cores), 16384 tokens 2.5 ms, 0.87 PFLOP/s.
+// 16 heads over 8 of 256 dimensions: 4096 tokens 0.19 ms, 0.74 PFLOP/s (5.5 on the CUDA cores), 16384 tokens 2.6 ms, 0.85 PFLOP/s.
 //
 // What a row does not see must not reach it: scores are masked by comparison, but a weight of 0 times an infinity would be NaN. So
 // entries of those value tiles that are not finite are set to 0 before the products, and joined again at the end for the rows that

@@ -10,16 +10,20 @@
 //      collected, those outside summed;
 //   4. if all that can be kept is in the list, the first block makes the rest of it alone; else the sum of what is kept, warp by warp in
 //      index order, and the place where the running sum passes u times it.
-// Rows of more ties than the list takes, and comparisons that come out closer than the weights' errors allow (one row in many
-// thousands), go to one block, which reads the row from L2 as often as it needs, narrows the range by 2048 steps of the 64-bit number at
+// Rows of more ties than the list takes, and comparisons that come out closer than the weights' errors allow (of 151936 entries with top-p 0.9 one
+// row in 700, which then takes 0.3 to 0.8 ms; of 50272 one in 15000), go to one block, which reads the row from L2 as often as it needs, narrows the range by 2048 steps of the 64-bit number at
 // a time, and has weights from exp in 64 bits: the token is that of the 64-bit definition.
+//
+// The steps lie between the largest entry and the smallest, at most 45 temperatures below it, so that ids masked by -1e4 rather than -inf make
+// them coarser, and more entries lie between the bounds. Of flat rows that can be more than the list takes: 32 rows of 151936 of a spread
+// of 0.5, top-p 0.9, take 53 us with -inf and 940 with -1e4 (top-p 0.5: 960 and 1230); with a spread of 2.5 both take 50.
 //
 // Weights: 2^(n/256) from a table, 2^f for the rest |f| <= 1/512 by its series in 32 bits, off by 1.2e-9 at most; sums have 64 bits. (32-bit
 // weights would leave every tenth row of a flat distribution undecided.) Rows whose differences two floats do not hold (a largest entry of
 // +inf, temperatures below 1e-30 or above 1e25) are left to one block too.
 //
 // A row is read once, then swept two or three times in shared memory between block and cluster barriers. One row of 50272 entries (top-k 50,
-// top-p): 14 us, a chain of barriers and fetched code; 256 rows of settings of their own: 79 us, four waves of such chains and sweeps;
+// top-p): 14 us, a chain of barriers and fetched code; 256 rows of settings of their own: 80 us, four waves of such chains and sweeps;
 // 32 rows of 151936 (top-p 0.9): 49 us, a third of it the weights and their sums. (With pairs of floats as sums, and a warp alone
 // with the share that the token is in: 88 and 65.)
 #include <math.h>
@@ -1134,7 +1138,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(SampleArgs a, int
 
 // Blocks of a row: as many as are resident at once with B rows, two to a multiprocessor (clusters stay inside a group of multiprocessors, so
 // fewer of the larger ones fit), but not so few that a slice finds no room beside another one. Slices that find none are read from L2
-// in every sweep. (256 rows of 50272 entries: 88 us with four blocks per row in four waves, 134 with one block per row and L2; 79 by now.)
+// in every sweep. (256 rows of 50272 entries: 88 us with four blocks per row in four waves, 134 with one block per row and L2; 80 by now.)
 template <typename T>
 static cudaError_t launch_sample(const SampleArgs &a, int B, bool vec, cudaStream_t st) {
   constexpr int N = Chunk<T>::N, fixed = ((int)sizeof(SampleShared) + 15) / 16 * 16, most = 200 * 1024, beside = 112 * 1024;

@@ -918,7 +918,8 @@ def paged_append(q, k, v, k_pages, v_pages, table, pos, cu_seqlens=None, freqs=N
     and k are rotated, pairs (i, i + half) or, interleaved, (2i, 2i + 1), cos and sin times amp; None: no rotation.
     Returns q rotated (T, H, D), or None without q, and with `keys` the rotated k (T, G, D), for packed_attention, else None. Rows of
     no sequence and rows at negative positions (padding of a batch) are not stored and come back as zeros. Table entries that are no
-    page are not stored to but counted (paged_faults)."""
+    page are not stored to but counted (paged_faults). Rows of a prompt that goes on from stored tokens (pos > 0) are stored, but
+    packed_attention sees no tokens of before the call, and paged_attention takes one row per sequence."""
     device = _place(k, v, q, k_pages, v_pages, table, pos, cu_seqlens, freqs)
     if device != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
@@ -991,7 +992,8 @@ def paged_faults() -> int:
 def packed_attention(q, k, v, cu_seqlens, scale: float, out=None):
     """Causal attention over whole prompts, packed row after row (djv_packed_attention): rows cu[b] .. cu[b + 1] - 1 of q (T, H, D), k
     and v (T, G, D) are sequence b, cu_seqlens (B + 1,) int32. H a multiple of G, D at most 256; any row and head strides. Returns
-    (T, H, D). Rows of no sequence are zeros or, with `out` given (T, H, D, contiguous, apart from q, k and v), left as they are."""
+    (T, H, D). Rows of no sequence are zeros or, with `out` given (T, H, D, contiguous, apart from q, k and v, at any address: one that is no
+    multiple of 16 bytes goes through a copy), left as they are."""
     device = _place(q, k, v, cu_seqlens, out)
     if device != torch._C._cuda_getDevice():
         with torch.cuda.device(device):
@@ -1047,7 +1049,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     entries that are neither -inf nor NaN, largest first and equal ones by index, the first top_k are kept (0: all), of those the
     ones in front of which less than top_p of their weight lies (1: all), of those the ones with at least min_p of the largest
     weight; weights are exp(logit / temperature). The token is the lowest index at which the running weight of what is kept exceeds
-    uniform times its total. temperature 0: the largest entry. Each setting is a number or a tensor (B,) on the device (top_k int32,
+    uniform times its total. temperature 0: the largest entry. (Entries more than 45 temperatures below the largest only count where they could
+    be taken, which is for numbers below 1e-10.) Each setting is a number or a tensor (B,) on the device (top_k int32,
     the others fp32). Returns (B,) int64, -1 for a row without entries."""
     assert logits.dim() == 2 and logits.shape[1] >= 1, f"logits (B, V), got {tuple(logits.shape)}"
     B, V = logits.shape
